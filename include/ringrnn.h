@@ -292,6 +292,90 @@ int ringrnn_assemble_trials(int n, int n_all, int T, int n0, int N, const float*
                             float* A, float* target, float* r_init, void* stream);
 
 
+/* ---- layer operators beside the recurrence (no counterpart in the reference, which compares its network with gated
+ * recurrent and transformer baselines, train/train_gru.py, train/train_causal_transformer.py) ------------------------------
+ *
+ * Element types of their tensors. */
+enum { RINGRNN_F32 = 0, RINGRNN_BF16 = 1, RINGRNN_F16 = 2 };
+
+/* A tensor [batch, token, head, width] of such elements: address and strides in elements; the last dimension is contiguous.
+ * Strides may be zero (a tensor shared by heads, say). */
+typedef struct RingRnnStrided {
+  const void* data;
+  long long batch, token, head;
+} RingRnnStrided;
+
+/* Linear attention with a decay g = exp(log_decay[h]) for each head: per sequence and head
+ *   S_t = g * S_{t-1} + k_t v_t^T        out_t = scale * S_t^T q_t        t = 0 .. length-1, S_{-1} = initial_state (or zero)
+ * the linear form of the leaky recurrence above: a state that shrinks by a fixed factor each step, is added to, and read out.
+ *   q, k [B,T,H,dk], v [B,T,H,dv] of type `dtype`;  1 <= dk, dv <= 256
+ *   log_decay [H] fp32 device, <= 0 (-infinity: nothing is kept)
+ *   lengths [B] int32 device, NULL = T each; values are clamped to 0..T.  out beyond a sequence's length is zero, and the
+ *     inputs there have no influence, whatever they hold
+ *   initial_state, final_state [B,H,dk,dv] fp32 contiguous, NULL = zero / not wanted
+ * Sums and states are held in fp32.  With fp32 and fp16 tensors all products are fp32 too.  With bf16 tensors and widths up to
+ * 128 they run on tensor cores: keys weighted by their decay and states keep sixteen bits as sums of two bf16 numbers, the
+ * weighted scores q.k are rounded to bf16. */
+typedef struct RingRnnLinearAttention {
+  int B, T, H, dk, dv;
+  int dtype; /* RINGRNN_F32 ... */
+  float scale;
+  RingRnnStrided q, k, v;
+  const float* log_decay;
+  const int* lengths;
+  const float* initial_state;
+} RingRnnLinearAttention;
+
+/* workspace bytes of the forward (backward = 0) or the backward (1); (size_t)-1 for an invalid problem; may be 0 */
+size_t ringrnn_linear_attention_bytes(const RingRnnLinearAttention* p, int backward);
+/* out [B,T,H,dv] of the problem's type, contiguous.  The workspace is 256-byte aligned. */
+int ringrnn_linear_attention_fwd(const RingRnnLinearAttention* p, void* out, float* final_state, void* workspace,
+                                 size_t workspace_bytes, void* stream);
+/* Gradients from d_out (strides as given) and d_final (fp32 [B,H,dk,dv], NULL = zero): dq, dk, dv contiguous in the problem's
+ * type, zero beyond a sequence's length; d_initial fp32 (NULL = not wanted).  Nothing is kept from the forward. */
+int ringrnn_linear_attention_bwd(const RingRnnLinearAttention* p, const RingRnnStrided* d_out, const float* d_final, void* dq,
+                                 void* dk, void* dv, float* d_initial, void* workspace, size_t workspace_bytes, void* stream);
+/* One token for each sequence: the recurrence above once, `state` [B,H,dk,dv] fp32 updated in place.  q, k, v: token stride
+ * ignored.  out [B,H,dv] contiguous.  p->T, lengths and initial_state are ignored; active: [B] bytes or NULL; a sequence whose
+ * byte is zero keeps its state and gets an output of zero.  dk <= 1024, any dv. */
+int ringrnn_linear_attention_step(const RingRnnLinearAttention* p, float* state, const unsigned char* active, void* out,
+                                  void* stream);
+
+/* Rotary positions: the first `rotated` elements of each head of q [B,T,Hq,D] and k [B,T,Hk,D] (k.data NULL: q alone) turned
+ * in pairs by position * frequency[pair], the others copied:
+ *   (y1, y2) = amplitude * (x1 cos - x2 sin, x2 cos + x1 sin)
+ *   pairs: elements (2i, 2i+1) if interleaved, else (i, i + rotated/2);  rotated even, 0 < rotated <= D
+ *   frequency [rotated/2] double, device: radians per position; angles are formed and reduced in 64 bits
+ *   positions: position_bytes 0: NULL, token t of every sequence is at `first` + t; 4 or 8: integers of that size at
+ *     positions[b*position_batch + t*position_token], to which `first` is added
+ *   inverse: turn the other way (the gradient)
+ *   q_out, k_out contiguous; they may not overlap the inputs */
+typedef struct RingRnnRotary {
+  int B, T, Hq, Hk, D, rotated;
+  int dtype;
+  int interleaved, inverse;
+  float amplitude;
+  RingRnnStrided q, k;
+  const double* frequency;
+  const void* positions;
+  int position_bytes;
+  long long position_batch, position_token, first;
+  void* q_out;
+  void* k_out;
+} RingRnnRotary;
+int ringrnn_rotary(const RingRnnRotary* p, void* stream);
+
+/* Dropout whose mask is a function of numbers, never stored:  y = residual + (kept ? x / (1 - p) : 0)  for x [rows, n]
+ * contiguous.  Element j of row r is kept iff word j mod 4 of Philox4x32-10 (key = seed, counter = {j / 4, stream_id,
+ * low and high word of first_row + r}) is at least round(p * 2^32): like the trials above, a row draws the same numbers in
+ * whatever batch it stands.  The gradient is the same call on the gradient, without the residual.
+ *   residual NULL = none;  seed_and_stream: two 64-bit device integers {seed, stream_id} read by the kernel instead of the
+ *   arguments (for captured graphs), NULL = use the arguments.  0 <= p <= 1, n <= 2^34, stream_id < 2^32.
+ *   y may be x or residual. */
+int ringrnn_dropout(int dtype, long long rows, long long n, const void* x, const void* residual, void* y, double p,
+                    unsigned long long seed, unsigned long long stream_id, const long long* seed_and_stream,
+                    unsigned long long first_row, void* stream);
+
 /* Optimizer step on flat buffers, entirely on the device: clip the gradient to a global L2 norm of `max_norm`
  * (max_norm <= 0: no clipping), then one Adam update (no weight decay, no amsgrad).  Replaces the pair
  * torch.nn.utils.clip_grad_norm_(model.parameters(), 1.0); optimizer.step() of

@@ -17,6 +17,7 @@ ERR_UNSUPPORTED = 5
 ERR_DEVICE = 6
 ERR_TOO_LARGE = 7
 STATIC_LOSS_MAX_B = 65536
+INVALID_BYTES = C.c_size_t(-1).value  # what the functions that size a buffer return for an invalid problem
 
 c_float_p = C.c_void_p
 
@@ -50,6 +51,24 @@ class TrainArgs(C.Structure):
                 ("dec_u", C.c_void_p), ("dec_v", C.c_void_p), ("grad_Wo", C.c_void_p), ("grad_Wa", C.c_void_p),
                 ("grad_J", C.c_void_p), ("loss_out", C.c_void_p), ("decoded", C.c_void_p), ("final_state", C.c_void_p),
                 ("workspace", C.c_void_p), ("workspace_bytes", C.c_size_t)]
+
+
+class Strided(C.Structure):
+    _fields_ = [("data", C.c_void_p), ("batch", C.c_longlong), ("token", C.c_longlong), ("head", C.c_longlong)]
+
+
+class LinearAttention(C.Structure):
+    _fields_ = [("B", C.c_int), ("T", C.c_int), ("H", C.c_int), ("dk", C.c_int), ("dv", C.c_int), ("dtype", C.c_int),
+                ("scale", C.c_float), ("q", Strided), ("k", Strided), ("v", Strided), ("log_decay", C.c_void_p),
+                ("lengths", C.c_void_p), ("initial_state", C.c_void_p)]
+
+
+class Rotary(C.Structure):
+    _fields_ = [("B", C.c_int), ("T", C.c_int), ("Hq", C.c_int), ("Hk", C.c_int), ("D", C.c_int), ("rotated", C.c_int),
+                ("dtype", C.c_int), ("interleaved", C.c_int), ("inverse", C.c_int), ("amplitude", C.c_float), ("q", Strided),
+                ("k", Strided), ("frequency", C.c_void_p), ("positions", C.c_void_p), ("position_bytes", C.c_int),
+                ("position_batch", C.c_longlong), ("position_token", C.c_longlong), ("first", C.c_longlong),
+                ("q_out", C.c_void_p), ("k_out", C.c_void_p)]
 
 
 # every symbol include/ringrnn.h declares: name -> (restype, argtypes)
@@ -86,6 +105,15 @@ SYMBOLS = {
                                           C.c_void_p, C.c_void_p, C.c_void_p, C.c_void_p]),
     "ringrnn_clip_adam": (C.c_int, [C.c_void_p, C.c_void_p, C.c_void_p, C.c_void_p, C.c_size_t, C.c_float, C.c_float,
                                     C.c_float, C.c_float, C.c_int, C.c_float, C.c_void_p, C.c_void_p]),
+    "ringrnn_linear_attention_bytes": (C.c_size_t, [C.POINTER(LinearAttention), C.c_int]),
+    "ringrnn_linear_attention_fwd": (C.c_int, [C.POINTER(LinearAttention), C.c_void_p, C.c_void_p, C.c_void_p, C.c_size_t,
+                                               C.c_void_p]),
+    "ringrnn_linear_attention_bwd": (C.c_int, [C.POINTER(LinearAttention), C.POINTER(Strided), C.c_void_p, C.c_void_p,
+                                               C.c_void_p, C.c_void_p, C.c_void_p, C.c_void_p, C.c_size_t, C.c_void_p]),
+    "ringrnn_linear_attention_step": (C.c_int, [C.POINTER(LinearAttention), C.c_void_p, C.c_void_p, C.c_void_p, C.c_void_p]),
+    "ringrnn_rotary": (C.c_int, [C.POINTER(Rotary), C.c_void_p]),
+    "ringrnn_dropout": (C.c_int, [C.c_int, C.c_longlong, C.c_longlong, C.c_void_p, C.c_void_p, C.c_void_p, C.c_double,
+                                  C.c_ulonglong, C.c_ulonglong, C.c_void_p, C.c_ulonglong, C.c_void_p]),
     "ringrnn_device_status": (C.c_int, [C.POINTER(C.c_int)]),
     "ringrnn_last_device_code": (C.c_int, []),
     "ringrnn_selftest_wait": (C.c_int, [C.c_longlong, C.c_int, C.c_void_p, C.c_void_p]),

@@ -158,6 +158,12 @@ static int take_device_status() {
   return code;
 }
 static thread_local int g_last_device_code = 0;
+int earlier_failure() {
+  const int code = take_device_status();
+  if (code == 0) return RINGRNN_OK;
+  g_last_device_code = code;
+  return RINGRNN_ERR_DEVICE;
+}
 
 namespace {
 
@@ -386,7 +392,7 @@ extern "C" int ringrnn_last_device_code(void) { return g_last_device_code; }
 extern "C" long long ringrnn_launch_count(void) { return g_launches.load(); }
 extern "C" int ringrnn_timing_slots(void) { return K_SLOTS; }
 extern "C" const char* ringrnn_timing_name(int slot) {
-  static const char* names[K_SLOTS] = {"prep", "fwd_recurrent", "bwd_recurrent", "dw_product", "dw_reduce", "loss"};
+  static const char* names[K_SLOTS] = {"prep", "fwd_recurrent", "bwd_recurrent", "dw_product", "dw_reduce", "loss", "layer"};
   return (slot >= 0 && slot < K_SLOTS) ? names[slot] : "";
 }
 extern "C" int ringrnn_timing_enable(int on) {

@@ -25,7 +25,7 @@ void set_last_cuda_error(cudaError_t e);
   } while (0)
 
 // ---- launch accounting / optional per-kernel event timing ---------------------------------
-enum KernelSlot { K_PREP = 0, K_FWD = 1, K_BWD = 2, K_DW = 3, K_REDUCE = 4, K_LOSS = 5, K_SLOTS = 6 };
+enum KernelSlot { K_PREP = 0, K_FWD = 1, K_BWD = 2, K_DW = 3, K_REDUCE = 4, K_LOSS = 5, K_LAYER = 6, K_SLOTS = 7 };
 // Construct right before a kernel launch and let it go out of scope right after: counts the launch and,
 // when timing is enabled, records an event pair around it on `s`.
 struct LaunchScope {
@@ -94,6 +94,9 @@ int queue_status_report(const int* dev_status, cudaStream_t s);
 // The same without a copy behind every launch: a pinned host word, one for the process, that the thread which abandons a wait
 // writes itself.  Which launches give up together is still decided by the status word of their call.
 int host_status_word(volatile int** out);
+
+// RINGRNN_ERR_DEVICE, once, if an earlier launch abandoned a bounded wait: what an entry point whose kernels wait asks first.
+int earlier_failure();
 
 // dJ0 / dJ1 from the unscaled Wo gradient (ringrnn_fp32.cu); scratch: GRAD_J_BLOCKS * 2 doubles
 constexpr int GRAD_J_BLOCKS = 128;

@@ -1,0 +1,485 @@
+// Linear attention with decay: entry points, the fp32-arithmetic kernel, the scan over segments, and the single-token step.
+#include <string.h>
+
+#include "element.cuh"
+#include "linear_attention.cuh"
+
+namespace ringrnn {
+namespace {
+
+// ---- fp32 arithmetic: any type, any width up to 256 -----------------------------------------------------------------
+// One CTA per (job, sequence, head, segment) and slice of 64 outer columns, whose part of the state lives in shared memory
+// for the whole segment.  Chunks of 32 tokens: of 16, 32 and 64, 32 has the fewest products per token next to the state's own
+// 2 * inner * 64 (64 for the pairs' scores and 64 for their values) that still leave two CTAs per SM their shared memory.
+constexpr int PC = 32, PO = 64, P_THREADS = 256, P_LD = PC + 4;
+
+__host__ __device__ constexpr int plain_row(int inner) { return (inner + 3) / 4 * 4 + 4; }  // +4: rows a bank group apart
+size_t plain_smem(int inner) {
+  return sizeof(float) * (2 * PC * plain_row(inner) + PC * PO + PC * P_LD + 2 * PC + (size_t)(plain_row(inner) - 4) * PO);
+}
+
+template <class E, bool STATES>
+__global__ void __launch_bounds__(P_THREADS) la_plain_kernel(const __grid_constant__ LaLaunch L) {
+  extern __shared__ float sm[];
+  const int tid = threadIdx.x;
+  const int ji = (int)(blockIdx.x % L.jobs);
+  const LaJob& J = L.job[ji];
+  const int at = (int)(blockIdx.x / L.jobs), seg = at % L.segments, bh = at / L.segments, h = bh % L.H, b = bh / L.H;
+  const int o0 = blockIdx.y * PO;
+  if (o0 >= J.outer) return;
+  const int I = J.inner, IP = plain_row(I) - 4, ld = IP + 4, on = min(PO, J.outer - o0);
+  float* Q = sm;               // [PC][ld]
+  float* K = Q + PC * ld;      // [PC][ld]
+  float* V = K + PC * ld;      // [PC][PO]
+  float* P = V + PC * PO;      // [PC][P_LD]
+  float* wk = P + PC * P_LD;   // [PC] factor of a key in the state
+  float* wr = wk + PC;         // [PC] factor of the state in a row
+  float* S = wr + PC;          // [IP][PO]
+  const LaDecay g(L.log_decay[h]);
+  const int len = la_length(L, b);
+  const int begin = seg * L.segment_tokens, stop = min(L.T, begin + L.segment_tokens), end = min(len, stop);
+  const size_t mat = (size_t)at * J.inner * J.outer;
+
+  for (int e = tid; e < IP * PO; e += P_THREADS) {
+    const int i = e / PO, o = e % PO;
+    S[e] = (!STATES && J.init != nullptr && i < I && o < on) ? J.init[mat + (size_t)i * J.s_in + (size_t)(o0 + o) * J.s_out] : 0.f;
+  }
+  const E* q = static_cast<const E*>(J.q.p) + b * J.q.sb + h * J.q.sh;
+  const E* k = static_cast<const E*>(J.k.p) + b * J.k.sb + h * J.k.sh;
+  const E* v = static_cast<const E*>(J.v.p) + b * J.v.sb + h * J.v.sh + o0;
+  E* out = static_cast<E*>(J.out);
+
+  const int chunks = end > begin ? (end - begin + PC - 1) / PC : 0;
+  const LaFactor whole(L.log_decay[h], PC);
+  for (int c = 0; c < chunks; ++c) {
+    const int t0 = begin + (J.reverse ? chunks - 1 - c : c) * PC, n = min(PC, end - t0);
+    __syncthreads();
+    for (int e = tid; e < PC * IP; e += P_THREADS) {
+      const int r = e / IP, i = e - r * IP;
+      const bool in = r < n && i < I;
+      if (!STATES) Q[r * ld + i] = in ? up(q[(t0 + r) * J.q.st + i]) : 0.f;
+      K[r * ld + i] = in ? up(k[(t0 + r) * J.k.st + i]) : 0.f;
+    }
+    for (int e = tid; e < PC * PO; e += P_THREADS) {
+      const int r = e / PO, o = e % PO;
+      V[e] = (r < n && o < on) ? up(v[(t0 + r) * J.v.st + o]) : 0.f;
+    }
+    if (tid < PC) wk[tid] = tid < n ? J.key_scale * g.power(J.reverse ? tid + 1 : n - 1 - tid) : 0.f;
+    else if (tid < 2 * PC) {
+      const int r = tid - PC;
+      wr[r] = r < n ? J.row_scale * g.power(J.reverse ? n - 1 - r : r + 1) : 0.f;
+    }
+    __syncthreads();
+    if (!STATES) {
+      // scores of a row with four keys, eight apart: consecutive threads read consecutive rows of K
+      {
+        const int i = tid >> 3, j0 = tid & 7;
+        float acc[4] = {0.f, 0.f, 0.f, 0.f};
+        for (int d = 0; d < IP; d += 4) {
+          const float4 x = *reinterpret_cast<const float4*>(Q + i * ld + d);
+#pragma unroll
+          for (int m = 0; m < 4; ++m) {
+            const float4 y = *reinterpret_cast<const float4*>(K + (j0 + 8 * m) * ld + d);
+            acc[m] = fmaf(x.x, y.x, fmaf(x.y, y.y, fmaf(x.z, y.z, fmaf(x.w, y.w, acc[m]))));
+          }
+        }
+#pragma unroll
+        for (int m = 0; m < 4; ++m) {
+          const int j = j0 + 8 * m, far = J.reverse ? j - i : i - j;
+          P[i * P_LD + j] = (far >= 0 && i < n && j < n) ? acc[m] * J.pair_scale * g.power(far) : 0.f;
+        }
+      }
+      __syncthreads();
+      // two rows by four columns: the state's part, then the pairs'
+      {
+        const int r = (tid >> 4) * 2, o = (tid & 15) * 4;
+        float4 a0 = make_float4(0.f, 0.f, 0.f, 0.f), a1 = a0;
+        auto add = [](float4& a, float x, const float4& y) {
+          a.x = fmaf(x, y.x, a.x); a.y = fmaf(x, y.y, a.y); a.z = fmaf(x, y.z, a.z); a.w = fmaf(x, y.w, a.w);
+        };
+        for (int d = 0; d < IP; d += 4) {
+          const float4 x0 = *reinterpret_cast<const float4*>(Q + r * ld + d), x1 = *reinterpret_cast<const float4*>(Q + (r + 1) * ld + d);
+          const float4* s4 = reinterpret_cast<const float4*>(S + d * PO + o);
+          const float4 y0 = s4[0], y1 = s4[PO / 4], y2 = s4[PO / 2], y3 = s4[3 * PO / 4];
+          add(a0, x0.x, y0); add(a0, x0.y, y1); add(a0, x0.z, y2); add(a0, x0.w, y3);
+          add(a1, x1.x, y0); add(a1, x1.y, y1); add(a1, x1.z, y2); add(a1, x1.w, y3);
+        }
+        const float w0 = wr[r], w1 = wr[r + 1];
+        a0.x *= w0; a0.y *= w0; a0.z *= w0; a0.w *= w0;
+        a1.x *= w1; a1.y *= w1; a1.z *= w1; a1.w *= w1;
+        for (int j = 0; j < PC; j += 4) {
+          const float4 p0 = *reinterpret_cast<const float4*>(P + r * P_LD + j), p1 = *reinterpret_cast<const float4*>(P + (r + 1) * P_LD + j);
+          const float4* v4 = reinterpret_cast<const float4*>(V + j * PO + o);
+          const float4 y0 = v4[0], y1 = v4[PO / 4], y2 = v4[PO / 2], y3 = v4[3 * PO / 4];
+          add(a0, p0.x, y0); add(a0, p0.y, y1); add(a0, p0.z, y2); add(a0, p0.w, y3);
+          add(a1, p1.x, y0); add(a1, p1.y, y1); add(a1, p1.z, y2); add(a1, p1.w, y3);
+        }
+        const float w[2][4] = {{a0.x, a0.y, a0.z, a0.w}, {a1.x, a1.y, a1.z, a1.w}};
+#pragma unroll
+        for (int m = 0; m < 2; ++m)
+#pragma unroll
+          for (int e = 0; e < 4; ++e)
+            if (r + m < n && o + e < on)
+              out[(((size_t)b * L.T + t0 + r + m) * L.H + h) * J.outer + o0 + o + e] = down<E>(w[m][e]);
+      }
+      __syncthreads();
+    }
+    // the state: blocks of 4 x 4, two of them per thread at a time where the width has that many
+    {
+      const LaFactor gn = n == PC ? whole : LaFactor(L.log_decay[h], n);
+      const int o = (tid & 15) * 4, d0 = (tid >> 4) * 4;
+      for (int d = d0; d < IP; d += 128) {
+        const bool two = d + 64 < IP;
+        float acc[8][4];
+#pragma unroll
+        for (int m = 0; m < 8; ++m)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) acc[m][e] = 0.f;
+        for (int r = 0; r < n; ++r) {
+          const float w = wk[r];
+          float4 y = *reinterpret_cast<const float4*>(V + r * PO + o);
+          y.x *= w; y.y *= w; y.z *= w; y.w *= w;
+          const float4 x = *reinterpret_cast<const float4*>(K + r * ld + d);
+          const float4 z = two ? *reinterpret_cast<const float4*>(K + r * ld + d + 64) : make_float4(0.f, 0.f, 0.f, 0.f);
+          const float xs[8] = {x.x, x.y, x.z, x.w, z.x, z.y, z.z, z.w};
+#pragma unroll
+          for (int m = 0; m < 8; ++m) {
+            acc[m][0] = fmaf(xs[m], y.x, acc[m][0]); acc[m][1] = fmaf(xs[m], y.y, acc[m][1]);
+            acc[m][2] = fmaf(xs[m], y.z, acc[m][2]); acc[m][3] = fmaf(xs[m], y.w, acc[m][3]);
+          }
+        }
+#pragma unroll
+        for (int m = 0; m < 8; ++m) {
+          if (m >= 4 && !two) break;
+          float4* s4 = reinterpret_cast<float4*>(S + (d + (m & 3) + (m >> 2) * 64) * PO + o);
+          float4 x = *s4;
+          x.x = gn.times(x.x, acc[m][0]); x.y = gn.times(x.y, acc[m][1]);
+          x.z = gn.times(x.z, acc[m][2]); x.w = gn.times(x.w, acc[m][3]);
+          *s4 = x;
+        }
+      }
+    }
+  }
+  __syncthreads();
+  if (!STATES) {  // rows behind the sequence
+    const int first = max(begin, end), rows = stop - first;
+    for (int e = tid; e < rows * on; e += P_THREADS)
+      out[(((size_t)b * L.T + first + e / on) * L.H + h) * J.outer + o0 + e % on] = down<E>(0.f);
+  }
+  if (J.fin != nullptr)
+    for (int e = tid; e < I * PO; e += P_THREADS) {
+      const int i = e / PO, o = e % PO;
+      if (o < on) J.fin[mat + (size_t)i * J.s_in + (size_t)(o0 + o) * J.s_out] = S[e];
+    }
+}
+
+template <class E, bool STATES>
+int plain_launch(const LaLaunch& L, cudaStream_t s) {
+  int inner = 0, outer = 0;
+  for (int j = 0; j < L.jobs; ++j) {
+    inner = L.job[j].inner > inner ? L.job[j].inner : inner;
+    outer = L.job[j].outer > outer ? L.job[j].outer : outer;
+  }
+  const size_t smem = plain_smem(inner);
+  RINGRNN_CUDA_TRY(cudaFuncSetAttribute(la_plain_kernel<E, STATES>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)plain_smem(256)));
+  const dim3 grid((unsigned)(L.B * L.H * L.segments * L.jobs), (unsigned)((outer + PO - 1) / PO));
+  LaunchScope ls(K_LAYER, s);
+  la_plain_kernel<E, STATES><<<grid, P_THREADS, smem, s>>>(L);
+  RINGRNN_CUDA_TRY(cudaGetLastError());
+  return RINGRNN_OK;
+}
+template <bool STATES>
+int plain_launch(int dtype, const LaLaunch& L, cudaStream_t s) {
+  return dtype == RINGRNN_F32    ? plain_launch<float, STATES>(L, s)
+         : dtype == RINGRNN_BF16 ? plain_launch<__nv_bfloat16, STATES>(L, s)
+                                 : plain_launch<__half, STATES>(L, s);
+}
+
+// ---- scan over segments -----------------------------------------------------------------------------------------------
+// sums[bh][segment][elems] (each segment's own sum) becomes the state it starts from, in place; `last`: the state behind all
+// of them.  A thread owns one element; eight segments are in flight at a time.
+__global__ void __launch_bounds__(256) la_scan_kernel(int B, int T, int H, int segments, int segment_tokens, int elems,
+                                                      int reverse, const float* log_decay, const int* lengths,
+                                                      const float* init, float* sums, float* last) {
+  const int bh = blockIdx.x, b = bh / H, e = blockIdx.y * 256 + threadIdx.x;
+  if (e >= elems) return;
+  const LaFactor whole(log_decay[bh % H], segment_tokens);
+  int len = lengths == nullptr ? T : lengths[b];
+  len = len < 0 ? 0 : len > T ? T : len;
+  float x = init != nullptr ? init[(size_t)bh * elems + e] : 0.f;
+  float* u = sums + (size_t)bh * segments * elems + e;
+  constexpr int AHEAD = 8;
+  for (int j0 = 0; j0 < segments; j0 += AHEAD) {
+    float y[AHEAD];
+#pragma unroll
+    for (int a = 0; a < AHEAD; ++a) {
+      const int j = reverse ? segments - 1 - (j0 + a) : j0 + a;
+      y[a] = j0 + a < segments ? u[(size_t)j * elems] : 0.f;
+    }
+#pragma unroll
+    for (int a = 0; a < AHEAD; ++a) {
+      if (j0 + a >= segments) break;
+      const int j = reverse ? segments - 1 - (j0 + a) : j0 + a;
+      int n = len - j * segment_tokens;
+      n = n < 0 ? 0 : n > segment_tokens ? segment_tokens : n;
+      u[(size_t)j * elems] = x;
+      x = (n == segment_tokens ? whole : LaFactor(log_decay[bh % H], n)).times(x, y[a]);
+    }
+  }
+  if (last != nullptr) last[(size_t)bh * elems + e] = x;
+}
+int scan_launch(const LaLaunch& L, int elems, int reverse, const float* init, float* sums, float* last, cudaStream_t s) {
+  LaunchScope ls(K_LAYER, s);
+  la_scan_kernel<<<dim3(L.B * L.H, (elems + 255) / 256), 256, 0, s>>>(L.B, L.T, L.H, L.segments, L.segment_tokens, elems, reverse,
+                                                                     L.log_decay, L.lengths, init, sums, last);
+  RINGRNN_CUDA_TRY(cudaGetLastError());
+  return RINGRNN_OK;
+}
+
+// ---- one token ----------------------------------------------------------------------------------------------------------
+// Bound by the state, read and written once: 8 * dk * dv bytes per sequence and head.  A CTA takes 32 columns of one state:
+// they are independent of one another, a single head then spreads over dv / 32 SMs, and a row's part is a whole 128-byte line.
+// VEC = 4: a thread owns 4 columns of every 32nd row; VEC = 1 (odd widths or addresses): 1 column of every 8th.
+constexpr int STEP_THREADS = 256, STEP_COLS = 32, STEP_MAX_DK = 1024;
+template <class E, int VEC>
+__global__ void __launch_bounds__(STEP_THREADS) la_step_kernel(int H, int dk, int dv, float scale, LaOperand q, LaOperand k,
+                                                               LaOperand v, const float* __restrict__ log_decay,
+                                                               const unsigned char* __restrict__ active,
+                                                               float* __restrict__ state, E* __restrict__ out) {
+  constexpr int CG = STEP_COLS / VEC, ROWS = STEP_THREADS / CG;
+  __shared__ float sq[STEP_MAX_DK], sk[STEP_MAX_DK];
+  __shared__ float part[ROWS][STEP_COLS];
+  const int tid = threadIdx.x, bh = blockIdx.x, h = bh % H, b = bh / H;
+  const int cg = tid % CG, row = tid / CG, col = blockIdx.y * STEP_COLS + cg * VEC;
+  if (active != nullptr && active[b] == 0) {
+    if (row == 0)
+      for (int e = 0; e < VEC; ++e)
+        if (col + e < dv) out[(size_t)bh * dv + col + e] = down<E>(0.f);
+    return;
+  }
+  const bool in = col < dv;  // VEC == 4: dv is a multiple of 4
+  float* S = state + (size_t)bh * dk * dv + col;
+  // the state's first rows are under way while q and k come in
+  constexpr int AHEAD = VEC == 4 ? 4 : 8;
+  float s0[AHEAD][VEC];
+  auto fetch = [&](float* x, int i) {
+    if constexpr (VEC == 4) {
+      const float4 y = *reinterpret_cast<const float4*>(S + (size_t)i * dv);
+      x[0] = y.x; x[1] = y.y; x[2] = y.z; x[3] = y.w;
+    } else {
+      x[0] = S[(size_t)i * dv];
+    }
+  };
+#pragma unroll
+  for (int a = 0; a < AHEAD; ++a)
+    if (in && row + a * ROWS < dk) fetch(s0[a], row + a * ROWS);
+  const E* qp = static_cast<const E*>(q.p) + b * q.sb + h * q.sh;
+  const E* kp = static_cast<const E*>(k.p) + b * k.sb + h * k.sh;
+  const E* vp = static_cast<const E*>(v.p) + b * v.sb + h * v.sh;
+  for (int i = tid; i < dk; i += STEP_THREADS) {
+    sq[i] = up(qp[i]);
+    sk[i] = up(kp[i]);
+  }
+  const float g = expf(log_decay[h]);
+  float vv[VEC], acc[VEC];
+#pragma unroll
+  for (int e = 0; e < VEC; ++e) {
+    vv[e] = in ? up(vp[col + e]) : 0.f;
+    acc[e] = 0.f;
+  }
+  __syncthreads();
+  if (in) {
+    for (int i0 = row; i0 < dk; i0 += AHEAD * ROWS) {
+#pragma unroll
+      for (int a = 0; a < AHEAD; ++a) {
+        const int i = i0 + a * ROWS;
+        if (i >= dk) break;
+        const float kk = sk[i], qq = sq[i];
+#pragma unroll
+        for (int e = 0; e < VEC; ++e) {
+          s0[a][e] = fmaf(g, s0[a][e], kk * vv[e]);
+          acc[e] = fmaf(qq, s0[a][e], acc[e]);
+        }
+        if constexpr (VEC == 4) *reinterpret_cast<float4*>(S + (size_t)i * dv) = make_float4(s0[a][0], s0[a][1], s0[a][2], s0[a][3]);
+        else S[(size_t)i * dv] = s0[a][0];
+      }
+#pragma unroll
+      for (int a = 0; a < AHEAD; ++a)
+        if (i0 + (AHEAD + a) * ROWS < dk) fetch(s0[a], i0 + (AHEAD + a) * ROWS);
+    }
+  }
+#pragma unroll
+  for (int e = 0; e < VEC; ++e) part[row][cg * VEC + e] = acc[e];
+  __syncthreads();
+  if (tid < STEP_COLS && blockIdx.y * STEP_COLS + tid < dv) {
+    float x = 0.f;
+#pragma unroll 8
+    for (int r = 0; r < ROWS; ++r) x += part[r][tid];
+    out[(size_t)bh * dv + blockIdx.y * STEP_COLS + tid] = down<E>(scale * x);
+  }
+}
+template <class E>
+int step_launch(const RingRnnLinearAttention& p, const LaOperand& q, const LaOperand& k, const LaOperand& v, float* state,
+                const unsigned char* active, void* out, cudaStream_t s) {
+  const dim3 grid(p.B * p.H, (p.dv + STEP_COLS - 1) / STEP_COLS);
+  LaunchScope ls(K_LAYER, s);
+  if (p.dv % 4 == 0 && (reinterpret_cast<uintptr_t>(state) & 15) == 0)
+    la_step_kernel<E, 4><<<grid, STEP_THREADS, 0, s>>>(p.H, p.dk, p.dv, p.scale, q, k, v, p.log_decay, active, state, static_cast<E*>(out));
+  else
+    la_step_kernel<E, 1><<<grid, STEP_THREADS, 0, s>>>(p.H, p.dk, p.dv, p.scale, q, k, v, p.log_decay, active, state, static_cast<E*>(out));
+  RINGRNN_CUDA_TRY(cudaGetLastError());
+  return RINGRNN_OK;
+}
+
+// ---- host -----------------------------------------------------------------------------------------------------------------
+int check_linear(const RingRnnLinearAttention& p, bool step) {
+  if (p.B <= 0 || p.H <= 0 || p.dk <= 0 || p.dv <= 0 || (!step && p.T <= 0)) return RINGRNN_ERR_SHAPE;
+  if (step ? p.dk > STEP_MAX_DK : p.dk > 256 || p.dv > 256) return RINGRNN_ERR_SHAPE;
+  // grid sizes (segments times jobs is at most 3 where there are that many heads)
+  if ((long long)p.B * p.H > (1 << 29) || (step && (p.dv + STEP_COLS - 1) / STEP_COLS > 65535)) return RINGRNN_ERR_SHAPE;
+  if (!step && p.T > (1 << 30)) return RINGRNN_ERR_SHAPE;
+  if (p.dtype != RINGRNN_F32 && p.dtype != RINGRNN_BF16 && p.dtype != RINGRNN_F16) return RINGRNN_ERR_ARG;
+  return RINGRNN_OK;
+}
+LaOperand operand(const RingRnnStrided& t) { return LaOperand{t.data, t.batch, t.token, t.head}; }
+
+// How a call runs: chunk and segments.
+struct Plan {
+  int segments, segment_tokens;
+  size_t sums;   // floats per set of segment sums
+  size_t bytes;  // whole workspace
+};
+
+// Segments: as many as fill the GPU, if a sequence's share of the work is then still a few chunks.  Forming the sums first reads
+// keys and values once more, about half of a forward's work, so cutting has to at least double the number of CTAs at work.
+Plan make_plan(const RingRnnLinearAttention& p, int backward) {
+  Plan l;
+  const int chunk = PC, least = 8 * chunk;
+  const long long ctas = (long long)p.B * p.H * (backward ? 3 : 1) * ((p.dv + PO - 1) / PO);
+  long long n = 296 / ctas;
+  const long long most = (p.T + least - 1) / least;
+  n = n > most ? most : n;
+  if (n < 2) n = 1;
+  l.segment_tokens = (int)(((p.T + n - 1) / n + chunk - 1) / chunk * chunk);
+  l.segments = (p.T + l.segment_tokens - 1) / l.segment_tokens;
+  l.sums = l.segments > 1 ? (size_t)p.B * p.H * l.segments * p.dk * p.dv : 0;
+  l.bytes = align_up(l.sums * sizeof(float), 256) * (backward ? 2 : 1);
+  return l;
+}
+
+LaLaunch base_launch(const RingRnnLinearAttention& p, const Plan& l) {
+  LaLaunch L;
+  memset(&L, 0, sizeof(L));
+  L.B = p.B; L.T = p.T; L.H = p.H;
+  L.segments = l.segments; L.segment_tokens = l.segment_tokens;
+  L.log_decay = p.log_decay; L.lengths = p.lengths;
+  return L;
+}
+int check_workspace(const Plan& l, const void* workspace, size_t bytes) {
+  if (l.bytes == 0) return RINGRNN_OK;
+  return workspace == nullptr || bytes < l.bytes || (reinterpret_cast<uintptr_t>(workspace) & 255) != 0 ? RINGRNN_ERR_WORKSPACE : RINGRNN_OK;
+}
+
+}  // namespace
+}  // namespace ringrnn
+
+using namespace ringrnn;
+
+extern "C" size_t ringrnn_linear_attention_bytes(const RingRnnLinearAttention* p, int backward) {
+  if (p == nullptr || check_linear(*p, false) != RINGRNN_OK) return (size_t)-1;
+  return make_plan(*p, backward).bytes;
+}
+
+extern "C" int ringrnn_linear_attention_fwd(const RingRnnLinearAttention* p, void* out, float* final_state, void* workspace,
+                                            size_t workspace_bytes, void* stream) {
+  if (p == nullptr) return RINGRNN_ERR_ARG;
+  int rc = check_linear(*p, false);
+  if (rc != RINGRNN_OK) return rc;
+  if (!p->q.data || !p->k.data || !p->v.data || !p->log_decay || !out) return RINGRNN_ERR_ARG;
+  const Plan l = make_plan(*p, 0);
+  rc = check_workspace(l, workspace, workspace_bytes);
+  if (rc != RINGRNN_OK) return rc;
+  cudaStream_t s = static_cast<cudaStream_t>(stream);
+  LaLaunch L = base_launch(*p, l);
+  float* sums = static_cast<float*>(workspace);
+  L.jobs = 1;
+  LaJob& j = L.job[0];
+  j.q = operand(p->q); j.k = operand(p->k); j.v = operand(p->v);
+  j.out = out;
+  j.inner = p->dk; j.outer = p->dv;
+  j.pair_scale = j.row_scale = p->scale;
+  j.key_scale = 1.f;
+  j.s_in = p->dv; j.s_out = 1;
+  if (l.segments > 1) {
+    j.fin = sums;
+    rc = plain_launch<true>(p->dtype, L, s);
+    if (rc == RINGRNN_OK) rc = scan_launch(L, p->dk * p->dv, 0, p->initial_state, sums, final_state, s);
+    if (rc != RINGRNN_OK) return rc;
+    j.init = sums;
+    j.fin = nullptr;
+  } else {
+    j.init = p->initial_state;
+    j.fin = final_state;
+  }
+  return plain_launch<false>(p->dtype, L, s);
+}
+
+extern "C" int ringrnn_linear_attention_bwd(const RingRnnLinearAttention* p, const RingRnnStrided* d_out, const float* d_final,
+                                            void* dq, void* dk, void* dv, float* d_initial, void* workspace,
+                                            size_t workspace_bytes, void* stream) {
+  if (p == nullptr || d_out == nullptr) return RINGRNN_ERR_ARG;
+  int rc = check_linear(*p, false);
+  if (rc != RINGRNN_OK) return rc;
+  if (!p->q.data || !p->k.data || !p->v.data || !p->log_decay || !d_out->data || !dq || !dk || !dv) return RINGRNN_ERR_ARG;
+  const Plan l = make_plan(*p, 1);
+  rc = check_workspace(l, workspace, workspace_bytes);
+  if (rc != RINGRNN_OK) return rc;
+  cudaStream_t s = static_cast<cudaStream_t>(stream);
+  const LaOperand q = operand(p->q), k = operand(p->k), v = operand(p->v), g = operand(*d_out);
+  LaLaunch L = base_launch(*p, l);
+  L.jobs = 3;
+  LaJob &jq = L.job[0], &jk = L.job[1], &jv = L.job[2];
+  jq.q = g; jq.k = v; jq.v = k; jq.out = dq;
+  jk.q = v; jk.k = g; jk.v = q; jk.out = dk;
+  jv.q = k; jv.k = q; jv.v = g; jv.out = dv;
+  jq.inner = jk.inner = p->dv; jq.outer = jk.outer = p->dk;
+  jv.inner = p->dk; jv.outer = p->dv;
+  jk.reverse = jv.reverse = 1;
+  jq.pair_scale = jk.pair_scale = jv.pair_scale = p->scale;
+  jq.row_scale = p->scale; jq.key_scale = 1.f;
+  jk.row_scale = jv.row_scale = 1.f; jk.key_scale = jv.key_scale = p->scale;
+  jq.s_in = jk.s_in = 1; jq.s_out = jk.s_out = p->dv;  // states are kept as [dk][dv]
+  jv.s_in = p->dv; jv.s_out = 1;
+  if (l.segments > 1) {
+    float* S = static_cast<float*>(workspace);
+    float* E = reinterpret_cast<float*>(static_cast<char*>(workspace) + align_up(l.sums * sizeof(float), 256));
+    LaLaunch M = L;
+    M.jobs = 2;
+    M.job[0] = jq; M.job[0].fin = S;
+    M.job[1] = jv; M.job[1].fin = E;
+    rc = plain_launch<true>(p->dtype, M, s);
+    if (rc == RINGRNN_OK) rc = scan_launch(L, p->dk * p->dv, 0, p->initial_state, S, nullptr, s);
+    if (rc == RINGRNN_OK) rc = scan_launch(L, p->dk * p->dv, 1, d_final, E, d_initial, s);
+    if (rc != RINGRNN_OK) return rc;
+    jq.init = S;
+    jk.init = jv.init = E;
+  } else {
+    jq.init = p->initial_state;
+    jk.init = jv.init = d_final;
+    jv.fin = d_initial;
+  }
+  return plain_launch<false>(p->dtype, L, s);
+}
+
+extern "C" int ringrnn_linear_attention_step(const RingRnnLinearAttention* p, float* state, const unsigned char* active, void* out,
+                                             void* stream) {
+  if (p == nullptr) return RINGRNN_ERR_ARG;
+  const int rc = check_linear(*p, true);
+  if (rc != RINGRNN_OK) return rc;
+  if (!p->q.data || !p->k.data || !p->v.data || !p->log_decay || !out || !state) return RINGRNN_ERR_ARG;
+  cudaStream_t s = static_cast<cudaStream_t>(stream);
+  const LaOperand q = operand(p->q), k = operand(p->k), v = operand(p->v);
+  return p->dtype == RINGRNN_F32    ? step_launch<float>(*p, q, k, v, state, active, out, s)
+         : p->dtype == RINGRNN_BF16 ? step_launch<__nv_bfloat16>(*p, q, k, v, state, active, out, s)
+                                    : step_launch<__half>(*p, q, k, v, state, active, out, s);
+}
