@@ -326,8 +326,8 @@ typedef struct RingRnnLinearAttention {
   const float* initial_state;
 } RingRnnLinearAttention;
 
-/* workspace bytes of the forward (backward = 0) or the backward (1); (size_t)-1 for an invalid problem; may be 0 */
-size_t ringrnn_linear_attention_bytes(const RingRnnLinearAttention* p, int backward);
+/* workspace bytes of the forward (d_out NULL) or of the backward with that d_out; (size_t)-1 for an invalid problem; may be 0 */
+size_t ringrnn_linear_attention_bytes(const RingRnnLinearAttention* p, const RingRnnStrided* d_out);
 /* out [B,T,H,dv] of the problem's type, contiguous.  The workspace is 256-byte aligned. */
 int ringrnn_linear_attention_fwd(const RingRnnLinearAttention* p, void* out, float* final_state, void* workspace,
                                  size_t workspace_bytes, void* stream);

@@ -105,7 +105,7 @@ SYMBOLS = {
                                           C.c_void_p, C.c_void_p, C.c_void_p, C.c_void_p]),
     "ringrnn_clip_adam": (C.c_int, [C.c_void_p, C.c_void_p, C.c_void_p, C.c_void_p, C.c_size_t, C.c_float, C.c_float,
                                     C.c_float, C.c_float, C.c_int, C.c_float, C.c_void_p, C.c_void_p]),
-    "ringrnn_linear_attention_bytes": (C.c_size_t, [C.POINTER(LinearAttention), C.c_int]),
+    "ringrnn_linear_attention_bytes": (C.c_size_t, [C.POINTER(LinearAttention), C.POINTER(Strided)]),
     "ringrnn_linear_attention_fwd": (C.c_int, [C.POINTER(LinearAttention), C.c_void_p, C.c_void_p, C.c_void_p, C.c_size_t,
                                                C.c_void_p]),
     "ringrnn_linear_attention_bwd": (C.c_int, [C.POINTER(LinearAttention), C.POINTER(Strided), C.c_void_p, C.c_void_p,

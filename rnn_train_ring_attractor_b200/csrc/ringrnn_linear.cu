@@ -343,28 +343,104 @@ int check_linear(const RingRnnLinearAttention& p, bool step) {
 }
 LaOperand operand(const RingRnnStrided& t) { return LaOperand{t.data, t.batch, t.token, t.head}; }
 
-// How a call runs: chunk and segments.
+// ---- operands for the tensor cores ------------------------------------------------------------------------------------
+// A tensor that TMA cannot read as it is (a stride or an address that is not a multiple of 16 bytes, tokens that share a row)
+// is copied to rows of a multiple of 8 elements first.
+struct PackJobs {
+  LaOperand from[4];
+  __nv_bfloat16* to[4];
+  int width[4], padded[4];
+};
+__global__ void __launch_bounds__(256) la_pack_kernel(const __grid_constant__ PackJobs p, int B, int T, int H) {
+  const int j = blockIdx.y, width = p.width[j], per = p.padded[j] / 8;
+  const LaOperand o = p.from[j];
+  const size_t total = (size_t)B * T * H * per;
+  for (size_t id = blockIdx.x * (size_t)256 + threadIdx.x; id < total; id += (size_t)gridDim.x * 256) {
+    const size_t row = id / per;
+    const int i0 = (int)(id - row * per) * 8, h = (int)(row % H);
+    const size_t bt = row / H;
+    const int t = (int)(bt % T), b = (int)(bt / T);
+    const unsigned short* x = static_cast<const unsigned short*>(o.p) + b * o.sb + t * o.st + h * o.sh + i0;
+    unsigned short y[8];
+#pragma unroll
+    for (int e = 0; e < 8; ++e) y[e] = i0 + e < width ? x[e] : (unsigned short)0;
+    reinterpret_cast<uint4*>(p.to[j])[id] = make_uint4(y[0] | (uint32_t)y[1] << 16, y[2] | (uint32_t)y[3] << 16,
+                                                       y[4] | (uint32_t)y[5] << 16, y[6] | (uint32_t)y[7] << 16);
+  }
+}
+
+// How a call runs.
 struct Plan {
+  bool tensor_cores;
   int segments, segment_tokens;
-  size_t sums;   // floats per set of segment sums
-  size_t bytes;  // whole workspace
+  size_t sums;         // bytes of a set of segment sums
+  LaOperand op[4];     // q, k, v, d_out
+  int width[4];
+  size_t packed[4];    // bytes of a packed copy, 0: read as it is
+  size_t bytes;        // whole workspace: one set of sums (backward: two), then the copies
 };
 
-// Segments: as many as fill the GPU, if a sequence's share of the work is then still a few chunks.  Forming the sums first reads
-// keys and values once more, about half of a forward's work, so cutting has to at least double the number of CTAs at work.
-Plan make_plan(const RingRnnLinearAttention& p, int backward) {
+// Segments.  Forming the sums reads keys and values once more, so a sequence is only cut where that brings more CTAs to work.
+int cut(const RingRnnLinearAttention& p, bool tensor_cores, int backward) {
+  const int chunk = tensor_cores ? LA_TC_CHUNK : PC;
+  const long long bh = (long long)p.B * p.H;
+  if (!tensor_cores) {
+    // two CTAs per SM; a segment of at least eight chunks, and at least twice the CTAs
+    const long long ctas = bh * (backward ? 3 : 1) * ((p.dv + PO - 1) / PO), most = (p.T + 8 * chunk - 1) / (8 * chunk);
+    const long long n = 296 / ctas < most ? 296 / ctas : most;
+    return n < 2 ? 1 : (int)n;
+  }
+  const int chunks = (p.T + chunk - 1) / chunk;
+  if (bh * (backward ? 3 : 1) > 148 || chunks < 4) return 1;
+  const long long n = 148 / (bh * (backward ? 3 : 1));
+  const int most = (chunks + 1) / 2;
+  return n < 2 ? 1 : n < most ? (int)n : most;
+}
+
+Plan make_plan(const RingRnnLinearAttention& p, const RingRnnStrided* d_out) {
   Plan l;
-  const int chunk = PC, least = 8 * chunk;
-  const long long ctas = (long long)p.B * p.H * (backward ? 3 : 1) * ((p.dv + PO - 1) / PO);
-  long long n = 296 / ctas;
-  const long long most = (p.T + least - 1) / least;
-  n = n > most ? most : n;
-  if (n < 2) n = 1;
-  l.segment_tokens = (int)(((p.T + n - 1) / n + chunk - 1) / chunk * chunk);
-  l.segments = (p.T + l.segment_tokens - 1) / l.segment_tokens;
-  l.sums = l.segments > 1 ? (size_t)p.B * p.H * l.segments * p.dk * p.dv : 0;
-  l.bytes = align_up(l.sums * sizeof(float), 256) * (backward ? 2 : 1);
+  memset(&l, 0, sizeof(l));
+  const bool backward = d_out != nullptr;
+  l.tensor_cores = p.dtype == RINGRNN_BF16 && p.dk <= LA_TC_WIDTH && p.dv <= LA_TC_WIDTH;
+  const int chunk = l.tensor_cores ? LA_TC_CHUNK : PC, n = cut(p, l.tensor_cores, backward);
+  l.segment_tokens = (int)((((long long)p.T + n - 1) / n + chunk - 1) / chunk * chunk);
+  l.segments = (int)(((long long)p.T + l.segment_tokens - 1) / l.segment_tokens);
+  l.sums = l.segments > 1 ? align_up((size_t)p.B * p.H * l.segments * p.dk * p.dv * sizeof(float), 256) : 0;
+  l.bytes = l.sums * (backward ? 2 : 1);
+  l.op[0] = operand(p.q); l.op[1] = operand(p.k); l.op[2] = operand(p.v);
+  l.width[0] = l.width[1] = p.dk; l.width[2] = l.width[3] = p.dv;
+  if (backward) l.op[3] = operand(*d_out);
+  if (l.tensor_cores)
+    for (int x = 0; x < (backward ? 4 : 3); ++x)
+      if (!la_tc_operand_ok(l.op[x], p.B, p.T, p.H)) {
+        l.packed[x] = align_up((size_t)p.B * p.T * p.H * align_up(l.width[x], 8) * 2, 256);
+        l.bytes += l.packed[x];
+      }
   return l;
+}
+
+// Copies what has to be copied into the workspace behind the sums; l.op then names the copies.
+int pack(const RingRnnLinearAttention& p, Plan* l, char* at, cudaStream_t s) {
+  PackJobs jobs;
+  memset(&jobs, 0, sizeof(jobs));
+  int n = 0, most = 0;
+  for (int x = 0; x < 4; ++x) {
+    if (l->packed[x] == 0) continue;
+    const int padded = (int)align_up(l->width[x], 8);
+    jobs.from[n] = l->op[x];
+    jobs.to[n] = reinterpret_cast<__nv_bfloat16*>(at);
+    jobs.width[n] = l->width[x];
+    jobs.padded[n++] = padded;
+    most = padded > most ? padded : most;
+    l->op[x] = LaOperand{at, (long long)p.T * p.H * padded, (long long)p.H * padded, padded};
+    at += l->packed[x];
+  }
+  if (n == 0) return RINGRNN_OK;
+  const size_t blocks = ((size_t)p.B * p.T * p.H * (most / 8) + 255) / 256;
+  LaunchScope ls(K_LAYER, s);
+  la_pack_kernel<<<dim3((unsigned)(blocks < 148 * 16 ? blocks : 148 * 16), n), 256, 0, s>>>(jobs, p.B, p.T, p.H);
+  RINGRNN_CUDA_TRY(cudaGetLastError());
+  return RINGRNN_OK;
 }
 
 LaLaunch base_launch(const RingRnnLinearAttention& p, const Plan& l) {
@@ -379,15 +455,19 @@ int check_workspace(const Plan& l, const void* workspace, size_t bytes) {
   if (l.bytes == 0) return RINGRNN_OK;
   return workspace == nullptr || bytes < l.bytes || (reinterpret_cast<uintptr_t>(workspace) & 255) != 0 ? RINGRNN_ERR_WORKSPACE : RINGRNN_OK;
 }
+template <bool STATES>
+int launch(const RingRnnLinearAttention& p, const Plan& l, const LaLaunch& L, cudaStream_t s) {
+  return l.tensor_cores ? la_tc_launch(L, STATES, s) : plain_launch<STATES>(p.dtype, L, s);
+}
 
 }  // namespace
 }  // namespace ringrnn
 
 using namespace ringrnn;
 
-extern "C" size_t ringrnn_linear_attention_bytes(const RingRnnLinearAttention* p, int backward) {
+extern "C" size_t ringrnn_linear_attention_bytes(const RingRnnLinearAttention* p, const RingRnnStrided* d_out) {
   if (p == nullptr || check_linear(*p, false) != RINGRNN_OK) return (size_t)-1;
-  return make_plan(*p, backward).bytes;
+  return make_plan(*p, d_out).bytes;
 }
 
 extern "C" int ringrnn_linear_attention_fwd(const RingRnnLinearAttention* p, void* out, float* final_state, void* workspace,
@@ -396,15 +476,18 @@ extern "C" int ringrnn_linear_attention_fwd(const RingRnnLinearAttention* p, voi
   int rc = check_linear(*p, false);
   if (rc != RINGRNN_OK) return rc;
   if (!p->q.data || !p->k.data || !p->v.data || !p->log_decay || !out) return RINGRNN_ERR_ARG;
-  const Plan l = make_plan(*p, 0);
+  Plan l = make_plan(*p, nullptr);
   rc = check_workspace(l, workspace, workspace_bytes);
+  if (rc == RINGRNN_OK && l.tensor_cores) rc = earlier_failure();
   if (rc != RINGRNN_OK) return rc;
   cudaStream_t s = static_cast<cudaStream_t>(stream);
+  rc = pack(*p, &l, static_cast<char*>(workspace) + l.sums, s);
+  if (rc != RINGRNN_OK) return rc;
   LaLaunch L = base_launch(*p, l);
   float* sums = static_cast<float*>(workspace);
   L.jobs = 1;
   LaJob& j = L.job[0];
-  j.q = operand(p->q); j.k = operand(p->k); j.v = operand(p->v);
+  j.q = l.op[0]; j.k = l.op[1]; j.v = l.op[2];
   j.out = out;
   j.inner = p->dk; j.outer = p->dv;
   j.pair_scale = j.row_scale = p->scale;
@@ -412,7 +495,7 @@ extern "C" int ringrnn_linear_attention_fwd(const RingRnnLinearAttention* p, voi
   j.s_in = p->dv; j.s_out = 1;
   if (l.segments > 1) {
     j.fin = sums;
-    rc = plain_launch<true>(p->dtype, L, s);
+    rc = launch<true>(*p, l, L, s);
     if (rc == RINGRNN_OK) rc = scan_launch(L, p->dk * p->dv, 0, p->initial_state, sums, final_state, s);
     if (rc != RINGRNN_OK) return rc;
     j.init = sums;
@@ -421,7 +504,7 @@ extern "C" int ringrnn_linear_attention_fwd(const RingRnnLinearAttention* p, voi
     j.init = p->initial_state;
     j.fin = final_state;
   }
-  return plain_launch<false>(p->dtype, L, s);
+  return launch<false>(*p, l, L, s);
 }
 
 extern "C" int ringrnn_linear_attention_bwd(const RingRnnLinearAttention* p, const RingRnnStrided* d_out, const float* d_final,
@@ -431,11 +514,14 @@ extern "C" int ringrnn_linear_attention_bwd(const RingRnnLinearAttention* p, con
   int rc = check_linear(*p, false);
   if (rc != RINGRNN_OK) return rc;
   if (!p->q.data || !p->k.data || !p->v.data || !p->log_decay || !d_out->data || !dq || !dk || !dv) return RINGRNN_ERR_ARG;
-  const Plan l = make_plan(*p, 1);
+  Plan l = make_plan(*p, d_out);
   rc = check_workspace(l, workspace, workspace_bytes);
+  if (rc == RINGRNN_OK && l.tensor_cores) rc = earlier_failure();
   if (rc != RINGRNN_OK) return rc;
   cudaStream_t s = static_cast<cudaStream_t>(stream);
-  const LaOperand q = operand(p->q), k = operand(p->k), v = operand(p->v), g = operand(*d_out);
+  rc = pack(*p, &l, static_cast<char*>(workspace) + 2 * l.sums, s);
+  if (rc != RINGRNN_OK) return rc;
+  const LaOperand q = l.op[0], k = l.op[1], v = l.op[2], g = l.op[3];
   LaLaunch L = base_launch(*p, l);
   L.jobs = 3;
   LaJob &jq = L.job[0], &jk = L.job[1], &jv = L.job[2];
@@ -452,12 +538,12 @@ extern "C" int ringrnn_linear_attention_bwd(const RingRnnLinearAttention* p, con
   jv.s_in = p->dv; jv.s_out = 1;
   if (l.segments > 1) {
     float* S = static_cast<float*>(workspace);
-    float* E = reinterpret_cast<float*>(static_cast<char*>(workspace) + align_up(l.sums * sizeof(float), 256));
+    float* E = reinterpret_cast<float*>(static_cast<char*>(workspace) + l.sums);
     LaLaunch M = L;
     M.jobs = 2;
     M.job[0] = jq; M.job[0].fin = S;
     M.job[1] = jv; M.job[1].fin = E;
-    rc = plain_launch<true>(p->dtype, M, s);
+    rc = launch<true>(*p, l, M, s);
     if (rc == RINGRNN_OK) rc = scan_launch(L, p->dk * p->dv, 0, p->initial_state, S, nullptr, s);
     if (rc == RINGRNN_OK) rc = scan_launch(L, p->dk * p->dv, 1, d_final, E, d_initial, s);
     if (rc != RINGRNN_OK) return rc;
@@ -468,7 +554,7 @@ extern "C" int ringrnn_linear_attention_bwd(const RingRnnLinearAttention* p, con
     jk.init = jv.init = d_final;
     jv.fin = d_initial;
   }
-  return plain_launch<false>(p->dtype, L, s);
+  return launch<false>(*p, l, L, s);
 }
 
 extern "C" int ringrnn_linear_attention_step(const RingRnnLinearAttention* p, float* state, const unsigned char* active, void* out,

@@ -495,5 +495,9 @@ __device__ __forceinline__ uint32_t sw128_offset(uint32_t row, uint32_t k) {
 // box_cols * 2 bytes must not exceed the swizzle span (128 or 64 bytes)
 bool make_tmap_bf16_2d(CUtensorMap* out, const void* base, uint64_t rows, uint64_t cols, uint32_t box_rows,
                        uint32_t box_cols, int swizzle_bytes = 128);
+// 4-D bf16 tensor, dims[0] contiguous, the strides of the others in bytes (multiples of 16); 128-byte swizzle, so box[0] <= 64.
+// What a box covers beyond the tensor reads as zero.
+bool make_tmap_bf16_4d(CUtensorMap* out, const void* base, const uint64_t dims[4], const uint64_t stride_bytes[3],
+                       const uint32_t box[4]);
 
 }  // namespace ringrnn

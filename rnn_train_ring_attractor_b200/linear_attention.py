@@ -85,7 +85,7 @@ def _forward(q, k, v, log_decay, scale, lengths, initial_state):
     L = _lib.lib()
     with on_device(dev), nvtx_range("ringrnn_linear_attention_fwd"):
         p = _problem(q, k, v, log_decay, scale, lengths, initial_state)
-        n = L.ringrnn_linear_attention_bytes(C.byref(p), 0)
+        n = L.ringrnn_linear_attention_bytes(C.byref(p), None)
         if n == _lib.INVALID_BYTES:
             raise RuntimeError("linear_attention: batch, tokens or heads too large")
         ws = _scratch(n, dev)
@@ -124,7 +124,7 @@ class LinearAttentionFunc(Function):
         with on_device(dev), nvtx_range("ringrnn_linear_attention_bwd"):
             p = _problem(q, k, v, log_decay, ctx.scale, lengths, initial_state)
             g = strided(d_out)
-            n = L.ringrnn_linear_attention_bytes(C.byref(p), 1)
+            n = L.ringrnn_linear_attention_bytes(C.byref(p), C.byref(g))
             ws = _scratch(n, dev)
             _lib.check(L.ringrnn_linear_attention_bwd(
                 C.byref(p), C.byref(g), None if d_final is None else d_final.data_ptr(), dq.data_ptr(), dk.data_ptr(),

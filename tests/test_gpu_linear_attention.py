@@ -119,7 +119,7 @@ def test_long_sequences_of_few_heads(dtype, B, T, H, dk, dv):
         q, k, v, l, s, n, d_out, d_final = _inputs(dtype, B, T, H, dk, dv, seed=2, lengths=lengths)
         l[0] = -1e-3
         p = _lib.LinearAttention(B, T, H, dk, dv, 0, 1.0)
-        assert _lib.lib().ringrnn_linear_attention_bytes(p, 0) > 0
+        assert _lib.lib().ringrnn_linear_attention_bytes(p, None) > 0
         got, grads = _run(q, k, v, l, 0.3, s, n, d_out, d_final)
         _check_forward(got, q, k, v, l, 0.3, s, n)
         _check_grads(grads, q, k, v, l, 0.3, s, n, d_out, d_final)
@@ -381,7 +381,7 @@ def test_nothing_is_written_beyond_the_outputs():
         (a, pa), (b, pb), (c, pc), (e, pe) = (block(B * T * H * dk, dtype), block(B * T * H * dk, dtype), block(B * T * H * dv, dtype),
                                              block(B * H * dk * dv, FP32))
         for backward in (0, 1):
-            size = L.ringrnn_linear_attention_bytes(C.byref(p), backward)
+            size = L.ringrnn_linear_attention_bytes(C.byref(p), C.byref(sd(d_out)) if backward else None)
             ws = torch.full((size + 512,), 85, device="cuda", dtype=torch.uint8)
             if backward:
                 rc = L.ringrnn_linear_attention_bwd(C.byref(p), C.byref(sd(d_out)), d_final.data_ptr(), pa, pb, pc, pe, ws.data_ptr(), size, None)

@@ -42,7 +42,7 @@ def test_linear_attention_refuses_before_any_launch(L, bad, status):
     g = _lib.Strided(1 << 20, 4000, 100, 30)
     assert L.ringrnn_linear_attention_bwd(C.byref(p), C.byref(g), None, 256, 256, 256, None, 256, big, None) == status
     if status == 2:
-        assert L.ringrnn_linear_attention_bytes(C.byref(p), 0) == _lib.INVALID_BYTES
+        assert L.ringrnn_linear_attention_bytes(C.byref(p), None) == _lib.INVALID_BYTES
     if bad not in (dict(T=0), dict(dk=257), dict(dv=257)):  # the step has no tokens and wider heads
         assert L.ringrnn_linear_attention_step(C.byref(p), 256, None, 256, None) == status
 
@@ -58,10 +58,10 @@ def test_linear_attention_refuses_missing_buffers(L):
     p = _linear(dk=1025)
     assert L.ringrnn_linear_attention_step(C.byref(p), 256, None, 256, None) == 2
     long = _linear(B=1, T=100000, H=1, dk=128, dv=128)  # one head: cut into segments, which needs room for their sums
-    for backward in (0, 1):
+    for backward in (None, C.byref(g)):
         n = L.ringrnn_linear_attention_bytes(C.byref(long), backward)
         assert 0 < n < 1 << 30
-    n = L.ringrnn_linear_attention_bytes(C.byref(long), 0)
+    n = L.ringrnn_linear_attention_bytes(C.byref(long), None)
     assert L.ringrnn_linear_attention_fwd(C.byref(long), 256, None, None, n, None) == 3
     assert L.ringrnn_linear_attention_fwd(C.byref(long), 256, None, 256, n - 1, None) == 3
     assert L.ringrnn_linear_attention_fwd(C.byref(long), 256, None, 257, n, None) == 3
