@@ -32,6 +32,13 @@ static EncodeTiledFn encode_fn() {
       return reinterpret_cast<EncodeTiledFn>(p);
     return nullptr;
   }();
+  // The driver's encode fails in a host thread that has no context yet: autograd's worker threads, whose first call may be this
+  // (their allocations come from torch's cache).  Naming the device that is current anyway binds its context.
+  static thread_local bool bound = false;
+  if (!bound) {
+    int device = 0;
+    bound = cudaGetDevice(&device) == cudaSuccess && cudaSetDevice(device) == cudaSuccess;
+  }
   return fn;
 }
 

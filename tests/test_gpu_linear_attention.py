@@ -363,6 +363,26 @@ def test_captured_and_replayed(T, H):
         assert torch.equal(a, b)
 
 
+def test_first_cuda_call_of_a_host_thread():
+    """The library called from threads that have not touched the GPU before, as autograd's are."""
+    import ctypes as C
+    import threading
+    L = _lib.lib()
+    q, k, v, l, s, n, _, _ = _inputs(BF16, 1, 70, 2, 64, 64)
+    want, _ = linear_attention(q, k, v, l, scale=0.5)
+    out = torch.empty_like(want)
+    sd = lambda t: _lib.Strided(t.data_ptr(), *t.stride()[:3])  # noqa: E731
+    p = _lib.LinearAttention(1, 70, 2, 64, 64, 1, 0.5, sd(q), sd(k), sd(v), l.data_ptr())
+    torch.cuda.synchronize()
+    got = []
+    for _ in range(3):
+        t = threading.Thread(target=lambda: got.append(L.ringrnn_linear_attention_fwd(C.byref(p), out.data_ptr(), None, None, 0, None)))
+        t.start()
+        t.join()
+    torch.cuda.synchronize()
+    assert got == [0, 0, 0] and torch.equal(out, want)
+
+
 def test_nothing_is_written_beyond_the_outputs():
     """Exact-size outputs inside a larger block, by the C entry points: what surrounds them stays."""
     import ctypes as C
