@@ -13,8 +13,11 @@
 // Precision: the state is fp32 (registers); as an operand it and the weighted keys are two bf16 numbers, 2^-16 of an element, so
 // that states passed from call to call keep what fp32 is for; P alone is rounded to bf16, like the outputs.
 //
-// Roles (20 warps): 0 TMA; 1 MMA issue; 4-7 weight the keys (in place, the rest beside) and the scores; 8-11 write the outputs;
-// 12-19 keep the state, half a row each.  The tensor pipe's order per chunk is inter, delta, intra, next scores: while the state
+// Roles (24 warps): 0 TMA; 1 MMA issue; 4-11 weight the keys (in place, the rest beside) and the scores; 12-15 write the outputs;
+// 16-23 keep the state, half a row each.  A scheduler has one or two warps of a role at a time, each at its own place in the
+// code, and waits for instructions more than for anything else once that outgrows the instruction cache (13 cycles for each
+// instruction, with everything unrolled: 96 us instead of the present time for 8 x 2048 tokens of 16 heads): loops stay rolled,
+// pairs of fp32 are computed as such, and what only a partial chunk needs is done apart.  The tensor pipe's order per chunk is inter, delta, intra, next scores: while the state
 // warps work on delta, it has the last two to do.  Tensor memory: 4 x 128 columns, scores | inter | intra | state, where delta is
 // read from the columns that then receive the next operand.
 #include <string.h>
@@ -29,7 +32,10 @@ using namespace tc;
 
 constexpr int C = LA_TC_CHUNK;
 constexpr int TILE = C * 128;  // bytes of [128 tokens x 64 columns]
-constexpr int LT_THREADS = 640;
+constexpr int LT_THREADS = 768;
+// registers of warps 0-3, 4-11, 12-15, 16-23 (setmaxnreg): no more than the block is launched with
+constexpr int REGS_ISSUE = 32, REGS_WEIGHT = 72, REGS_OUT = 80, REGS_STATE = 104;
+static_assert((4 * REGS_ISSUE + 8 * REGS_WEIGHT + 4 * REGS_OUT + 8 * REGS_STATE) * 32 <= 65536 / LT_THREADS / 8 * 8 * LT_THREADS, "registers");
 constexpr uint32_t TM_SCORES = 0, TM_INTER = 128, TM_INTRA = 256, TM_STATE = 384, TM_COLS = 512;
 
 template <int DI, int DO>
@@ -40,8 +46,11 @@ struct LtCfg {
   // slots | scores (or, forming sums, a second buffer of keys) | keys' rest.  The last operand may be followed by what it reads
   // in place of rows that nobody uses, so another buffer stands behind the slots.
   static constexpr int P = SLOT * SLOTS, KL = P + 2 * TILE, BARS = KL + TILE * (DI / 64);
-  static constexpr int TABLES = BARS + 256;  // 128 row factors, 32 powers
-  static constexpr int SMEM = TABLES + 640 + 1024;
+  static constexpr int TABLES = BARS + 256;      // 128 row factors, 32 powers
+  static constexpr int STAGE = TABLES + 640;     // outputs on their way: 512 bytes for each of four warps
+  static constexpr int FLAGS = STAGE + 2048;
+  static constexpr int SMEM = FLAGS + 16;
+  static_assert(SMEM <= 232448, "shared memory of a block");
 };
 
 struct LtParams {
@@ -68,23 +77,34 @@ __device__ __forceinline__ uint32_t pack2(float lo, float hi) {
   const __nv_bfloat162 v = __floats2bfloat162_rn(lo, hi);
   return *reinterpret_cast<const uint32_t*>(&v);
 }
-__device__ __forceinline__ float lo_of(uint32_t v) { return __uint_as_float(v << 16); }
-__device__ __forceinline__ float hi_of(uint32_t v) { return __uint_as_float(v & 0xffff0000u); }
-// two fp32 as bf16, and what that leaves of them as bf16
-__device__ __forceinline__ void split2(float a, float b, uint32_t* hi, uint32_t* lo) {
-  *hi = pack2(a, b);
-  *lo = pack2(a - lo_of(*hi), b - hi_of(*hi));
+__device__ __forceinline__ uint32_t pack2(f32x2 v) {
+  float a, b;
+  upk2(v, a, b);
+  return pack2(a, b);
 }
+__device__ __forceinline__ f32x2 unpack2(uint32_t v) { return pk2u(v << 16, v & 0xffff0000u); }
+// two fp32 as bf16, and what that leaves of them as bf16
+__device__ __forceinline__ void split2(f32x2 v, uint32_t* hi, uint32_t* lo) {
+  *hi = pack2(v);
+  *lo = pack2(fma2(unpack2(*hi), pk2(-1.f, -1.f), v));
+}
+template <int REGS>
+__device__ __forceinline__ void regs_down() { asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(REGS)); }
+template <int REGS>
+__device__ __forceinline__ void regs_up() { asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(REGS)); }
 
 template <int DI, int DO, bool STATES>
 __global__ void __launch_bounds__(LT_THREADS, 1) la_tc_kernel(const __grid_constant__ LtParams A, volatile int* host_status) {
   using Cfg = LtCfg<DI, DO>;
   constexpr int NS = Cfg::SLOTS, TILES = STATES ? 2 : 3;  // tiles of a chunk: (q,) k, v
-  extern __shared__ uint8_t raw[];
-  const uint32_t base = (smem_u32(raw) + 1023u) & ~1023u;
-  uint8_t* const mem = raw + (base - smem_u32(raw));
-  __shared__ int dead, drain_dead[2];
-  __shared__ uint32_t tmem_base;
+  // (nothing else is in shared memory, so that this starts on a boundary of the swizzle's period; there is no room to move it)
+  extern __shared__ __align__(1024) uint8_t mem[];
+  const uint32_t base = smem_u32(mem);
+  if ((base & 1023u) != 0) {
+    if (threadIdx.x == 0) report_abandoned(WaitCtx{nullptr, nullptr, 0, host_status}, 100);
+    return;
+  }
+  int* const flags = reinterpret_cast<int*>(mem + Cfg::FLAGS);  // dead; one each for the two roles that drain; tensor memory
 
   const LaLaunch& L = A.L;
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
@@ -101,40 +121,42 @@ __global__ void __launch_bounds__(LT_THREADS, 1) la_tc_kernel(const __grid_const
   auto empty = [&](int i) { return bars + 8u * (NS + i); };
   const uint32_t one = bars + 16u * NS;
   const uint32_t scores_ready = one, keys_ready = one + 8, pairs_ready = one + 16, inter_done = one + 24, delta_ready = one + 32,
-                 state_ready = one + 40, out_ready = one + 48, out_free = one + 56, all_done = one + 64;
+                 state_ready = one + 40, out_ready = one + 48, out_free = one + 56, all_done = one + 64, tail_ready = one + 72;
   float* const row_factor = reinterpret_cast<float*>(mem + Cfg::TABLES);
   float* const powers = row_factor + C;
 
   if (warp == 0) {
     if (lane == 0) {
-      dead = drain_dead[0] = drain_dead[1] = 0;
+      flags[0] = flags[1] = flags[2] = 0;
       for (int i = 0; i < NS; ++i) {
         mbar_init(full(i), 1);
         mbar_init(empty(i), 1);
       }
       mbar_init(scores_ready, 1);
-      mbar_init(keys_ready, 128);
-      mbar_init(pairs_ready, 128);
+      mbar_init(keys_ready, 256);
+      mbar_init(pairs_ready, 256);
       mbar_init(inter_done, 1);
       mbar_init(delta_ready, 1);
       mbar_init(state_ready, 256);
       mbar_init(out_ready, 1);
       mbar_init(out_free, 128);
       mbar_init(all_done, 1);
+      mbar_init(tail_ready, 256);
       fence_mbar_init();
     }
   } else if (warp == 1) {
-    tmem_alloc(smem_u32(&tmem_base), TM_COLS);
+    tmem_alloc(base + Cfg::FLAGS + 12, TM_COLS);
   }
   const LaDecay g(L.log_decay[h]);
   if (warp == 2) powers[lane] = g.power(rev ? lane : 31 - lane);
   tcgen05_fence_before();
   __syncthreads();
   tcgen05_fence_after();
-  const uint32_t tm = tmem_base;
-  const WaitCtx w{&dead, nullptr, WAIT_LIMIT_CYCLES, host_status};
-  const WaitCtx drain{&drain_dead[warp & 1], nullptr, WAIT_LIMIT_CYCLES, host_status};
+  const uint32_t tm = *reinterpret_cast<volatile uint32_t*>(flags + 3);
+  const WaitCtx w{flags, nullptr, WAIT_LIMIT_CYCLES, host_status};
+  const WaitCtx drain{flags + 1 + (warp & 1), nullptr, WAIT_LIMIT_CYCLES, host_status};
 
+  if (warp < 4) regs_down<REGS_ISSUE>();
   if (warp == 0) {
     // ---- loads: q, k, v of each chunk through a ring of slots
     if (lane == 0) {
@@ -151,10 +173,10 @@ __global__ void __launch_bounds__(LT_THREADS, 1) la_tc_kernel(const __grid_const
             tma_load_4d(base + i * Cfg::SLOT + k * TILE, maps + x, full(i), k * 64, t0, h * A.h_step[ji][x], b * A.b_step[ji][x]);
           if (++i == NS) i = 0, ++round;
         }
-        if (*static_cast<volatile int*>(&dead)) break;
+        if (*static_cast<volatile int*>(flags)) break;
       }
       // where a wait was abandoned, what is on its way has to land before the block's shared memory goes to another
-      if (*static_cast<volatile int*>(&dead)) {
+      if (*static_cast<volatile int*>(flags)) {
         const int issued = round * NS + i, first = issued > NS ? issued - NS : 0;
         for (int x = first; x < issued; ++x) mbar_wait(full(x % NS), (x / NS) & 1, drain, 102);
       }
@@ -170,31 +192,34 @@ __global__ void __launch_bounds__(LT_THREADS, 1) la_tc_kernel(const __grid_const
     auto k_major = [&](uint32_t tile, int ks) { return desc_sw128(desc_lo(tile + (ks >> 2) * TILE + (ks & 3) * 32, 0)); };
     // M/N-major ones: 16 rows, blocks of 64 columns a tile apart
     auto mn_major = [&](uint32_t tile, int ks) { return desc_sw128(desc_lo(tile + ks * 2048, TILE)); };
-    auto scores = [&](int c) {
-      const uint32_t q = slot(TILES * c), k = slot(TILES * c + 1);
-      loaded(TILES * c, 110);
-      loaded(TILES * c + 1, 111);
-      for (int ks = 0; ks < DI / 16; ++ks) umma_ss_warp(tm + TM_SCORES, k_major(q, ks), k_major(k, ks), ID_SCORES, ks != 0, lead);
-      if (lead) umma_commit(scores_ready);
-      __syncwarp();
-    };
-    if (!STATES && chunks > 0) scores(0);
+    // (loops are left rolled where their instructions keep up: see the note on roles)
+#pragma unroll 1
     for (int c = 0; c < chunks; ++c) {
       const int kt = TILES * c + TILES - 2, vt = kt + 1;
       const uint32_t k = slot(kt), v = slot(vt);
       if (!STATES) {
-        const int qt = TILES * c;
+        const uint32_t q = slot(kt - 1);
+        loaded(kt - 1, 110);
+        loaded(kt, 111);
+        if (chunk_at(c) + C > end) mbar_wait(tail_ready, 0, w, 119);
+        tcgen05_fence_after();
+#pragma unroll 2
+        for (int ks = 0; ks < DI / 16; ++ks) umma_ss_warp(tm + TM_SCORES, k_major(q, ks), k_major(k, ks), ID_SCORES, ks != 0, lead);
+        if (lead) umma_commit(scores_ready);
+        __syncwarp();
         mbar_wait(state_ready, c & 1, w, 112);
         if (c > 0) mbar_wait(out_free, (c - 1) & 1, w, 113);
         tcgen05_fence_after();
         // the state's halves stand one behind the other, each as DI / 4 columns of hi and DI / 4 of lo
-        for (int part = 0; part < 2; ++part)
-          for (int ks = 0; ks < DI / 16; ++ks)
-            umma_ts_warp(tm + TM_INTER, tm + TM_STATE + (ks / (DI / 32)) * (DI / 2) + part * (DI / 4) + (ks % (DI / 32)) * 8,
-                         k_major(slot(qt), ks), ID_INTER, part + ks != 0, lead);
+#pragma unroll 2
+        for (int x = 0; x < DI / 8; ++x) {
+          const int part = x & 1, ks = x >> 1;
+          umma_ts_warp(tm + TM_INTER, tm + TM_STATE + (ks / (DI / 32)) * (DI / 2) + part * (DI / 4) + (ks % (DI / 32)) * 8,
+                       k_major(q, ks), ID_INTER, x != 0, lead);
+        }
         if (lead) {
           umma_commit(inter_done);
-          umma_commit(empty(qt % NS));
+          umma_commit(empty((kt - 1) % NS));
         }
         __syncwarp();
       }
@@ -204,9 +229,9 @@ __global__ void __launch_bounds__(LT_THREADS, 1) la_tc_kernel(const __grid_const
       if (!STATES) mbar_wait(inter_done, c & 1, w, 116);
       tcgen05_fence_after();
       const uint32_t rest = base + (STATES && (c & 1) ? Cfg::P : Cfg::KL);
-      for (int part = 0; part < 2; ++part)
-        for (int ks = 0; ks < C / 16; ++ks)
-          umma_ss_warp(tm + TM_STATE, mn_major(v, ks), mn_major(part ? rest : k, ks), ID_DELTA, (STATES && c > 0) || part + ks != 0, lead);
+#pragma unroll 2
+      for (int x = 0; x < C / 8; ++x)
+        umma_ss_warp(tm + TM_STATE, mn_major(v, x >> 1), mn_major(x & 1 ? rest : k, x >> 1), ID_DELTA, (STATES && c > 0) || x != 0, lead);
       if (lead) {
         if (STATES) umma_commit(c & 1 ? out_ready : inter_done);  // one barrier for even chunks, one for odd ones
         if (!STATES || c == chunks - 1) umma_commit(delta_ready);
@@ -217,6 +242,7 @@ __global__ void __launch_bounds__(LT_THREADS, 1) la_tc_kernel(const __grid_const
       if (!STATES) {
         mbar_wait(pairs_ready, c & 1, w, 117);
         tcgen05_fence_after();
+#pragma unroll 2
         for (int ks = 0; ks < C / 16; ++ks)
           umma_ss_warp(tm + TM_INTRA, mn_major(v, ks), k_major(base + Cfg::P, ks), ID_INTRA, ks != 0, lead);
         if (lead) {
@@ -224,23 +250,52 @@ __global__ void __launch_bounds__(LT_THREADS, 1) la_tc_kernel(const __grid_const
           umma_commit(empty(vt % NS));
         }
         __syncwarp();
-        if (c + 1 < chunks) scores(c + 1);
       }
     }
     // tensor memory is given back below: nothing may still be writing it (at once, unless a wait was abandoned)
     if (lead) umma_commit(all_done);
     mbar_wait(all_done, 0, drain, 118);
-  } else if (warp >= 4 && warp < 8) {
-    // ---- keys weighted for the state, then scores weighted: a thread has row r of both
-    const int r = tid - 128, q = warp - 4;
-    if (!STATES) {  // blocks of 32 keys that no token of this warp's rows sees: zero once and for all
-      for (int j = 0; j < 4; ++j)
-        if (rev ? j < q : j > q)
-          for (int i = 0; i < 4; ++i) sts128(base + Cfg::P + (j >> 1) * TILE + sw128_offset(r, (j & 1) * 32 + 8 * i), 0, 0, 0, 0);
+  } else if (warp >= 4 && warp < 12) {
+    // ---- keys weighted for the state, then scores weighted: a thread has half of row r of both
+    regs_down<REGS_WEIGHT>();
+    const int q = warp & 3, half = (warp - 4) >> 2, r = q * 32 + lane;
+    // a block of 32 keys seen by all, some or none of this warp's 32 tokens: j to q's one side, j == q, the other side
+    auto seen = [&](int j) { return rev ? j >= q : j <= q; };
+    auto pair_at = [&](int j) { return base + Cfg::P + (j >> 1) * TILE; };
+    const int col = half * 16;  // of each block
+    // Weights of scores, the same in every chunk.  The diagonal block's stand in registers.  Another block's are the power up to
+    // its near end, a factor per token (32 tokens more: times g^32), times one within the block: all at most one.
+    f32x2 diagonal[8];
+    const float near = J.pair_scale * g.power(rev ? 32 - lane : lane + 1), g32 = g.power(32);
+#pragma unroll
+    for (int s = 0; s < 16; s += 2) {
+      const int far = rev ? col + s - lane : lane - col - s, far1 = rev ? far + 1 : far - 1;
+      diagonal[s / 2] = pk2(far >= 0 ? J.pair_scale * g.power(far) : 0.f, far1 >= 0 ? J.pair_scale * g.power(far1) : 0.f);
     }
+    if (!STATES) {  // none: zero once and for all
+      for (int j = 0; j < 4; ++j)
+        if (!seen(j))
+          for (int i = 0; i < 2; ++i) sts128(pair_at(j) + sw128_offset(r, (j & 1) * 32 + col + 8 * i), 0, 0, 0, 0);
+    }
+#pragma unroll 1
     for (int c = 0; c < chunks; ++c) {
       const int t0 = chunk_at(c), n = min(C, end - t0), kt = TILES * c + TILES - 2, vt = kt + 1;
       const uint32_t k = base + (kt % NS) * Cfg::SLOT, rest = base + (STATES && (c & 1) ? Cfg::P : Cfg::KL);
+      const int steps = STATES ? (rev ? t0 + r - begin + 1 : end - 1 - t0 - r) : rev ? r + 1 : n - 1 - r;
+      const float wk = r < n ? J.key_scale * g.power(steps) : 0.f;
+      if (n < C) {
+        // what stands behind the sequence, a NaN included, becomes zero before anybody reads it
+        mbar_wait(full(kt % NS), (kt / NS) & 1, w, 120);
+        mbar_wait(full(vt % NS), (vt / NS) & 1, w, 123);
+        if (r >= n) {
+          const uint32_t v = base + (vt % NS) * Cfg::SLOT;
+          for (int i = half; i < DI / 8; i += 2) sts128(k + (i >> 3) * TILE + sw128_offset(r, (i & 7) * 8), 0, 0, 0, 0);
+          for (int i = half; i < DO / 8; i += 2) sts128(v + (i >> 3) * TILE + sw128_offset(r, (i & 7) * 8), 0, 0, 0, 0);
+        }
+        fence_proxy_async_smem();
+        if (!STATES) mbar_arrive(tail_ready);
+        else named_bar_sync(2, 256);
+      }
       if (STATES) {
         mbar_wait(full(kt % NS), (kt / NS) & 1, w, 120);
         // the sum of two chunks before has read its keys' rest
@@ -249,81 +304,92 @@ __global__ void __launch_bounds__(LT_THREADS, 1) la_tc_kernel(const __grid_const
         mbar_wait(scores_ready, c & 1, w, 122);
         tcgen05_fence_after();
       }
-      const int steps = STATES ? (rev ? t0 + r - begin + 1 : end - 1 - t0 - r) : rev ? r + 1 : n - 1 - r;
-      const float wk = r < n ? J.key_scale * g.power(steps) : 0.f;
-#pragma unroll 4
-      for (int i = 0; i < DI / 8; ++i) {
-        const uint32_t o = (i >> 3) * TILE + sw128_offset(r, (i & 7) * 8);
-        const uint4 x = lds128(k + o);
-        uint4 hi, lo;
-        split2(lo_of(x.x) * wk, hi_of(x.x) * wk, &hi.x, &lo.x);
-        split2(lo_of(x.y) * wk, hi_of(x.y) * wk, &hi.y, &lo.y);
-        split2(lo_of(x.z) * wk, hi_of(x.z) * wk, &hi.z, &lo.z);
-        split2(lo_of(x.w) * wk, hi_of(x.w) * wk, &hi.w, &lo.w);
-        if (r >= n) hi = lo = make_uint4(0, 0, 0, 0);  // whatever stands behind the sequence, a NaN included
-        sts128(k + o, hi.x, hi.y, hi.z, hi.w);
-        sts128(rest + o, lo.x, lo.y, lo.z, lo.w);
-      }
-      if (n < C) {
-        mbar_wait(full(vt % NS), (vt / NS) & 1, w, 123);
-        if (r >= n)
-          for (int i = 0; i < DO / 8; ++i) sts128(base + (vt % NS) * Cfg::SLOT + (i >> 3) * TILE + sw128_offset(r, (i & 7) * 8), 0, 0, 0, 0);
+      const f32x2 wk2 = pk2(wk, wk);
+#pragma unroll 1
+      for (int i = half * (DI / 16); i < (half + 1) * (DI / 16); i += 2) {
+        const uint32_t o0 = (i >> 3) * TILE + sw128_offset(r, (i & 7) * 8), o1 = (i >> 3) * TILE + sw128_offset(r, (i & 7) * 8 + 8);
+        const uint4 x0 = lds128(k + o0), x1 = lds128(k + o1);
+        const uint32_t x[8] = {x0.x, x0.y, x0.z, x0.w, x1.x, x1.y, x1.z, x1.w};
+        uint32_t hi[8], lo[8];
+#pragma unroll
+        for (int e = 0; e < 8; ++e) split2(mul2(unpack2(x[e]), wk2), hi + e, lo + e);
+        sts128(k + o0, hi[0], hi[1], hi[2], hi[3]);
+        sts128(k + o1, hi[4], hi[5], hi[6], hi[7]);
+        sts128(rest + o0, lo[0], lo[1], lo[2], lo[3]);
+        sts128(rest + o1, lo[4], lo[5], lo[6], lo[7]);
       }
       fence_proxy_async_smem();
       mbar_arrive(keys_ready);
       if (!STATES) {
+        const uint32_t from = tm + TM_SCORES + ((uint32_t)(q * 32) << 16) + col;
+        auto put = [&](int j, const f32x2* y) {
+#pragma unroll
+          for (int e = 0; e < 8; e += 4)
+            sts128(pair_at(j) + sw128_offset(r, (j & 1) * 32 + col + 2 * e), pack2(y[e]), pack2(y[e + 1]), pack2(y[e + 2]), pack2(y[e + 3]));
+        };
+        uint32_t x[16];
+        f32x2 y[8];
+        tmem_ld16(from + q * 32, x);
+        tmem_ld_wait();
+        // (selected: a score that is not finite may stand on the wrong side of the diagonal)
+#pragma unroll
+        for (int s = 0; s < 16; ++s) x[s] = (rev ? col + s >= lane : col + s <= lane) ? x[s] : 0u;
+#pragma unroll
+        for (int s = 0; s < 8; ++s) y[s] = mul2(pk2u(x[2 * s], x[2 * s + 1]), diagonal[s]);
+        put(q, y);
+        float f = near;
 #pragma unroll 1
-        for (int j = 0; j < 4; ++j) {
-          if (rev ? j < q : j > q) continue;
-          uint32_t x[32];
-          tmem_ld32(tm + TM_SCORES + ((uint32_t)(q * 32) << 16) + j * 32, x);
+        for (int j = rev ? q + 1 : q - 1; rev ? j < 4 : j >= 0; j += rev ? 1 : -1) {
+          tmem_ld16(from + j * 32, x);
+          const f32x2 f2 = pk2(f, f);
+          f *= g32;
+#pragma unroll
+          for (int s = 0; s < 8; s += 2) {
+            const float4 p = *reinterpret_cast<const float4*>(powers + col + 2 * s);
+            y[s] = mul2(f2, pk2(p.x, p.y));
+            y[s + 1] = mul2(f2, pk2(p.z, p.w));
+          }
           tmem_ld_wait();
-          if (j == q) {
 #pragma unroll
-            for (int s = 0; s < 32; ++s) {
-              const int far = rev ? s - lane : lane - s;
-              x[s] = far >= 0 ? __float_as_uint(__uint_as_float(x[s]) * (J.pair_scale * exp2f(g.hi * (float)far))) : 0u;
-            }
-          } else {
-            // g^(distance) as the distance to the block's near end times a power within it: both at most one
-            const float f = J.pair_scale * g.power(rev ? 32 * j - r : r - 32 * j - 31);
-#pragma unroll
-            for (int s = 0; s < 32; s += 4) {
-              const float4 p = *reinterpret_cast<const float4*>(powers + s);
-              x[s] = __float_as_uint(__uint_as_float(x[s]) * (f * p.x));
-              x[s + 1] = __float_as_uint(__uint_as_float(x[s + 1]) * (f * p.y));
-              x[s + 2] = __float_as_uint(__uint_as_float(x[s + 2]) * (f * p.z));
-              x[s + 3] = __float_as_uint(__uint_as_float(x[s + 3]) * (f * p.w));
-            }
-          }
-          if (n < C)
-#pragma unroll
-            for (int s = 0; s < 32; ++s)
-              if (32 * j + s >= n) x[s] = 0u;
-#pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            const uint32_t* y = x + 8 * i;
-            auto two = [&](int e) { return pack2(__uint_as_float(y[e]), __uint_as_float(y[e + 1])); };
-            sts128(base + Cfg::P + (j >> 1) * TILE + sw128_offset(r, (j & 1) * 32 + 8 * i), two(0), two(2), two(4), two(6));
-          }
+          for (int s = 0; s < 8; ++s) y[s] = mul2(pk2u(x[2 * s], x[2 * s + 1]), y[s]);
+          put(j, y);
         }
         fence_proxy_async_smem();
         tcgen05_fence_before();
         mbar_arrive(pairs_ready);
       }
     }
-  } else if (warp >= 8 && warp < 12) {
-    // ---- outputs: a thread has one outer column and the tokens of a chunk; neighbours trade tokens for columns, so that a store
-    // is 4 bytes and covers 64 bytes of each of two tokens' rows
+  } else if (warp >= 12 && warp < 16) {
+    // ---- outputs: fragments of 32 columns by 8 tokens, turned on their way through shared memory (512 bytes for each warp), so
+    // that a store is 16 bytes and covers 64 bytes of each of eight tokens' rows
+    regs_down<REGS_OUT>();
     if (!STATES) {
-      const int q = warp - 8, o = q * 32 + lane, r = tid - 256;
+      const int q = warp - 12, r = tid - 384, t8 = lane >> 2, o = q * 32 + (lane & 3) * 8;
       const size_t ld = (size_t)L.H * J.outer;
-      __nv_bfloat16* const out = static_cast<__nv_bfloat16*>(J.out) + ((size_t)b * L.T * L.H + h) * J.outer;
-      const bool pairs = (J.outer & 1) == 0 && (reinterpret_cast<uintptr_t>(J.out) & 3) == 0;
-      const bool odd = lane & 1;
+      __nv_bfloat16* const out = static_cast<__nv_bfloat16*>(J.out) + ((size_t)b * L.T * L.H + h) * J.outer + o;
+      const bool vec = (J.outer & 7) == 0 && (reinterpret_cast<uintptr_t>(J.out) & 15) == 0;
+      const uint32_t stage = base + Cfg::STAGE + q * 512;
+      // a token's 64 bytes: four blocks of eight columns, exchanged so that eight tokens' blocks lie in different banks
+      auto staged = [&](int t, int block) { return stage + t * 64 + ((block ^ (t >> 1)) & 3) * 16; };
+      const uint32_t put = staged(lane & 7, lane >> 3), get = staged(t8, lane & 3);
+      // token t of the sequence; zero from `live` on
+      auto store = [&](int t, int live, uint4 v) {
+        if (t >= stop || o >= J.outer) return;
+        if (t >= live) v = make_uint4(0, 0, 0, 0);
+        __nv_bfloat16* const to = out + (size_t)t * ld;
+        if (vec) {
+          *reinterpret_cast<uint4*>(to) = v;
+        } else {
+          const uint32_t x[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+          for (int e = 0; e < 8; ++e)
+            if (o + e < J.outer) to[e] = __ushort_as_bfloat16((unsigned short)(x[e >> 1] >> (16 * (e & 1))));
+        }
+      };
       int have = 0;
+#pragma unroll 1
       for (int c = 0; c < chunks; ++c) {
-        const int t0 = chunk_at(c), n = min(C, end - t0), rows = min(C, stop - t0);
+        const int t0 = chunk_at(c), n = min(C, end - t0);
         if (n != have) {  // factors of the rows: they change with the number of tokens only in reverse, and then once
           named_bar_sync(1, 128);
           row_factor[r] = r < n ? J.row_scale * g.power(rev ? n - 1 - r : r + 1) : 0.f;
@@ -333,73 +399,62 @@ __global__ void __launch_bounds__(LT_THREADS, 1) la_tc_kernel(const __grid_const
         mbar_wait(out_ready, c & 1, w, 130);
         tcgen05_fence_after();
         if (q * 32 < DO) {
+          const uint32_t from = tm + ((uint32_t)(q * 32) << 16);
+          uint32_t x[16], y[16];
+          auto fetch = [&](int i) {
+            tmem_ld_frag2(from + TM_INTER + i, x);
+            tmem_ld_frag2(from + (16u << 16) + TM_INTER + i, x + 8);
+            tmem_ld_frag2(from + TM_INTRA + i, y);
+            tmem_ld_frag2(from + (16u << 16) + TM_INTRA + i, y + 8);
+          };
+          fetch(0);
 #pragma unroll 1
           for (int i = 0; i < C; i += 16) {
-            uint32_t x[16], y[16];
-            tmem_ld16(tm + TM_INTER + ((uint32_t)(q * 32) << 16) + i, x);
-            tmem_ld16(tm + TM_INTRA + ((uint32_t)(q * 32) << 16) + i, y);
+            const f32x2 f0 = *reinterpret_cast<const f32x2*>(row_factor + i + 2 * (lane & 3)),
+                        f1 = *reinterpret_cast<const f32x2*>(row_factor + i + 8 + 2 * (lane & 3));
             tmem_ld_wait();
-            uint32_t v[8];
+            uint32_t v[8];  // of 16 columns (half), 8 tokens, 8 columns: half * 4 + tokens * 2 + columns
 #pragma unroll
-            for (int e = 0; e < 16; e += 4) {
-              const float4 f = *reinterpret_cast<const float4*>(row_factor + i + e);
-              const float a0 = fmaf(f.x, __uint_as_float(x[e]), __uint_as_float(y[e]));
-              const float a1 = fmaf(f.y, __uint_as_float(x[e + 1]), __uint_as_float(y[e + 1]));
-              const float a2 = fmaf(f.z, __uint_as_float(x[e + 2]), __uint_as_float(y[e + 2]));
-              const float a3 = fmaf(f.w, __uint_as_float(x[e + 3]), __uint_as_float(y[e + 3]));
-              v[e / 2] = pack2(a0, a1);
-              v[e / 2 + 1] = pack2(a2, a3);
+            for (int e = 0; e < 8; ++e)
+              v[e] = pack2(fma2((e >> 1) & 1 ? f1 : f0, pk2u(x[2 * e], x[2 * e + 1]), pk2u(y[2 * e], y[2 * e + 1])));
+            if (i + 16 < C) {
+              fetch(i + 16);
+            } else {  // all of it is in registers
+              tcgen05_fence_before();
+              mbar_arrive(out_free);
             }
 #pragma unroll
-            for (int e = 0; e < 8; ++e) {
-              const int t = i + 2 * e;  // this thread's column at tokens t (low half) and t + 1
-              if (n < C) {
-                if (t >= n) v[e] &= 0xffff0000u;
-                if (t + 1 >= n) v[e] &= 0x0000ffffu;
-              }
-              if (pairs) {
-                const uint32_t other = __shfl_xor_sync(0xffffffffu, v[e], 1);
-                const uint32_t z = odd ? __byte_perm(other, v[e], 0x7632) : __byte_perm(v[e], other, 0x5410);
-                const int tt = t + odd;
-                if (tt < rows && o < J.outer) *reinterpret_cast<uint32_t*>(out + (size_t)(t0 + tt) * ld + (o & ~1)) = z;
-              } else if (o < J.outer) {
-                if (t < rows) out[(size_t)(t0 + t) * ld + o] = __ushort_as_bfloat16((unsigned short)v[e]);
-                if (t + 1 < rows) out[(size_t)(t0 + t + 1) * ld + o] = __ushort_as_bfloat16((unsigned short)(v[e] >> 16));
-              }
+            for (int e = 0; e < 4; e += 2) {
+              __syncwarp();  // what stood here has been read
+              stmatrix_x4_trans(put, v[e], v[e + 1], v[e + 4], v[e + 5]);
+              __syncwarp();
+              store(t0 + i + 4 * e + t8, end, lds128(get));
             }
           }
+        } else {
+          mbar_arrive(out_free);
         }
-        tcgen05_fence_before();
-        mbar_arrive(out_free);
       }
       // tokens behind the sequence, beyond its last chunk
-      for (int t = begin + chunks * C; t < stop; ++t)
-        if (o < J.outer) out[(size_t)t * ld + o] = __float2bfloat16_rn(0.f);
+#pragma unroll 1
+      for (int t = begin + chunks * C + t8; t < stop; t += 8) store(t, 0, make_uint4(0, 0, 0, 0));
     }
-  } else if (warp >= 12) {
+  } else if (warp >= 16) {
     // ---- the state: a thread has half a row of S^T
+    regs_up<REGS_STATE>();
     constexpr int N = DI / 2;
-    const int q = warp & 3, half = (warp - 12) >> 2, o = q * 32 + lane, i0 = half * N;
+    const int q = warp & 3, half = (warp - 16) >> 2, o = q * 32 + lane, i0 = half * N;
     const uint32_t mine = tm + TM_STATE + ((uint32_t)(q * 32) << 16) + half * N;
     const size_t mat = (size_t)at * J.inner * J.outer;
-    float S[N];
+    f32x2 S[N / 2];
+    {
+      const float* from = J.init + mat + (size_t)o * J.s_out;
+      const bool given = !STATES && J.init != nullptr && o < J.outer;
 #pragma unroll
-    for (int i = 0; i < N; ++i)
-      S[i] = !STATES && J.init != nullptr && o < J.outer && i0 + i < J.inner ? J.init[mat + (size_t)(i0 + i) * J.s_in + (size_t)o * J.s_out] : 0.f;
-    auto publish = [&]() {
-#pragma unroll
-      for (int i = 0; i < N; i += 16) {
-        uint32_t hi[8], lo[8];
-#pragma unroll
-        for (int e = 0; e < 8; ++e) split2(S[i + 2 * e], S[i + 2 * e + 1], hi + e, lo + e);
-        tmem_st8(mine + i / 2, hi);
-        tmem_st8(mine + N / 2 + i / 2, lo);
-      }
-      tmem_st_wait();
-      tcgen05_fence_before();
-      mbar_arrive(state_ready);
-    };
-    if (!STATES && chunks > 0) publish();
+      for (int i = 0; i < N; i += 2)
+        S[i / 2] = pk2(given && i0 + i < J.inner ? from[(size_t)(i0 + i) * J.s_in] : 0.f,
+                       given && i0 + i + 1 < J.inner ? from[(size_t)(i0 + i + 1) * J.s_in] : 0.f);
+    }
     if (STATES) {
       if (chunks > 0) {
         mbar_wait(delta_ready, 0, w, 140);
@@ -410,31 +465,54 @@ __global__ void __launch_bounds__(LT_THREADS, 1) la_tc_kernel(const __grid_const
           tmem_ld16(mine + i, x);
           tmem_ld_wait();
 #pragma unroll
-          for (int e = 0; e < 16; ++e) S[i + e] = __uint_as_float(x[e]);
+          for (int e = 0; e < 8; ++e) S[i / 2 + e] = pk2u(x[2 * e], x[2 * e + 1]);
         }
       }
     } else {
-      const LaFactor whole(L.log_decay[h], C);
-      for (int c = 0; c < chunks; ++c) {
-        const int n = min(C, end - chunk_at(c));
-        const LaFactor gn = n == C ? whole : LaFactor(L.log_decay[h], n);
-        mbar_wait(delta_ready, c & 1, w, 141);
-        tcgen05_fence_after();
+      const int part = (end - begin) % C;  // tokens of the one chunk that is not whole, 0: there is none
+      const LaFactor whole(L.log_decay[h], C), rest(L.log_decay[h], part);
+#pragma unroll 1
+      for (int c = 0; c <= chunks && chunks > 0; ++c) {
+        if (c > 0) {
+          const bool all = part == 0 || chunk_at(c - 1) + C <= end;
+          const f32x2 g_hi = all ? pk2(whole.hi, whole.hi) : pk2(rest.hi, rest.hi), g_lo = all ? pk2(whole.lo, whole.lo) : pk2(rest.lo, rest.lo);
+          mbar_wait(delta_ready, (c - 1) & 1, w, 141);
+          tcgen05_fence_after();
+          uint32_t x[2][16];
 #pragma unroll
-        for (int i = 0; i < N; i += 16) {
-          uint32_t x[16];
-          tmem_ld16(mine + i, x);
-          tmem_ld_wait();
+          for (int i = 0; i < N; i += 16) {
+            if (i == 0) tmem_ld16(mine, x[0]);
+            tmem_ld_wait();
+            if (i + 16 < N) tmem_ld16(mine + i + 16, x[(i / 16 + 1) & 1]);
+            const uint32_t* y = x[(i / 16) & 1];
 #pragma unroll
-          for (int e = 0; e < 16; ++e) S[i + e] = gn.times(S[i + e], __uint_as_float(x[e]));
+            for (int e = 0; e < 8; ++e) S[i / 2 + e] = fma2(g_hi, S[i / 2 + e], fma2(g_lo, S[i / 2 + e], pk2u(y[2 * e], y[2 * e + 1])));
+          }
         }
-        if (c + 1 < chunks) publish();
+        if (c < chunks) {  // the next operand
+#pragma unroll
+          for (int i = 0; i < N; i += 16) {
+            uint32_t hi[8], lo[8];
+#pragma unroll
+            for (int e = 0; e < 8; ++e) split2(S[i / 2 + e], hi + e, lo + e);
+            tmem_st8(mine + i / 2, hi);
+            tmem_st8(mine + N / 2 + i / 2, lo);
+          }
+          tmem_st_wait();
+          tcgen05_fence_before();
+          mbar_arrive(state_ready);
+        }
       }
     }
     if (J.fin != nullptr && o < J.outer) {
+      float* to = J.fin + mat + (size_t)o * J.s_out;
 #pragma unroll
-      for (int i = 0; i < N; ++i)
-        if (i0 + i < J.inner) J.fin[mat + (size_t)(i0 + i) * J.s_in + (size_t)o * J.s_out] = S[i];
+      for (int i = 0; i < N; i += 2) {
+        float x, y;
+        upk2(S[i / 2], x, y);
+        if (i0 + i < J.inner) to[(size_t)(i0 + i) * J.s_in] = x;
+        if (i0 + i + 1 < J.inner) to[(size_t)(i0 + i + 1) * J.s_in] = y;
+      }
     }
   }
   tcgen05_fence_before();

@@ -234,32 +234,12 @@ __device__ __forceinline__ uint32_t mul_bf16x2(uint32_t a, uint32_t b) {
 __device__ __forceinline__ float bf16_lo(uint32_t v) { return __uint_as_float(v << 16); }
 __device__ __forceinline__ float bf16_hi(uint32_t v) { return __uint_as_float(v & 0xffff0000u); }
 
-// ---- packed fp32 pairs (fma.rn.f32x2 and friends: one instruction for two elements, same rounding as the scalar
-// forms).  The epilogues are bound by their instruction count, not by the fp32 pipe.
-using f32x2 = unsigned long long;
-__device__ __forceinline__ f32x2 pk2(float a, float b) {
-  f32x2 r;
-  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(a), "f"(b));
-  return r;
-}
-__device__ __forceinline__ f32x2 pk2u(uint32_t a, uint32_t b) {
-  f32x2 r;
-  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "r"(a), "r"(b));
-  return r;
-}
-__device__ __forceinline__ void upk2(f32x2 v, float& a, float& b) {
-  asm("mov.b64 {%0, %1}, %2;" : "=f"(a), "=f"(b) : "l"(v));
-}
-__device__ __forceinline__ f32x2 fma2(f32x2 a, f32x2 b, f32x2 c) {
-  f32x2 d;
-  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(d) : "l"(a), "l"(b), "l"(c));
-  return d;
-}
-__device__ __forceinline__ f32x2 mul2(f32x2 a, f32x2 b) {
-  f32x2 d;
-  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
-  return d;
-}
+using tc::f32x2;
+using tc::fma2;
+using tc::mul2;
+using tc::pk2;
+using tc::pk2u;
+using tc::upk2;
 
 // 2^x and 1/x as single special-function instructions (no range fix-ups: results that would be denormal are flushed
 // to zero, which is what erf and the Gaussian density want in their tails; relative error 2^-22 resp. 1 ulp)
