@@ -5,21 +5,24 @@
 // leaves them (c: this chunk of n tokens; t, s: tokens in it; weights as in the forward, "reverse" mirrors them):
 //
 //   scores   [t x s]      = Q K^T                                     both from shared memory
-//   inter^T  [outer x t]  = S^T Q^T        S^T = hi + lo: two bf16 numbers per element, in tensor memory
-//   delta^T  [outer x in] = V^T K'         K'_s = g^(n-1-s) k_s = hi + lo, beside each other in shared memory
+//   inter^T  [outer x t]  = bf16(S^T) Q^T  S in tensor memory
 //   intra^T  [outer x t]  = V^T P^T        P_ts = bf16(scale g^(t-s) scores_ts), s <= t
+//   delta^T  [outer x in] = V^T K'         K'_s = g^(n-1-s) k_s = hi + lo, two bf16 numbers, beside each other in shared memory
 //   out_t    = row_scale g^(t+1) inter_t + intra_t                    S = g^n S + delta
 //
-// Precision: the state is fp32 (registers); as an operand it and the weighted keys are two bf16 numbers, 2^-16 of an element, so
-// that states passed from call to call keep what fp32 is for; P alone is rounded to bf16, like the outputs.
+// Precision: the state is fp32 (registers) and what is added to it keeps sixteen bits, so that states passed from call to call
+// and their gradients are good for what fp32 is for: 2e-6 of their size, where keys rounded to bf16 would leave 2e-3.  Where it
+// only goes into bf16 outputs the state is rounded to bf16, like P: next to the outputs' own rounding that costs a factor of 1.4
+// in their error, a second product for the rest of the state would make it 1.1 and take 512 of a chunk's cycles.
 //
-// Roles (24 warps): 0 TMA; 1 MMA issue; 4-11 weight the keys (in place, the rest beside) and the scores; 12-15 write the outputs;
-// 16-23 keep the state, half a row each.  A scheduler has one or two warps of a role at a time, each at its own place in the
-// code, and waits for instructions more than for anything else once that outgrows the instruction cache (13 cycles for each
-// instruction, with everything unrolled: 96 us instead of the present time for 8 x 2048 tokens of 16 heads): loops stay rolled,
-// pairs of fp32 are computed as such, and what only a partial chunk needs is done apart.  The tensor pipe's order per chunk is inter, delta, intra, next scores: while the state
-// warps work on delta, it has the last two to do.  Tensor memory: 4 x 128 columns, scores | inter | intra | state, where delta is
-// read from the columns that then receive the next operand.
+// Roles (24 warps): 0 TMA loads; 1 MMA issue; 2 TMA stores; 4-11 weight the scores and the keys (in place, the rest beside);
+// 12-15 bring the outputs to shared memory (where this chunk's q was); 16-23 keep the state, half a row each.  A scheduler has one
+// or two warps of a role at a time, each at its own place in the code, and waits for instructions more than for anything else
+// once that outgrows the instruction cache (13 cycles for each instruction, with everything unrolled: 96 us instead of 82 for
+// 8 x 2048 tokens of 16 heads): loops stay rolled, pairs of fp32 are computed as such, and what only a partial chunk needs is done
+// apart.  The tensor pipe's order per chunk is scores, inter, intra, delta: the chain is inter, intra, delta, state, and the next
+// scores fill the pipe while the state warps work.  Tensor memory: 4 x 128 columns, scores | inter | intra | state, where delta
+// is read from the columns that then receive the next operand.
 #include <string.h>
 
 #include "linear_attention.cuh"
@@ -34,7 +37,7 @@ constexpr int C = LA_TC_CHUNK;
 constexpr int TILE = C * 128;  // bytes of [128 tokens x 64 columns]
 constexpr int LT_THREADS = 768;
 // registers of warps 0-3, 4-11, 12-15, 16-23 (setmaxnreg): no more than the block is launched with
-constexpr int REGS_ISSUE = 32, REGS_WEIGHT = 72, REGS_OUT = 80, REGS_STATE = 104;
+constexpr int REGS_ISSUE = 40, REGS_WEIGHT = 80, REGS_OUT = 72, REGS_STATE = 104;
 static_assert((4 * REGS_ISSUE + 8 * REGS_WEIGHT + 4 * REGS_OUT + 8 * REGS_STATE) * 32 <= 65536 / LT_THREADS / 8 * 8 * LT_THREADS, "registers");
 constexpr uint32_t TM_SCORES = 0, TM_INTER = 128, TM_INTRA = 256, TM_STATE = 384, TM_COLS = 512;
 
@@ -47,8 +50,7 @@ struct LtCfg {
   // in place of rows that nobody uses, so another buffer stands behind the slots.
   static constexpr int P = SLOT * SLOTS, KL = P + 2 * TILE, BARS = KL + TILE * (DI / 64);
   static constexpr int TABLES = BARS + 256;      // 128 row factors, 32 powers
-  static constexpr int STAGE = TABLES + 640;     // outputs on their way: 512 bytes for each of four warps
-  static constexpr int FLAGS = STAGE + 2048;
+  static constexpr int FLAGS = TABLES + 640;
   static constexpr int SMEM = FLAGS + 16;
   static_assert(SMEM <= 232448, "shared memory of a block");
 };
@@ -56,7 +58,8 @@ struct LtCfg {
 struct LtParams {
   LaLaunch L;
   int h_step[LA_MAX_JOBS][3], b_step[LA_MAX_JOBS][3];  // 0: a tensor that all heads / sequences share
-  alignas(64) CUtensorMap map[LA_MAX_JOBS][3];
+  int store[LA_MAX_JOBS];  // out can be written by TMA
+  alignas(64) CUtensorMap map[LA_MAX_JOBS][4];  // q, k, v, out
 };
 
 __device__ __forceinline__ void tma_load_4d(uint32_t dst, const CUtensorMap* m, uint32_t bar, int x, int t, int h, int b) {
@@ -64,6 +67,12 @@ __device__ __forceinline__ void tma_load_4d(uint32_t dst, const CUtensorMap* m, 
       "cp.async.bulk.tensor.4d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4, %5, %6}], [%2];" ::"r"(dst),
       "l"(reinterpret_cast<uint64_t>(m)), "r"(bar), "r"(x), "r"(t), "r"(h), "r"(b)
       : "memory");
+}
+__device__ __forceinline__ void tma_store_4d(const CUtensorMap* m, uint32_t src, int x, int t, int h, int b) {
+  asm volatile("cp.async.bulk.tensor.4d.global.shared::cta.bulk_group [%0, {%2, %3, %4, %5}], [%1];" ::"l"(
+                   reinterpret_cast<uint64_t>(m)),
+               "r"(src), "r"(x), "r"(t), "r"(h), "r"(b)
+               : "memory");
 }
 __device__ __forceinline__ uint4 lds128(uint32_t a) {
   uint4 v;
@@ -122,6 +131,10 @@ __global__ void __launch_bounds__(LT_THREADS, 1) la_tc_kernel(const __grid_const
   const uint32_t one = bars + 16u * NS;
   const uint32_t scores_ready = one, keys_ready = one + 8, pairs_ready = one + 16, inter_done = one + 24, delta_ready = one + 32,
                  state_ready = one + 40, out_ready = one + 48, out_free = one + 56, all_done = one + 64, tail_ready = one + 72;
+  // A barrier's waiter can only tell one phase from the next.  Two barriers in turn where the other side can be a chunk ahead.
+  auto staged = [&](int c) { return one + 80 + 8u * (c & 1); };
+  auto sum_keys_ready = [&](int c) { return c & 1 ? pairs_ready : keys_ready; };  // forming sums: keys two chunks ahead at most
+  auto sum_done = [&](int c) { return c & 1 ? out_ready : inter_done; };          // and what they were added to
   float* const row_factor = reinterpret_cast<float*>(mem + Cfg::TABLES);
   float* const powers = row_factor + C;
 
@@ -142,6 +155,8 @@ __global__ void __launch_bounds__(LT_THREADS, 1) la_tc_kernel(const __grid_const
       mbar_init(out_free, 128);
       mbar_init(all_done, 1);
       mbar_init(tail_ready, 256);
+      mbar_init(staged(0), 128);
+      mbar_init(staged(1), 128);
       fence_mbar_init();
     }
   } else if (warp == 1) {
@@ -210,22 +225,26 @@ __global__ void __launch_bounds__(LT_THREADS, 1) la_tc_kernel(const __grid_const
         mbar_wait(state_ready, c & 1, w, 112);
         if (c > 0) mbar_wait(out_free, (c - 1) & 1, w, 113);
         tcgen05_fence_after();
-        // the state's halves stand one behind the other, each as DI / 4 columns of hi and DI / 4 of lo
+        // the state's halves stand one behind the other, DI / 4 of DI / 2 columns each
 #pragma unroll 2
-        for (int x = 0; x < DI / 8; ++x) {
-          const int part = x & 1, ks = x >> 1;
-          umma_ts_warp(tm + TM_INTER, tm + TM_STATE + (ks / (DI / 32)) * (DI / 2) + part * (DI / 4) + (ks % (DI / 32)) * 8,
-                       k_major(q, ks), ID_INTER, x != 0, lead);
-        }
-        if (lead) {
-          umma_commit(inter_done);
-          umma_commit(empty((kt - 1) % NS));
-        }
+        for (int ks = 0; ks < DI / 16; ++ks)
+          umma_ts_warp(tm + TM_INTER, tm + TM_STATE + (ks / (DI / 32)) * (DI / 2) + (ks % (DI / 32)) * 8, k_major(q, ks), ID_INTER, ks != 0, lead);
+        if (lead) umma_commit(inter_done);
         __syncwarp();
+        loaded(vt, 115);
+        mbar_wait(pairs_ready, c & 1, w, 117);
+        tcgen05_fence_after();
+#pragma unroll 2
+        for (int ks = 0; ks < C / 16; ++ks)
+          umma_ss_warp(tm + TM_INTRA, mn_major(v, ks), k_major(base + Cfg::P, ks), ID_INTRA, ks != 0, lead);
+        if (lead) umma_commit(out_ready);
+        __syncwarp();
+      } else {
+        loaded(vt, 115);
       }
-      mbar_wait(keys_ready, c & 1, w, 114);
-      loaded(vt, 115);
-      // delta overwrites the columns that inter has just read: no order holds between MMAs of different accumulators
+      if (STATES) mbar_wait(sum_keys_ready(c), (c >> 1) & 1, w, 114);
+      else mbar_wait(keys_ready, c & 1, w, 114);
+      // delta overwrites the columns that inter has read: no order holds between MMAs of different accumulators
       if (!STATES) mbar_wait(inter_done, c & 1, w, 116);
       tcgen05_fence_after();
       const uint32_t rest = base + (STATES && (c & 1) ? Cfg::P : Cfg::KL);
@@ -233,28 +252,31 @@ __global__ void __launch_bounds__(LT_THREADS, 1) la_tc_kernel(const __grid_const
       for (int x = 0; x < C / 8; ++x)
         umma_ss_warp(tm + TM_STATE, mn_major(v, x >> 1), mn_major(x & 1 ? rest : k, x >> 1), ID_DELTA, (STATES && c > 0) || x != 0, lead);
       if (lead) {
-        if (STATES) umma_commit(c & 1 ? out_ready : inter_done);  // one barrier for even chunks, one for odd ones
+        if (STATES) umma_commit(sum_done(c));
         if (!STATES || c == chunks - 1) umma_commit(delta_ready);
         umma_commit(empty(kt % NS));
-        if (STATES) umma_commit(empty(vt % NS));
+        umma_commit(empty(vt % NS));
       }
       __syncwarp();
-      if (!STATES) {
-        mbar_wait(pairs_ready, c & 1, w, 117);
-        tcgen05_fence_after();
-#pragma unroll 2
-        for (int ks = 0; ks < C / 16; ++ks)
-          umma_ss_warp(tm + TM_INTRA, mn_major(v, ks), k_major(base + Cfg::P, ks), ID_INTRA, ks != 0, lead);
-        if (lead) {
-          umma_commit(out_ready);
-          umma_commit(empty(vt % NS));
-        }
-        __syncwarp();
-      }
     }
     // tensor memory is given back below: nothing may still be writing it (at once, unless a wait was abandoned)
     if (lead) umma_commit(all_done);
     mbar_wait(all_done, 0, drain, 118);
+  } else if (warp == 2) {
+    // ---- stores: outputs from the slot that held q, which is free after that
+    if (!STATES && lane == 0) {
+      for (int c = 0; c < chunks; ++c) {
+        const int slot = (TILES * c) % NS;
+        if (!mbar_wait(staged(c), (c >> 1) & 1, w, 150)) break;
+        if (A.store[ji]) {
+          for (int k = 0; k < DO / 64; ++k) tma_store_4d(A.map[ji] + 3, base + slot * Cfg::SLOT + k * TILE, k * 64, chunk_at(c), h, b);
+          bulk_commit();
+          bulk_wait_read<0>();
+        }
+        mbar_arrive(empty(slot));
+      }
+      bulk_wait_all<0>();
+    }
   } else if (warp >= 4 && warp < 12) {
     // ---- keys weighted for the state, then scores weighted: a thread has half of row r of both
     regs_down<REGS_WEIGHT>();
@@ -299,27 +321,11 @@ __global__ void __launch_bounds__(LT_THREADS, 1) la_tc_kernel(const __grid_const
       if (STATES) {
         mbar_wait(full(kt % NS), (kt / NS) & 1, w, 120);
         // the sum of two chunks before has read its keys' rest
-        if (c > 1) mbar_wait(c & 1 ? out_ready : inter_done, ((c >> 1) - 1) & 1, w, 121);
+        if (c > 1) mbar_wait(sum_done(c), ((c >> 1) - 1) & 1, w, 121);
       } else {
         mbar_wait(scores_ready, c & 1, w, 122);
         tcgen05_fence_after();
       }
-      const f32x2 wk2 = pk2(wk, wk);
-#pragma unroll 1
-      for (int i = half * (DI / 16); i < (half + 1) * (DI / 16); i += 2) {
-        const uint32_t o0 = (i >> 3) * TILE + sw128_offset(r, (i & 7) * 8), o1 = (i >> 3) * TILE + sw128_offset(r, (i & 7) * 8 + 8);
-        const uint4 x0 = lds128(k + o0), x1 = lds128(k + o1);
-        const uint32_t x[8] = {x0.x, x0.y, x0.z, x0.w, x1.x, x1.y, x1.z, x1.w};
-        uint32_t hi[8], lo[8];
-#pragma unroll
-        for (int e = 0; e < 8; ++e) split2(mul2(unpack2(x[e]), wk2), hi + e, lo + e);
-        sts128(k + o0, hi[0], hi[1], hi[2], hi[3]);
-        sts128(k + o1, hi[4], hi[5], hi[6], hi[7]);
-        sts128(rest + o0, lo[0], lo[1], lo[2], lo[3]);
-        sts128(rest + o1, lo[4], lo[5], lo[6], lo[7]);
-      }
-      fence_proxy_async_smem();
-      mbar_arrive(keys_ready);
       if (!STATES) {
         const uint32_t from = tm + TM_SCORES + ((uint32_t)(q * 32) << 16) + col;
         auto put = [&](int j, const f32x2* y) {
@@ -358,38 +364,37 @@ __global__ void __launch_bounds__(LT_THREADS, 1) la_tc_kernel(const __grid_const
         tcgen05_fence_before();
         mbar_arrive(pairs_ready);
       }
+      const f32x2 wk2 = pk2(wk, wk);
+#pragma unroll 1
+      for (int i = half * (DI / 16); i < (half + 1) * (DI / 16); i += 2) {
+        const uint32_t o0 = (i >> 3) * TILE + sw128_offset(r, (i & 7) * 8), o1 = (i >> 3) * TILE + sw128_offset(r, (i & 7) * 8 + 8);
+        const uint4 x0 = lds128(k + o0), x1 = lds128(k + o1);
+        const uint32_t x[8] = {x0.x, x0.y, x0.z, x0.w, x1.x, x1.y, x1.z, x1.w};
+        uint32_t hi[8], lo[8];
+#pragma unroll
+        for (int e = 0; e < 8; ++e) split2(mul2(unpack2(x[e]), wk2), hi + e, lo + e);
+        sts128(k + o0, hi[0], hi[1], hi[2], hi[3]);
+        sts128(k + o1, hi[4], hi[5], hi[6], hi[7]);
+        sts128(rest + o0, lo[0], lo[1], lo[2], lo[3]);
+        sts128(rest + o1, lo[4], lo[5], lo[6], lo[7]);
+      }
+      fence_proxy_async_smem();
+      mbar_arrive(STATES ? sum_keys_ready(c) : keys_ready);
     }
   } else if (warp >= 12 && warp < 16) {
-    // ---- outputs: fragments of 32 columns by 8 tokens, turned on their way through shared memory (512 bytes for each warp), so
-    // that a store is 16 bytes and covers 64 bytes of each of eight tokens' rows
+    // ---- outputs: fragments of 32 columns by 16 tokens, turned by the matrix stores: [token][column] tiles in q's slot
     regs_down<REGS_OUT>();
     if (!STATES) {
-      const int q = warp - 12, r = tid - 384, t8 = lane >> 2, o = q * 32 + (lane & 3) * 8;
+      const int q = warp - 12, r = tid - 384;
       const size_t ld = (size_t)L.H * J.outer;
-      __nv_bfloat16* const out = static_cast<__nv_bfloat16*>(J.out) + ((size_t)b * L.T * L.H + h) * J.outer + o;
-      const bool vec = (J.outer & 7) == 0 && (reinterpret_cast<uintptr_t>(J.out) & 15) == 0;
-      const uint32_t stage = base + Cfg::STAGE + q * 512;
-      // a token's 64 bytes: four blocks of eight columns, exchanged so that eight tokens' blocks lie in different banks
-      auto staged = [&](int t, int block) { return stage + t * 64 + ((block ^ (t >> 1)) & 3) * 16; };
-      const uint32_t put = staged(lane & 7, lane >> 3), get = staged(t8, lane & 3);
-      // token t of the sequence; zero from `live` on
-      auto store = [&](int t, int live, uint4 v) {
-        if (t >= stop || o >= J.outer) return;
-        if (t >= live) v = make_uint4(0, 0, 0, 0);
-        __nv_bfloat16* const to = out + (size_t)t * ld;
-        if (vec) {
-          *reinterpret_cast<uint4*>(to) = v;
-        } else {
-          const uint32_t x[4] = {v.x, v.y, v.z, v.w};
-#pragma unroll
-          for (int e = 0; e < 8; ++e)
-            if (o + e < J.outer) to[e] = __ushort_as_bfloat16((unsigned short)(x[e >> 1] >> (16 * (e & 1))));
-        }
-      };
+      __nv_bfloat16* const out = static_cast<__nv_bfloat16*>(J.out) + ((size_t)b * L.T * L.H + h) * J.outer;
+      const uint32_t from = tm + ((uint32_t)(q * 32) << 16);
+      const uint32_t put = (q >> 1) * TILE + sw128_offset(lane & 7, (q & 1) * 32 + (lane >> 3) * 8);
       int have = 0;
 #pragma unroll 1
       for (int c = 0; c < chunks; ++c) {
         const int t0 = chunk_at(c), n = min(C, end - t0);
+        const uint32_t slot = base + ((TILES * c) % NS) * Cfg::SLOT;
         if (n != have) {  // factors of the rows: they change with the number of tokens only in reverse, and then once
           named_bar_sync(1, 128);
           row_factor[r] = r < n ? J.row_scale * g.power(rev ? n - 1 - r : r + 1) : 0.f;
@@ -399,7 +404,6 @@ __global__ void __launch_bounds__(LT_THREADS, 1) la_tc_kernel(const __grid_const
         mbar_wait(out_ready, c & 1, w, 130);
         tcgen05_fence_after();
         if (q * 32 < DO) {
-          const uint32_t from = tm + ((uint32_t)(q * 32) << 16);
           uint32_t x[16], y[16];
           auto fetch = [&](int i) {
             tmem_ld_frag2(from + TM_INTER + i, x);
@@ -423,21 +427,34 @@ __global__ void __launch_bounds__(LT_THREADS, 1) la_tc_kernel(const __grid_const
               tcgen05_fence_before();
               mbar_arrive(out_free);
             }
+            if (i + 16 > n) {
 #pragma unroll
-            for (int e = 0; e < 4; e += 2) {
-              __syncwarp();  // what stood here has been read
-              stmatrix_x4_trans(put, v[e], v[e + 1], v[e + 4], v[e + 5]);
-              __syncwarp();
-              store(t0 + i + 4 * e + t8, end, lds128(get));
+              for (int e = 0; e < 8; ++e) {
+                const int t = i + ((e >> 1) & 1) * 8 + 2 * (lane & 3);
+                if (t >= n) v[e] &= 0xffff0000u;
+                if (t + 1 >= n) v[e] &= 0x0000ffffu;
+              }
             }
+            stmatrix_x4_trans(slot + put + i * 128, v[0], v[1], v[4], v[5]);
+            stmatrix_x4_trans(slot + put + i * 128 + 1024, v[2], v[3], v[6], v[7]);
           }
         } else {
           mbar_arrive(out_free);
         }
+        if (!A.store[ji]) {  // widths and addresses that TMA does not take: element by element
+          named_bar_sync(1, 128);
+#pragma unroll 1
+          for (int t = 0; t < C && t0 + t < stop; ++t)
+            if (r < J.outer)
+              out[(size_t)(t0 + t) * ld + r] = *reinterpret_cast<const __nv_bfloat16*>(mem + (slot - base) + (r >> 6) * TILE + sw128_offset(t, r & 63));
+        }
+        fence_proxy_async_smem();
+        mbar_arrive(staged(c));
       }
       // tokens behind the sequence, beyond its last chunk
 #pragma unroll 1
-      for (int t = begin + chunks * C + t8; t < stop; t += 8) store(t, 0, make_uint4(0, 0, 0, 0));
+      for (int t = begin + chunks * C; t < stop; ++t)
+        if (r < J.outer) out[(size_t)t * ld + r] = __float2bfloat16_rn(0.f);
     }
   } else if (warp >= 16) {
     // ---- the state: a thread has half a row of S^T
@@ -492,11 +509,10 @@ __global__ void __launch_bounds__(LT_THREADS, 1) la_tc_kernel(const __grid_const
         if (c < chunks) {  // the next operand
 #pragma unroll
           for (int i = 0; i < N; i += 16) {
-            uint32_t hi[8], lo[8];
+            uint32_t x[8];
 #pragma unroll
-            for (int e = 0; e < 8; ++e) split2(S[i / 2 + e], hi + e, lo + e);
-            tmem_st8(mine + i / 2, hi);
-            tmem_st8(mine + N / 2 + i / 2, lo);
+            for (int e = 0; e < 8; ++e) x[e] = pack2(S[i / 2 + e]);
+            tmem_st8(mine + i / 2, x);
           }
           tmem_st_wait();
           tcgen05_fence_before();
@@ -569,6 +585,10 @@ int la_tc_launch(const LaLaunch& L, bool states_only, cudaStream_t s) {
       for (int x = states_only ? 1 : 0; x < 3; ++x)
         if (!make_map(&P.map[to][x], *ops[x], x == 2 ? J.outer : J.inner, L.B, L.T, L.H, &P.h_step[to][x], &P.b_step[to][x]))
           return RINGRNN_ERR_CUDA;
+      int unused[2];
+      const LaOperand out{J.out, (long long)L.T * L.H * J.outer, (long long)L.H * J.outer, J.outer};
+      P.store[to] = !states_only && J.outer % 8 == 0 && (reinterpret_cast<uintptr_t>(J.out) & 15) == 0;
+      if (P.store[to] && !make_map(&P.map[to][3], out, J.outer, L.B, L.T, L.H, unused, unused + 1)) return RINGRNN_ERR_CUDA;
     }
     if (P.L.jobs == 0) continue;
     int rc;

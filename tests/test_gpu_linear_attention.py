@@ -130,6 +130,25 @@ def test_long_sequences_of_few_heads(dtype, B, T, H, dk, dv):
     _check_forward((whole, final), q, k, v, l, 0.3, s, None)
 
 
+@pytest.mark.parametrize("T,H,dk,dv", [(30011, 8, 128, 128), (20003, 20, 64, 64), (9000, 37, 64, 128)])
+def test_many_chunks_in_a_segment(T, H, dk, dv):
+    """Against the fp32 kernel on the same numbers (itself held to the definition above): what the two may differ by."""
+    q, k, v, l, s, n, d_out, d_final = _inputs(BF16, 1, T, H, dk, dv, seed=15)
+    l = l - 1e-3
+    one = [x.float() for x in (q, k, v)]
+    for _ in range(3):  # (the kernels' roles run ahead of each other by what the loads leave them)
+        got, grads = _run(q, k, v, l, 0.1, s, n, d_out, d_final)
+    want, want_g = _run(*one, l, 0.1, s, n, d_out.float(), d_final)
+    top, top_g = _run(*(x.abs() for x in one), l, 0.1, s.abs(), n, d_out.float().abs(), d_final.abs())
+    u = ref.U[BF16]
+    # (the fp32 kernel gives the bound's own sums to a part in 2^10, which the factor 1.01 covers)
+    for i, (a, b, t) in enumerate(zip((*got, *grads), (*want, *want_g), (*top, *top_g))):
+        # a memory is at most a thousand steps long here: sums of 8192 terms at most count, in either kernel
+        f = ref.attend_bounds(BF16, 8192, 128, True)[i in (1, 5)] + 2 * ref.attend_bounds(FP32, 8192, 128, False)[0]
+        allowed = 1.01 * (f + (0 if i in (1, 5) else u * (1 + f))) * t.double() + ref.TINY[BF16]
+        assert ref.worst(a, b.double(), allowed) <= 1.0, i
+
+
 @pytest.mark.parametrize("decay", [0.0, -1e-5, -0.3, -5.0, -60.0, -3e38, float("-inf")])
 @pytest.mark.parametrize("dtype", [FP32, BF16])
 def test_decays_from_none_to_all(dtype, decay):
