@@ -15,9 +15,9 @@
 // only goes into bf16 outputs the state is rounded to bf16, like P: next to the outputs' own rounding that costs a factor of 1.4
 // in their error, a second product for the rest of the state would make it 1.1 and take 512 of a chunk's cycles.
 //
-// Roles (24 warps): 0 TMA loads; 1 MMA issue; 2 TMA stores; 4-11 weight the scores and the keys (in place, the rest beside);
-// 12-15 bring the outputs to shared memory (where this chunk's q was); 16-23 keep the state, half a row each.  A scheduler has one
-// or two warps of a role at a time, each at its own place in the code, and waits for instructions more than for anything else
+// Roles (28 warps): 0 TMA loads; 1 MMA issue; 2 TMA stores; 4-11 weight the scores and the keys (in place, the rest where q was);
+// 12-19 bring the outputs to shared memory (where P was); 20-27 keep the state, half a row each.  A scheduler has two warps of a
+// role at a time, each at its own place in the code, and waits for instructions more than for anything else
 // once that outgrows the instruction cache (13 cycles for each instruction, with everything unrolled: 96 us instead of 82 for
 // 8 x 2048 tokens of 16 heads): loops stay rolled, pairs of fp32 are computed as such, and what only a partial chunk needs is done
 // apart.  The tensor pipe's order per chunk is scores, inter, intra, delta: the chain is inter, intra, delta, state, and the next
@@ -35,21 +35,22 @@ using namespace tc;
 
 constexpr int C = LA_TC_CHUNK;
 constexpr int TILE = C * 128;  // bytes of [128 tokens x 64 columns]
-constexpr int LT_THREADS = 768;
-// registers of warps 0-3, 4-11, 12-15, 16-23 (setmaxnreg): no more than the block is launched with
-constexpr int REGS_ISSUE = 40, REGS_WEIGHT = 80, REGS_OUT = 72, REGS_STATE = 104;
-static_assert((4 * REGS_ISSUE + 8 * REGS_WEIGHT + 4 * REGS_OUT + 8 * REGS_STATE) * 32 <= 65536 / LT_THREADS / 8 * 8 * LT_THREADS, "registers");
+constexpr int LT_THREADS = 896;
+// registers of warps 0-3, 4-11, 12-19, 20-27 (setmaxnreg): no more than the block is launched with
+constexpr int REGS_ISSUE = 32, REGS_WEIGHT = 72, REGS_OUT = 64, REGS_STATE = 96;
+static_assert((4 * REGS_ISSUE + 8 * REGS_WEIGHT + 8 * REGS_OUT + 8 * REGS_STATE) * 32 <= 65536 / LT_THREADS / 8 * 8 * LT_THREADS, "registers");
 constexpr uint32_t TM_SCORES = 0, TM_INTER = 128, TM_INTRA = 256, TM_STATE = 384, TM_COLS = 512;
 
 template <int DI, int DO>
 struct LtCfg {
   static constexpr int WIDE = DI > DO ? DI : DO;
   static constexpr int SLOT = TILE * (WIDE / 64);
-  static constexpr int SLOTS = WIDE == 128 ? 5 : 8;
-  // slots | scores (or, forming sums, a second buffer of keys) | keys' rest.  The last operand may be followed by what it reads
-  // in place of rows that nobody uses, so another buffer stands behind the slots.
-  static constexpr int P = SLOT * SLOTS, KL = P + 2 * TILE, BARS = KL + TILE * (DI / 64);
-  static constexpr int TABLES = BARS + 256;      // 128 row factors, 32 powers
+  static constexpr int SLOTS = WIDE == 128 ? 6 : 12;  // two chunks' q, k and v or four's: what it takes to keep the memory busy
+  // slots | P, then the outputs on their way.  The last v may be followed by what the MMAs read in place of rows that nobody uses,
+  // so another buffer stands behind the slots.
+  static constexpr int P = SLOT * SLOTS, BARS = P + 2 * TILE;
+  static constexpr int TABLES = BARS + (2 * SLOTS + 12) * 8 + 32;  // 128 row factors, 32 powers
+  static_assert(TABLES % 16 == 0, "alignment");
   static constexpr int FLAGS = TABLES + 640;
   static constexpr int SMEM = FLAGS + 16;
   static_assert(SMEM <= 232448, "shared memory of a block");
@@ -105,7 +106,8 @@ __device__ __forceinline__ void regs_up() { asm volatile("setmaxnreg.inc.sync.al
 template <int DI, int DO, bool STATES>
 __global__ void __launch_bounds__(LT_THREADS, 1) la_tc_kernel(const __grid_constant__ LtParams A, volatile int* host_status) {
   using Cfg = LtCfg<DI, DO>;
-  constexpr int NS = Cfg::SLOTS, TILES = STATES ? 2 : 3;  // tiles of a chunk: (q,) k, v
+  // Tiles of a chunk: (q,) k, v.  What the weighted keys leave goes where q was; forming sums, to P and the last slot in turn.
+  constexpr int NS = Cfg::SLOTS - (STATES ? 1 : 0), TILES = STATES ? 2 : 3;
   // (nothing else is in shared memory, so that this starts on a boundary of the swizzle's period; there is no room to move it)
   extern __shared__ __align__(1024) uint8_t mem[];
   const uint32_t base = smem_u32(mem);
@@ -130,9 +132,8 @@ __global__ void __launch_bounds__(LT_THREADS, 1) la_tc_kernel(const __grid_const
   auto empty = [&](int i) { return bars + 8u * (NS + i); };
   const uint32_t one = bars + 16u * NS;
   const uint32_t scores_ready = one, keys_ready = one + 8, pairs_ready = one + 16, inter_done = one + 24, delta_ready = one + 32,
-                 state_ready = one + 40, out_ready = one + 48, out_free = one + 56, all_done = one + 64, tail_ready = one + 72;
+                 state_ready = one + 40, out_ready = one + 48, out_free = one + 56, all_done = one + 64, tail_ready = one + 72, staged = one + 80, stored = one + 88;
   // A barrier's waiter can only tell one phase from the next.  Two barriers in turn where the other side can be a chunk ahead.
-  auto staged = [&](int c) { return one + 80 + 8u * (c & 1); };
   auto sum_keys_ready = [&](int c) { return c & 1 ? pairs_ready : keys_ready; };  // forming sums: keys two chunks ahead at most
   auto sum_done = [&](int c) { return c & 1 ? out_ready : inter_done; };          // and what they were added to
   float* const row_factor = reinterpret_cast<float*>(mem + Cfg::TABLES);
@@ -152,11 +153,11 @@ __global__ void __launch_bounds__(LT_THREADS, 1) la_tc_kernel(const __grid_const
       mbar_init(delta_ready, 1);
       mbar_init(state_ready, 256);
       mbar_init(out_ready, 1);
-      mbar_init(out_free, 128);
+      mbar_init(out_free, 256);
       mbar_init(all_done, 1);
       mbar_init(tail_ready, 256);
-      mbar_init(staged(0), 128);
-      mbar_init(staged(1), 128);
+      mbar_init(staged, 256);
+      mbar_init(stored, 1);
       fence_mbar_init();
     }
   } else if (warp == 1) {
@@ -247,7 +248,7 @@ __global__ void __launch_bounds__(LT_THREADS, 1) la_tc_kernel(const __grid_const
       // delta overwrites the columns that inter has read: no order holds between MMAs of different accumulators
       if (!STATES) mbar_wait(inter_done, c & 1, w, 116);
       tcgen05_fence_after();
-      const uint32_t rest = base + (STATES && (c & 1) ? Cfg::P : Cfg::KL);
+      const uint32_t rest = STATES ? base + (c & 1 ? NS * Cfg::SLOT : Cfg::P) : slot(kt - 1);
 #pragma unroll 2
       for (int x = 0; x < C / 8; ++x)
         umma_ss_warp(tm + TM_STATE, mn_major(v, x >> 1), mn_major(x & 1 ? rest : k, x >> 1), ID_DELTA, (STATES && c > 0) || x != 0, lead);
@@ -256,6 +257,7 @@ __global__ void __launch_bounds__(LT_THREADS, 1) la_tc_kernel(const __grid_const
         if (!STATES || c == chunks - 1) umma_commit(delta_ready);
         umma_commit(empty(kt % NS));
         umma_commit(empty(vt % NS));
+        if (!STATES) umma_commit(empty((kt - 1) % NS));
       }
       __syncwarp();
     }
@@ -263,17 +265,16 @@ __global__ void __launch_bounds__(LT_THREADS, 1) la_tc_kernel(const __grid_const
     if (lead) umma_commit(all_done);
     mbar_wait(all_done, 0, drain, 118);
   } else if (warp == 2) {
-    // ---- stores: outputs from the slot that held q, which is free after that
+    // ---- stores: outputs from where P was
     if (!STATES && lane == 0) {
       for (int c = 0; c < chunks; ++c) {
-        const int slot = (TILES * c) % NS;
-        if (!mbar_wait(staged(c), (c >> 1) & 1, w, 150)) break;
+        if (!mbar_wait(staged, c & 1, w, 150)) break;
         if (A.store[ji]) {
-          for (int k = 0; k < DO / 64; ++k) tma_store_4d(A.map[ji] + 3, base + slot * Cfg::SLOT + k * TILE, k * 64, chunk_at(c), h, b);
+          for (int k = 0; k < DO / 64; ++k) tma_store_4d(A.map[ji] + 3, base + Cfg::P + k * TILE, k * 64, chunk_at(c), h, b);
           bulk_commit();
           bulk_wait_read<0>();
         }
-        mbar_arrive(empty(slot));
+        mbar_arrive(stored);
       }
       bulk_wait_all<0>();
     }
@@ -281,8 +282,7 @@ __global__ void __launch_bounds__(LT_THREADS, 1) la_tc_kernel(const __grid_const
     // ---- keys weighted for the state, then scores weighted: a thread has half of row r of both
     regs_down<REGS_WEIGHT>();
     const int q = warp & 3, half = (warp - 4) >> 2, r = q * 32 + lane;
-    // a block of 32 keys seen by all, some or none of this warp's 32 tokens: j to q's one side, j == q, the other side
-    auto seen = [&](int j) { return rev ? j >= q : j <= q; };
+    // a block of 32 keys is seen by all, some or none of this warp's 32 tokens: j to q's one side, j == q, the other side
     auto pair_at = [&](int j) { return base + Cfg::P + (j >> 1) * TILE; };
     const int col = half * 16;  // of each block
     // Weights of scores, the same in every chunk.  The diagonal block's stand in registers.  Another block's are the power up to
@@ -294,15 +294,10 @@ __global__ void __launch_bounds__(LT_THREADS, 1) la_tc_kernel(const __grid_const
       const int far = rev ? col + s - lane : lane - col - s, far1 = rev ? far + 1 : far - 1;
       diagonal[s / 2] = pk2(far >= 0 ? J.pair_scale * g.power(far) : 0.f, far1 >= 0 ? J.pair_scale * g.power(far1) : 0.f);
     }
-    if (!STATES) {  // none: zero once and for all
-      for (int j = 0; j < 4; ++j)
-        if (!seen(j))
-          for (int i = 0; i < 2; ++i) sts128(pair_at(j) + sw128_offset(r, (j & 1) * 32 + col + 8 * i), 0, 0, 0, 0);
-    }
 #pragma unroll 1
     for (int c = 0; c < chunks; ++c) {
       const int t0 = chunk_at(c), n = min(C, end - t0), kt = TILES * c + TILES - 2, vt = kt + 1;
-      const uint32_t k = base + (kt % NS) * Cfg::SLOT, rest = base + (STATES && (c & 1) ? Cfg::P : Cfg::KL);
+      const uint32_t k = base + (kt % NS) * Cfg::SLOT, rest = base + (STATES ? (c & 1 ? NS * Cfg::SLOT : Cfg::P) : ((kt - 1) % NS) * Cfg::SLOT);
       const int steps = STATES ? (rev ? t0 + r - begin + 1 : end - 1 - t0 - r) : rev ? r + 1 : n - 1 - r;
       const float wk = r < n ? J.key_scale * g.power(steps) : 0.f;
       if (n < C) {
@@ -325,6 +320,7 @@ __global__ void __launch_bounds__(LT_THREADS, 1) la_tc_kernel(const __grid_const
       } else {
         mbar_wait(scores_ready, c & 1, w, 122);
         tcgen05_fence_after();
+        if (c > 0) mbar_wait(stored, (c - 1) & 1, w, 124);
       }
       if (!STATES) {
         const uint32_t from = tm + TM_SCORES + ((uint32_t)(q * 32) << 16) + col;
@@ -336,6 +332,9 @@ __global__ void __launch_bounds__(LT_THREADS, 1) la_tc_kernel(const __grid_const
         uint32_t x[16];
         f32x2 y[8];
         tmem_ld16(from + q * 32, x);
+#pragma unroll 1
+        for (int j = rev ? q - 1 : q + 1; rev ? j >= 0 : j < 4; j += rev ? -1 : 1)  // blocks that none of this warp's tokens see
+          for (int e = 0; e < 16; e += 8) sts128(pair_at(j) + sw128_offset(r, (j & 1) * 32 + col + e), 0, 0, 0, 0);
         tmem_ld_wait();
         // (selected: a score that is not finite may stand on the wrong side of the diagonal)
 #pragma unroll
@@ -364,6 +363,7 @@ __global__ void __launch_bounds__(LT_THREADS, 1) la_tc_kernel(const __grid_const
         tcgen05_fence_before();
         mbar_arrive(pairs_ready);
       }
+      if (!STATES) mbar_wait(inter_done, c & 1, w, 125);  // q has been read for the last time: the keys' rest goes there
       const f32x2 wk2 = pk2(wk, wk);
 #pragma unroll 1
       for (int i = half * (DI / 16); i < (half + 1) * (DI / 16); i += 2) {
@@ -381,24 +381,24 @@ __global__ void __launch_bounds__(LT_THREADS, 1) la_tc_kernel(const __grid_const
       fence_proxy_async_smem();
       mbar_arrive(STATES ? sum_keys_ready(c) : keys_ready);
     }
-  } else if (warp >= 12 && warp < 16) {
-    // ---- outputs: fragments of 32 columns by 16 tokens, turned by the matrix stores: [token][column] tiles in q's slot
+  } else if (warp >= 12 && warp < 20) {
+    // ---- outputs: fragments of 32 columns by 16 tokens, turned by the matrix stores: [token][column] tiles where P was;
+    // each of two warps with the same columns takes half of the tokens
     regs_down<REGS_OUT>();
     if (!STATES) {
-      const int q = warp - 12, r = tid - 384;
+      const int q = warp & 3, half = (warp - 12) >> 2, r = tid - 384, i0 = half * (C / 2);
       const size_t ld = (size_t)L.H * J.outer;
       __nv_bfloat16* const out = static_cast<__nv_bfloat16*>(J.out) + ((size_t)b * L.T * L.H + h) * J.outer;
       const uint32_t from = tm + ((uint32_t)(q * 32) << 16);
-      const uint32_t put = (q >> 1) * TILE + sw128_offset(lane & 7, (q & 1) * 32 + (lane >> 3) * 8);
+      const uint32_t put = base + Cfg::P + (q >> 1) * TILE + sw128_offset(lane & 7, (q & 1) * 32 + (lane >> 3) * 8);
       int have = 0;
 #pragma unroll 1
       for (int c = 0; c < chunks; ++c) {
         const int t0 = chunk_at(c), n = min(C, end - t0);
-        const uint32_t slot = base + ((TILES * c) % NS) * Cfg::SLOT;
         if (n != have) {  // factors of the rows: they change with the number of tokens only in reverse, and then once
-          named_bar_sync(1, 128);
-          row_factor[r] = r < n ? J.row_scale * g.power(rev ? n - 1 - r : r + 1) : 0.f;
-          named_bar_sync(1, 128);
+          named_bar_sync(1, 256);
+          if (r < C) row_factor[r] = r < n ? J.row_scale * g.power(rev ? n - 1 - r : r + 1) : 0.f;
+          named_bar_sync(1, 256);
           have = n;
         }
         mbar_wait(out_ready, c & 1, w, 130);
@@ -411,9 +411,9 @@ __global__ void __launch_bounds__(LT_THREADS, 1) la_tc_kernel(const __grid_const
             tmem_ld_frag2(from + TM_INTRA + i, y);
             tmem_ld_frag2(from + (16u << 16) + TM_INTRA + i, y + 8);
           };
-          fetch(0);
+          fetch(i0);
 #pragma unroll 1
-          for (int i = 0; i < C; i += 16) {
+          for (int i = i0; i < i0 + C / 2; i += 16) {
             const f32x2 f0 = *reinterpret_cast<const f32x2*>(row_factor + i + 2 * (lane & 3)),
                         f1 = *reinterpret_cast<const f32x2*>(row_factor + i + 8 + 2 * (lane & 3));
             tmem_ld_wait();
@@ -421,7 +421,7 @@ __global__ void __launch_bounds__(LT_THREADS, 1) la_tc_kernel(const __grid_const
 #pragma unroll
             for (int e = 0; e < 8; ++e)
               v[e] = pack2(fma2((e >> 1) & 1 ? f1 : f0, pk2u(x[2 * e], x[2 * e + 1]), pk2u(y[2 * e], y[2 * e + 1])));
-            if (i + 16 < C) {
+            if (i + 16 < i0 + C / 2) {
               fetch(i + 16);
             } else {  // all of it is in registers
               tcgen05_fence_before();
@@ -435,32 +435,33 @@ __global__ void __launch_bounds__(LT_THREADS, 1) la_tc_kernel(const __grid_const
                 if (t + 1 >= n) v[e] &= 0x0000ffffu;
               }
             }
-            stmatrix_x4_trans(slot + put + i * 128, v[0], v[1], v[4], v[5]);
-            stmatrix_x4_trans(slot + put + i * 128 + 1024, v[2], v[3], v[6], v[7]);
+            stmatrix_x4_trans(put + i * 128, v[0], v[1], v[4], v[5]);
+            stmatrix_x4_trans(put + i * 128 + 1024, v[2], v[3], v[6], v[7]);
           }
         } else {
           mbar_arrive(out_free);
         }
         if (!A.store[ji]) {  // widths and addresses that TMA does not take: element by element
-          named_bar_sync(1, 128);
+          named_bar_sync(1, 256);
+          const int o = r & 127;
 #pragma unroll 1
-          for (int t = 0; t < C && t0 + t < stop; ++t)
-            if (r < J.outer)
-              out[(size_t)(t0 + t) * ld + r] = *reinterpret_cast<const __nv_bfloat16*>(mem + (slot - base) + (r >> 6) * TILE + sw128_offset(t, r & 63));
+          for (int t = r >> 7; t < C && t0 + t < stop; t += 2)
+            if (o < J.outer)
+              out[(size_t)(t0 + t) * ld + o] = *reinterpret_cast<const __nv_bfloat16*>(mem + Cfg::P + (o >> 6) * TILE + sw128_offset(t, o & 63));
         }
         fence_proxy_async_smem();
-        mbar_arrive(staged(c));
+        mbar_arrive(staged);
       }
       // tokens behind the sequence, beyond its last chunk
 #pragma unroll 1
-      for (int t = begin + chunks * C; t < stop; ++t)
-        if (r < J.outer) out[(size_t)t * ld + r] = __float2bfloat16_rn(0.f);
+      for (int t = begin + chunks * C + (r >> 7); t < stop; t += 2)
+        if ((r & 127) < J.outer) out[(size_t)t * ld + (r & 127)] = __float2bfloat16_rn(0.f);
     }
-  } else if (warp >= 16) {
+  } else if (warp >= 20) {
     // ---- the state: a thread has half a row of S^T
     regs_up<REGS_STATE>();
     constexpr int N = DI / 2;
-    const int q = warp & 3, half = (warp - 16) >> 2, o = q * 32 + lane, i0 = half * N;
+    const int q = warp & 3, half = (warp - 20) >> 2, o = q * 32 + lane, i0 = half * N;
     const uint32_t mine = tm + TM_STATE + ((uint32_t)(q * 32) << 16) + half * N;
     const size_t mat = (size_t)at * J.inner * J.outer;
     f32x2 S[N / 2];
@@ -495,13 +496,11 @@ __global__ void __launch_bounds__(LT_THREADS, 1) la_tc_kernel(const __grid_const
           const f32x2 g_hi = all ? pk2(whole.hi, whole.hi) : pk2(rest.hi, rest.hi), g_lo = all ? pk2(whole.lo, whole.lo) : pk2(rest.lo, rest.lo);
           mbar_wait(delta_ready, (c - 1) & 1, w, 141);
           tcgen05_fence_after();
-          uint32_t x[2][16];
 #pragma unroll
           for (int i = 0; i < N; i += 16) {
-            if (i == 0) tmem_ld16(mine, x[0]);
+            uint32_t y[16];
+            tmem_ld16(mine + i, y);
             tmem_ld_wait();
-            if (i + 16 < N) tmem_ld16(mine + i + 16, x[(i / 16 + 1) & 1]);
-            const uint32_t* y = x[(i / 16) & 1];
 #pragma unroll
             for (int e = 0; e < 8; ++e) S[i / 2 + e] = fma2(g_hi, S[i / 2 + e], fma2(g_lo, S[i / 2 + e], pk2u(y[2 * e], y[2 * e + 1])));
           }
