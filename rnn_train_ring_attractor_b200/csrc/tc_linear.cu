@@ -20,8 +20,8 @@
 // role at a time, each at its own place in the code, and waits for instructions more than for anything else
 // once that outgrows the instruction cache (13 cycles for each instruction, with everything unrolled: 96 us instead of 82 for
 // 8 x 2048 tokens of 16 heads): loops stay rolled, pairs of fp32 are computed as such, and what only a partial chunk needs is done
-// apart.  The tensor pipe's order per chunk is scores, inter, intra, delta: the chain is inter, intra, delta, state, and the next
-// scores fill the pipe while the state warps work.  Tensor memory: 4 x 128 columns, scores | inter | intra | state, where delta
+// apart.  The tensor pipe's order is inter and intra of a chunk, the next one's scores, delta: the weights of the next
+// scores and keys are then formed while delta and the state follow.  Tensor memory: 4 x 128 columns, scores | inter | intra | state, where delta
 // is read from the columns that then receive the next operand.
 #include <string.h>
 
@@ -91,12 +91,6 @@ __device__ __forceinline__ uint32_t pack2(f32x2 v) {
   float a, b;
   upk2(v, a, b);
   return pack2(a, b);
-}
-__device__ __forceinline__ f32x2 unpack2(uint32_t v) { return pk2u(v << 16, v & 0xffff0000u); }
-// two fp32 as bf16, and what that leaves of them as bf16
-__device__ __forceinline__ void split2(f32x2 v, uint32_t* hi, uint32_t* lo) {
-  *hi = pack2(v);
-  *lo = pack2(fma2(unpack2(*hi), pk2(-1.f, -1.f), v));
 }
 template <int REGS>
 __device__ __forceinline__ void regs_down() { asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(REGS)); }
@@ -208,28 +202,19 @@ __global__ void __launch_bounds__(LT_THREADS, 1) la_tc_kernel(const __grid_const
     auto k_major = [&](uint32_t tile, int ks) { return desc_sw128(desc_lo(tile + (ks >> 2) * TILE + (ks & 3) * 32, 0)); };
     // M/N-major ones: 16 rows, blocks of 64 columns a tile apart
     auto mn_major = [&](uint32_t tile, int ks) { return desc_sw128(desc_lo(tile + ks * 2048, TILE)); };
-    // (loops are left rolled where their instructions keep up: see the note on roles)
+    // inter(c - 1), intra(c - 1), scores(c), delta(c - 1); loops are left rolled where their instructions keep up (see above)
 #pragma unroll 1
-    for (int c = 0; c < chunks; ++c) {
-      const int kt = TILES * c + TILES - 2, vt = kt + 1;
-      const uint32_t k = slot(kt), v = slot(vt);
-      if (!STATES) {
-        const uint32_t q = slot(kt - 1);
-        loaded(kt - 1, 110);
-        loaded(kt, 111);
-        if (chunk_at(c) + C > end) mbar_wait(tail_ready, 0, w, 119);
-        tcgen05_fence_after();
-#pragma unroll 2
-        for (int ks = 0; ks < DI / 16; ++ks) umma_ss_warp(tm + TM_SCORES, k_major(q, ks), k_major(k, ks), ID_SCORES, ks != 0, lead);
-        if (lead) umma_commit(scores_ready);
-        __syncwarp();
+    for (int i = STATES ? 1 : 0; i <= chunks; ++i) {
+      const int c = i - 1, kt = TILES * c + TILES - 2, vt = kt + 1;  // of the chunk before
+      if (!STATES && i > 0) {
         mbar_wait(state_ready, c & 1, w, 112);
         if (c > 0) mbar_wait(out_free, (c - 1) & 1, w, 113);
         tcgen05_fence_after();
         // the state's halves stand one behind the other, DI / 4 of DI / 2 columns each
 #pragma unroll 2
         for (int ks = 0; ks < DI / 16; ++ks)
-          umma_ts_warp(tm + TM_INTER, tm + TM_STATE + (ks / (DI / 32)) * (DI / 2) + (ks % (DI / 32)) * 8, k_major(q, ks), ID_INTER, ks != 0, lead);
+          umma_ts_warp(tm + TM_INTER, tm + TM_STATE + (ks / (DI / 32)) * (DI / 2) + (ks % (DI / 32)) * 8, k_major(slot(kt - 1), ks), ID_INTER,
+                       ks != 0, lead);
         if (lead) umma_commit(inter_done);
         __syncwarp();
         loaded(vt, 115);
@@ -237,29 +222,44 @@ __global__ void __launch_bounds__(LT_THREADS, 1) la_tc_kernel(const __grid_const
         tcgen05_fence_after();
 #pragma unroll 2
         for (int ks = 0; ks < C / 16; ++ks)
-          umma_ss_warp(tm + TM_INTRA, mn_major(v, ks), k_major(base + Cfg::P, ks), ID_INTRA, ks != 0, lead);
+          umma_ss_warp(tm + TM_INTRA, mn_major(slot(vt), ks), k_major(base + Cfg::P, ks), ID_INTRA, ks != 0, lead);
         if (lead) umma_commit(out_ready);
         __syncwarp();
-      } else {
-        loaded(vt, 115);
       }
-      if (STATES) mbar_wait(sum_keys_ready(c), (c >> 1) & 1, w, 114);
-      else mbar_wait(keys_ready, c & 1, w, 114);
-      // delta overwrites the columns that inter has read: no order holds between MMAs of different accumulators
-      if (!STATES) mbar_wait(inter_done, c & 1, w, 116);
-      tcgen05_fence_after();
-      const uint32_t rest = STATES ? base + (c & 1 ? NS * Cfg::SLOT : Cfg::P) : slot(kt - 1);
+      if (!STATES && i < chunks) {
+        const uint32_t q = slot(TILES * i), k = slot(TILES * i + 1);
+        loaded(TILES * i, 110);
+        loaded(TILES * i + 1, 111);
+        if (chunk_at(i) + C > end) mbar_wait(tail_ready, 0, w, 119);
+        tcgen05_fence_after();
 #pragma unroll 2
-      for (int x = 0; x < C / 8; ++x)
-        umma_ss_warp(tm + TM_STATE, mn_major(v, x >> 1), mn_major(x & 1 ? rest : k, x >> 1), ID_DELTA, (STATES && c > 0) || x != 0, lead);
-      if (lead) {
-        if (STATES) umma_commit(sum_done(c));
-        if (!STATES || c == chunks - 1) umma_commit(delta_ready);
-        umma_commit(empty(kt % NS));
-        umma_commit(empty(vt % NS));
-        if (!STATES) umma_commit(empty((kt - 1) % NS));
+        for (int ks = 0; ks < DI / 16; ++ks) umma_ss_warp(tm + TM_SCORES, k_major(q, ks), k_major(k, ks), ID_SCORES, ks != 0, lead);
+        if (lead) umma_commit(scores_ready);
+        __syncwarp();
       }
-      __syncwarp();
+      if (i > 0) {
+        if (STATES) {
+          loaded(vt, 115);
+          mbar_wait(sum_keys_ready(c), (c >> 1) & 1, w, 114);
+        } else {
+          mbar_wait(keys_ready, c & 1, w, 114);
+          // delta overwrites the columns that inter has read: no order holds between MMAs of different accumulators
+          mbar_wait(inter_done, c & 1, w, 116);
+        }
+        tcgen05_fence_after();
+        const uint32_t k = slot(kt), v = slot(vt), rest = STATES ? base + (c & 1 ? NS * Cfg::SLOT : Cfg::P) : slot(kt - 1);
+#pragma unroll 2
+        for (int x = 0; x < C / 8; ++x)
+          umma_ss_warp(tm + TM_STATE, mn_major(v, x >> 1), mn_major(x & 1 ? rest : k, x >> 1), ID_DELTA, (STATES && c > 0) || x != 0, lead);
+        if (lead) {
+          if (STATES) umma_commit(sum_done(c));
+          if (!STATES || c == chunks - 1) umma_commit(delta_ready);
+          umma_commit(empty(kt % NS));
+          umma_commit(empty(vt % NS));
+          if (!STATES) umma_commit(empty((kt - 1) % NS));
+        }
+        __syncwarp();
+      }
     }
     // tensor memory is given back below: nothing may still be writing it (at once, unless a wait was abandoned)
     if (lead) umma_commit(all_done);
@@ -336,9 +336,6 @@ __global__ void __launch_bounds__(LT_THREADS, 1) la_tc_kernel(const __grid_const
         for (int j = rev ? q - 1 : q + 1; rev ? j >= 0 : j < 4; j += rev ? -1 : 1)  // blocks that none of this warp's tokens see
           for (int e = 0; e < 16; e += 8) sts128(pair_at(j) + sw128_offset(r, (j & 1) * 32 + col + e), 0, 0, 0, 0);
         tmem_ld_wait();
-        // (selected: a score that is not finite may stand on the wrong side of the diagonal)
-#pragma unroll
-        for (int s = 0; s < 16; ++s) x[s] = (rev ? col + s >= lane : col + s <= lane) ? x[s] : 0u;
 #pragma unroll
         for (int s = 0; s < 8; ++s) y[s] = mul2(pk2u(x[2 * s], x[2 * s + 1]), diagonal[s]);
         put(q, y);
@@ -364,7 +361,10 @@ __global__ void __launch_bounds__(LT_THREADS, 1) la_tc_kernel(const __grid_const
         mbar_arrive(pairs_ready);
       }
       if (!STATES) mbar_wait(inter_done, c & 1, w, 125);  // q has been read for the last time: the keys' rest goes there
-      const f32x2 wk2 = pk2(wk, wk);
+      // k w = hi + lo with w = w_hi + w_lo, all bf16: hi = k w_hi rounded, what that leaves is exact in bf16 (eight bits of the
+      // sixteen), lo = k w_lo + that, rounded.  Three instructions for two elements, where the way through fp32 takes eight.
+      const __nv_bfloat16 w_hi = __float2bfloat16_rn(wk);
+      const __nv_bfloat162 wh = __bfloat162bfloat162(w_hi), wl = __bfloat162bfloat162(__float2bfloat16_rn(wk - __bfloat162float(w_hi)));
 #pragma unroll 1
       for (int i = half * (DI / 16); i < (half + 1) * (DI / 16); i += 2) {
         const uint32_t o0 = (i >> 3) * TILE + sw128_offset(r, (i & 7) * 8), o1 = (i >> 3) * TILE + sw128_offset(r, (i & 7) * 8 + 8);
@@ -372,7 +372,12 @@ __global__ void __launch_bounds__(LT_THREADS, 1) la_tc_kernel(const __grid_const
         const uint32_t x[8] = {x0.x, x0.y, x0.z, x0.w, x1.x, x1.y, x1.z, x1.w};
         uint32_t hi[8], lo[8];
 #pragma unroll
-        for (int e = 0; e < 8; ++e) split2(mul2(unpack2(x[e]), wk2), hi + e, lo + e);
+        for (int e = 0; e < 8; ++e) {
+          const __nv_bfloat162 y = *reinterpret_cast<const __nv_bfloat162*>(x + e), h2 = __hmul2_rn(y, wh);
+          const __nv_bfloat162 l2 = __hfma2(y, wl, __hfma2(y, wh, __hneg2(h2)));
+          hi[e] = *reinterpret_cast<const uint32_t*>(&h2);
+          lo[e] = *reinterpret_cast<const uint32_t*>(&l2);
+        }
         sts128(k + o0, hi[0], hi[1], hi[2], hi[3]);
         sts128(k + o1, hi[4], hi[5], hi[6], hi[7]);
         sts128(rest + o0, lo[0], lo[1], lo[2], lo[3]);

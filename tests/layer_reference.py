@@ -74,12 +74,15 @@ def attend_bounds(dtype, T, widest, tensor_cores):
 
     fp32 arithmetic: a product of two factors and a decay, summed over a head's width and over T tokens by way of chunks: at
     most T + widest + 16 roundings in a row (the decay's powers count for sixteen).
-    Tensor cores: scores of pairs rounded to bf16 (2^-8) and, beside those sums in fp32, weighted keys and states as two bf16 numbers
-    each: 2^-8 * 2^-8 = 2^-16 for each of the two."""
+    Tensor cores, beside those sums in fp32: scores of pairs, or the state, rounded to bf16 (2^-8; an output is a sum of products
+    of the two kinds).  A key k with its weight w is hi + lo: w as two bf16 numbers is off by 2^-8 * 2^-8 of it; hi = k w_hi
+    rounded leaves at most 2^-8, which is exact; lo, of that size, is rounded once more: 2^-8 * 2^-8 again.  Together 2^-15, with
+    a part in 2^7 for the products of these parts."""
     sums = (T + widest + 16) * 2.0 ** -23
     if not tensor_cores:
         return sums, sums
-    return 2.0 ** -8 + 2 * 2.0 ** -16 + sums, 2.0 ** -16 + sums
+    keys = 2.0 ** -15 * (1 + 2.0 ** -7)
+    return 2.0 ** -8 * (1 + 2 * keys) + keys + sums, keys + sums
 
 
 def philox(counter, key):
