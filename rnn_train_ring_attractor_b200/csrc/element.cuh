@@ -18,6 +18,20 @@ __device__ __forceinline__ __nv_bfloat16 down<__nv_bfloat16>(float x) { return _
 template <>
 __device__ __forceinline__ __half down<__half>(float x) { return __float2half_rn(x); }
 
+// two at a time: one conversion and no packing
+template <class E>
+__device__ __forceinline__ void down2(float a, float b, E* to) { to[0] = a, to[1] = b; }
+template <>
+__device__ __forceinline__ void down2<__nv_bfloat16>(float a, float b, __nv_bfloat16* to) {
+  const __nv_bfloat162 y = __floats2bfloat162_rn(a, b);
+  to[0] = y.x, to[1] = y.y;
+}
+template <>
+__device__ __forceinline__ void down2<__half>(float a, float b, __half* to) {
+  const __half2 y = __floats2half2_rn(a, b);
+  to[0] = y.x, to[1] = y.y;
+}
+
 template <class E, int V>
 struct alignas(sizeof(E) * V) Pack {
   E v[V];

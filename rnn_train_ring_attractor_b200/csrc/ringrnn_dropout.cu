@@ -12,13 +12,22 @@
 namespace ringrnn {
 namespace {
 
-__device__ __forceinline__ uint4 philox10(uint4 c, uint32_t k0, uint32_t k1) {
+// the ten rounds' keys: from the host they are constants of the launch, which an instruction takes as they are
+struct Keys {
+  uint32_t k[10][2];
+  __host__ __device__ explicit Keys(unsigned long long seed) {
+#pragma unroll
+    for (int i = 0; i < 10; ++i) {
+      k[i][0] = (uint32_t)seed + (uint32_t)i * 0x9E3779B9u;
+      k[i][1] = (uint32_t)(seed >> 32) + (uint32_t)i * 0xBB67AE85u;
+    }
+  }
+};
+__device__ __forceinline__ uint4 philox10(uint4 c, const Keys& key) {
 #pragma unroll
   for (int i = 0; i < 10; ++i) {
     const uint64_t a = (uint64_t)c.x * 0xD2511F53u, b = (uint64_t)c.z * 0xCD9E8D57u;
-    c = make_uint4((uint32_t)(b >> 32) ^ c.y ^ k0, (uint32_t)b, (uint32_t)(a >> 32) ^ c.w ^ k1, (uint32_t)a);
-    k0 += 0x9E3779B9u;
-    k1 += 0xBB67AE85u;
+    c = make_uint4((uint32_t)(b >> 32) ^ c.y ^ key.k[i][0], (uint32_t)b, (uint32_t)(a >> 32) ^ c.w ^ key.k[i][1], (uint32_t)a);
   }
   return c;
 }
@@ -26,54 +35,58 @@ __device__ __forceinline__ uint4 philox10(uint4 c, uint32_t k0, uint32_t k1) {
 struct DropoutArgs {
   long long n, packs;        // elements of a row; packs of V elements in it (the last may be short where V does not divide n)
   unsigned long long total;  // rows * packs
-  unsigned long long threshold;  // kept iff word >= threshold; 2^32 keeps nothing
+  long long step_rows, step_packs;  // what the grid's threads add up to, in whole rows and packs of one
+  uint32_t threshold;        // kept iff word >= threshold
+  bool none;                 // p = 1: nothing is kept
   float scale;
-  unsigned long long seed, stream_id;
-  const long long* seed_and_stream;
+  Keys keys;
+  uint32_t stream_id;
+  const long long* seed_and_stream;  // DEVICE_SEED: in the place of both
   unsigned long long first_row;
 };
 
 // V elements of one row at a time: a whole number of counters.  WHOLE: n is a multiple of V and addresses are aligned, so a pack
 // is one vector of each tensor.
-template <class E, int V, bool WHOLE>
-__global__ void __launch_bounds__(256) dropout_kernel(DropoutArgs a, const E* x, const E* residual, E* y) {
+template <class E, int V, bool WHOLE, bool RESIDUAL, bool DEVICE_SEED>
+__global__ void __launch_bounds__(256) dropout_kernel(const __grid_constant__ DropoutArgs a, const E* x, const E* residual, E* y) {
   typedef Pack<E, V> P;
-  unsigned long long seed = a.seed, stream_id = a.stream_id;
-  if (a.seed_and_stream != nullptr) {
-    seed = (unsigned long long)a.seed_and_stream[0];
-    stream_id = (unsigned long long)a.seed_and_stream[1];
-  }
+  const Keys own(DEVICE_SEED ? (unsigned long long)a.seed_and_stream[0] : 0ull);
+  const Keys& keys = DEVICE_SEED ? own : a.keys;
+  const uint32_t stream_id = DEVICE_SEED ? (uint32_t)a.seed_and_stream[1] : a.stream_id;
+  unsigned long long id = blockIdx.x * 256ULL + threadIdx.x;
   const unsigned long long step = gridDim.x * 256ULL;
-  for (unsigned long long id = blockIdx.x * 256ULL + threadIdx.x; id < a.total; id += step) {
-    // (32-bit division where it can be: half the instructions of a counter otherwise)
-    const unsigned long long row = (a.total >> 32) == 0 ? (unsigned)id / (unsigned)a.packs : id / (unsigned long long)a.packs;
-    const unsigned long long pack = id - row * a.packs;
-    const long long i = (long long)(row * a.n + pack * V);
-    const int here = WHOLE || (long long)pack * V + V <= a.n ? V : (int)(a.n - (long long)pack * V);
+  long long row = (long long)(id / (unsigned long long)a.packs), pack = (long long)id - row * a.packs;
+  for (; id < a.total; id += step) {
+    const long long i = row * a.n + pack * V;
+    const int here = WHOLE || pack * V + V <= a.n ? V : (int)(a.n - pack * V);
     P v, r;
     if constexpr (WHOLE) {
       v = *reinterpret_cast<const P*>(x + i);
-      if (residual != nullptr) r = *reinterpret_cast<const P*>(residual + i);
+      if (RESIDUAL) r = *reinterpret_cast<const P*>(residual + i);
     } else {
 #pragma unroll
       for (int e = 0; e < V; ++e) {
         v.v[e] = e < here ? x[i + e] : down<E>(0.f);
-        r.v[e] = residual != nullptr && e < here ? residual[i + e] : down<E>(0.f);
+        if (RESIDUAL) r.v[e] = e < here ? residual[i + e] : down<E>(0.f);
       }
     }
-    const unsigned long long in_all = a.first_row + row;
+    const unsigned long long in_all = a.first_row + (unsigned long long)row;
+    uint4 w[V / 4];
+#pragma unroll
+    for (int g = 0; g < V / 4; ++g)
+      w[g] = philox10(make_uint4((uint32_t)(pack * (V / 4) + g), stream_id, (uint32_t)in_all, (uint32_t)(in_all >> 32)), keys);
 #pragma unroll
     for (int g = 0; g < V / 4; ++g) {
-      const uint4 w = philox10(make_uint4((uint32_t)(pack * (V / 4) + g), (uint32_t)stream_id, (uint32_t)in_all, (uint32_t)(in_all >> 32)),
-                               (uint32_t)seed, (uint32_t)(seed >> 32));
-      const uint32_t word[4] = {w.x, w.y, w.z, w.w};
+      const uint32_t word[4] = {w[g].x, w[g].y, w[g].z, w[g].w};
+      float f[4];
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
         // selected, not multiplied by zero: an infinity that is dropped is gone
-        float f = word[e] >= a.threshold ? up(v.v[4 * g + e]) * a.scale : 0.f;
-        if (residual != nullptr) f += up(r.v[4 * g + e]);
-        v.v[4 * g + e] = down<E>(f);
+        f[e] = word[e] >= a.threshold && !a.none ? up(v.v[4 * g + e]) * a.scale : 0.f;
+        if (RESIDUAL) f[e] += up(r.v[4 * g + e]);
       }
+      down2(f[0], f[1], v.v + 4 * g);
+      down2(f[2], f[3], v.v + 4 * g + 2);
     }
     if constexpr (WHOLE) {
       *reinterpret_cast<P*>(y + i) = v;
@@ -82,10 +95,16 @@ __global__ void __launch_bounds__(256) dropout_kernel(DropoutArgs a, const E* x,
       for (int e = 0; e < V; ++e)
         if (e < here) y[i + e] = v.v[e];
     }
+    row += a.step_rows;
+    pack += a.step_packs;
+    if (pack >= a.packs) {
+      pack -= a.packs;
+      ++row;
+    }
   }
 }
 
-template <class E>
+template <class E, bool RESIDUAL, bool DEVICE_SEED>
 int launch(DropoutArgs a, long long rows, const void* x, const void* residual, void* y, cudaStream_t s) {
   constexpr int V = 16 / sizeof(E);
   const uintptr_t at = reinterpret_cast<uintptr_t>(x) | reinterpret_cast<uintptr_t>(residual) | reinterpret_cast<uintptr_t>(y);
@@ -93,12 +112,21 @@ int launch(DropoutArgs a, long long rows, const void* x, const void* residual, v
   a.packs = (a.n + V - 1) / V;
   a.total = (unsigned long long)rows * (unsigned long long)a.packs;
   const unsigned long long need = (a.total + 255) / 256;
-  const unsigned blocks = (unsigned)(need < 148 * 32 ? need : 148 * 32);
+  const unsigned blocks = (unsigned)(need < 148 * 16 ? need : 148 * 16);
+  a.step_rows = (long long)blocks * 256 / a.packs;
+  a.step_packs = (long long)blocks * 256 % a.packs;
   LaunchScope ls(K_LAYER, s);
-  if (whole) dropout_kernel<E, V, true><<<blocks, 256, 0, s>>>(a, static_cast<const E*>(x), static_cast<const E*>(residual), static_cast<E*>(y));
-  else dropout_kernel<E, V, false><<<blocks, 256, 0, s>>>(a, static_cast<const E*>(x), static_cast<const E*>(residual), static_cast<E*>(y));
+  const E *px = static_cast<const E*>(x), *pr = static_cast<const E*>(residual);
+  if (whole) dropout_kernel<E, V, true, RESIDUAL, DEVICE_SEED><<<blocks, 256, 0, s>>>(a, px, pr, static_cast<E*>(y));
+  else dropout_kernel<E, V, false, RESIDUAL, DEVICE_SEED><<<blocks, 256, 0, s>>>(a, px, pr, static_cast<E*>(y));
   RINGRNN_CUDA_TRY(cudaGetLastError());
   return RINGRNN_OK;
+}
+template <class E>
+int launch(const DropoutArgs& a, long long rows, const void* x, const void* residual, void* y, cudaStream_t s) {
+  const bool device_seed = a.seed_and_stream != nullptr;
+  return residual != nullptr ? (device_seed ? launch<E, true, true>(a, rows, x, residual, y, s) : launch<E, true, false>(a, rows, x, residual, y, s))
+                             : (device_seed ? launch<E, false, true>(a, rows, x, residual, y, s) : launch<E, false, false>(a, rows, x, residual, y, s));
 }
 
 }  // namespace
@@ -110,16 +138,10 @@ extern "C" int ringrnn_dropout(int dtype, long long rows, long long n, const voi
   using namespace ringrnn;
   if (rows <= 0 || n <= 0 || n > (1LL << 34) || rows > (1LL << 46) / n) return RINGRNN_ERR_SHAPE;
   if (!x || !y || !(p >= 0.0 && p <= 1.0) || (seed_and_stream == nullptr && stream_id > 0xFFFFFFFFull)) return RINGRNN_ERR_ARG;
-  DropoutArgs a;
-  a.n = n;
-  a.packs = 0;
-  a.total = 0;
-  a.threshold = (unsigned long long)rint(p * 4294967296.0);  // halves to even
-  a.scale = p < 1.0 ? (float)(1.0 / (1.0 - p)) : 0.f;
-  a.seed = seed;
-  a.stream_id = stream_id;
-  a.seed_and_stream = seed_and_stream;
-  a.first_row = first_row;
+  const unsigned long long threshold = (unsigned long long)rint(p * 4294967296.0);  // halves to even
+  const bool none = threshold > 0xFFFFFFFFull;
+  DropoutArgs a{n, 0, 0, 0, 0, (uint32_t)(none ? 0 : threshold), none, p < 1.0 ? (float)(1.0 / (1.0 - p)) : 0.f, Keys(seed),
+                (uint32_t)stream_id, seed_and_stream, first_row};
   cudaStream_t s = static_cast<cudaStream_t>(stream);
   switch (dtype) {
     case RINGRNN_F32: return launch<float>(a, rows, x, residual, y, s);

@@ -239,9 +239,11 @@ int scan_launch(const LaLaunch& L, int elems, int reverse, const float* init, fl
 // ---- one token ----------------------------------------------------------------------------------------------------------
 // Bound by the state, read and written once: 8 * dk * dv bytes per sequence and head.  A CTA takes 32 columns of one state:
 // they are independent of one another, a single head then spreads over dv / 32 SMs, and a row's part is a whole 128-byte line.
-// VEC = 4: a thread owns 4 columns of every 32nd row; VEC = 1 (odd widths or addresses): 1 column of every 8th.
-constexpr int STEP_THREADS = 256, STEP_COLS = 32, STEP_MAX_DK = 1024;
-template <class E, int VEC>
+// VEC = 4: a thread owns 4 columns of every THREADS / 8th row; VEC = 1 (odd widths or addresses): 1 column of every THREADS / 32nd.
+// Threads: as many as leave each four rows, all of them under way at once; a block for each 32 x 64 of a small state would be
+// half idle with 256 (256 sequences of 32 heads of 64: 62 us, and TODO with 128).
+constexpr int STEP_COLS = 32, STEP_MAX_DK = 1024;
+template <class E, int VEC, int STEP_THREADS>
 __global__ void __launch_bounds__(STEP_THREADS) la_step_kernel(int H, int dk, int dv, float scale, LaOperand q, LaOperand k,
                                                                LaOperand v, const float* __restrict__ log_decay,
                                                                const unsigned char* __restrict__ active,
@@ -318,17 +320,20 @@ __global__ void __launch_bounds__(STEP_THREADS) la_step_kernel(int H, int dk, in
     out[(size_t)bh * dv + blockIdx.y * STEP_COLS + tid] = down<E>(scale * x);
   }
 }
-template <class E>
+template <class E, int VEC, int THREADS>
 int step_launch(const RingRnnLinearAttention& p, const LaOperand& q, const LaOperand& k, const LaOperand& v, float* state,
                 const unsigned char* active, void* out, cudaStream_t s) {
   const dim3 grid(p.B * p.H, (p.dv + STEP_COLS - 1) / STEP_COLS);
   LaunchScope ls(K_LAYER, s);
-  if (p.dv % 4 == 0 && (reinterpret_cast<uintptr_t>(state) & 15) == 0)
-    la_step_kernel<E, 4><<<grid, STEP_THREADS, 0, s>>>(p.H, p.dk, p.dv, p.scale, q, k, v, p.log_decay, active, state, static_cast<E*>(out));
-  else
-    la_step_kernel<E, 1><<<grid, STEP_THREADS, 0, s>>>(p.H, p.dk, p.dv, p.scale, q, k, v, p.log_decay, active, state, static_cast<E*>(out));
+  la_step_kernel<E, VEC, THREADS><<<grid, THREADS, 0, s>>>(p.H, p.dk, p.dv, p.scale, q, k, v, p.log_decay, active, state, static_cast<E*>(out));
   RINGRNN_CUDA_TRY(cudaGetLastError());
   return RINGRNN_OK;
+}
+template <class E>
+int step_launch(const RingRnnLinearAttention& p, const LaOperand& q, const LaOperand& k, const LaOperand& v, float* state,
+                const unsigned char* active, void* out, cudaStream_t s) {
+  if (p.dv % 4 != 0 || (reinterpret_cast<uintptr_t>(state) & 15) != 0) return step_launch<E, 1, 256>(p, q, k, v, state, active, out, s);
+  return p.dk <= 64 ? step_launch<E, 4, 128>(p, q, k, v, state, active, out, s) : step_launch<E, 4, 256>(p, q, k, v, state, active, out, s);
 }
 
 // ---- host -----------------------------------------------------------------------------------------------------------------

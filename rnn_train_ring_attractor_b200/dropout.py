@@ -10,8 +10,8 @@ from torch.autograd import Function
 from torch.autograd.function import once_differentiable
 
 from . import _lib
-from .linear_attention import DTYPES
-from .ring_rnn_cuda import nvtx_range, on_device, stream_of
+from .linear_attention import DTYPES, raw_stream
+from .ring_rnn_cuda import nvtx_range, on_device
 
 
 def _call(x, residual, p, seed, stream, first_row):
@@ -25,7 +25,7 @@ def _call(x, residual, p, seed, stream, first_row):
         _lib.check(_lib.lib().ringrnn_dropout(
             DTYPES[x.dtype], rows, x.numel() // rows, x.data_ptr(), None if residual is None else residual.data_ptr(),
             y.data_ptr(), p, 0 if numbers is not None else seed, stream, None if numbers is None else numbers.data_ptr(),
-            first_row, stream_of(dev)))
+            first_row, raw_stream(dev.index)))
     return y
 
 

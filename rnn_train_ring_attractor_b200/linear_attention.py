@@ -7,23 +7,22 @@ to, and is read out linearly.  With rotary queries and keys (``rotary``) the sta
 reference has no counterpart; its comparison models are gated recurrent and softmax-attention networks (train/train_gru.py,
 train/train_causal_transformer.py).
 """
-import ctypes as C
-
 import torch
+from torch._C import _cuda_getCurrentRawStream as raw_stream
 from torch.autograd import Function
 from torch.autograd.function import once_differentiable
 
 from . import _lib
-from .ring_rnn_cuda import _scratch, nvtx_range, on_device, stream_of
+from .ring_rnn_cuda import nvtx_range, on_device
 
 DTYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
 MAX_WIDTH = 256
 
 
 def strided(t):
-    """RingRnnStrided of a [B, T, H, d] tensor whose last dimension is contiguous."""
-    b, n, h = t.stride()[:3]
-    return _lib.Strided(t.data_ptr(), b, n, h)
+    """The fields of RingRnnStrided for a [B, T, H, d] tensor whose last dimension is contiguous."""
+    b, n, h, _ = t.stride()
+    return t.data_ptr(), b, n, h
 
 
 def last_contiguous(t):
@@ -31,14 +30,15 @@ def last_contiguous(t):
 
 
 def _check(name, t, shape, device, dtype):
+    if t.is_cuda and t.device == device and t.dtype == dtype and t.shape == shape:
+        return
     if not t.is_cuda:
         raise RuntimeError(f"{name} must be a CUDA tensor (the operator has no CPU path)")
     if t.device != device:
         raise RuntimeError(f"{name} must be on {device}, like q")
     if t.dtype != dtype:
         raise RuntimeError(f"{name} must be {str(dtype).replace('torch.', '')}")
-    if tuple(t.shape) != shape:
-        raise RuntimeError(f"{name} must have shape {shape}")
+    raise RuntimeError(f"{name} must have shape {tuple(shape)}")
 
 
 def _check_state(name, t, shape, device):
@@ -52,44 +52,53 @@ def _check_qkv(q, k, v, log_decay, dims, widest):
         raise RuntimeError("q must be float32, bfloat16 or float16")
     if q.dim() != dims or k.dim() != dims or v.dim() != dims:
         raise RuntimeError(f"q, k and v must have {dims} dimensions")
-    lead, dk, dv = tuple(q.shape[:-1]), q.shape[-1], v.shape[-1]
-    _check("q", q, lead + (dk,), q.device, q.dtype)
-    _check("k", k, lead + (dk,), q.device, q.dtype)
-    _check("v", v, lead + (dv,), q.device, q.dtype)
+    lead, dk, dv, dev = q.shape[:-1], q.shape[-1], v.shape[-1], q.device
+    _check("q", q, q.shape, dev, q.dtype)
+    _check("k", k, q.shape, dev, q.dtype)
+    _check("v", v, (*lead, dv), dev, q.dtype)
     if not 1 <= dk <= widest or not 1 <= dv <= max(widest, MAX_WIDTH):
         raise RuntimeError(f"head widths must be between 1 and {widest}")
-    _check("log_decay", log_decay, (lead[-1],), q.device, torch.float32)
+    _check("log_decay", log_decay, (lead[-1],), dev, torch.float32)
     if log_decay.requires_grad and torch.is_grad_enabled():
         raise RuntimeError("log_decay has no gradient: the decays are constants of the layer (pass log_decay.detach())")
     return lead, dk, dv
 
 
+def _ptr(t):
+    return 0 if t is None else t.data_ptr()
+
+
 def _problem(q, k, v, log_decay, scale, lengths, initial_state):
     B, T, H, dk = q.shape
-    p = _lib.LinearAttention(B, T, H, dk, v.shape[-1], DTYPES[q.dtype], scale, strided(q), strided(k), strided(v),
-                             log_decay.data_ptr())
-    if lengths is not None:
-        p.lengths = lengths.data_ptr()
-    if initial_state is not None:
-        p.initial_state = initial_state.data_ptr()
-    return p
+    return _lib.LINEAR_ATTENTION.pack(B, T, H, dk, v.shape[-1], DTYPES[q.dtype], scale, *strided(q), *strided(k), *strided(v),
+                                      log_decay.data_ptr(), _ptr(lengths), _ptr(initial_state))
+
+
+def _workspace(n, dev):
+    """(tensor that owns n bytes, its address)"""
+    if n == _lib.INVALID_BYTES:
+        raise RuntimeError("linear_attention: batch, tokens or heads too large")
+    if n == 0:
+        return None, None
+    ws = torch.empty(n, dtype=torch.uint8, device=dev)
+    return ws, ws.data_ptr()
 
 
 def _forward(q, k, v, log_decay, scale, lengths, initial_state):
     B, T, H, dk = q.shape
     dv, dev = v.shape[-1], q.device
-    out = torch.empty(B, T, H, dv, device=dev, dtype=q.dtype)
-    final = torch.empty(B, H, dk, dv, device=dev, dtype=torch.float32)
+    out = torch.empty((B, T, H, dv), device=dev, dtype=q.dtype)
+    final = torch.empty((B, H, dk, dv), device=dev, dtype=torch.float32)
     if out.numel() == 0:  # no tokens or no sequences: the state is what it was
         return out, final.copy_(initial_state) if initial_state is not None else final.zero_()
     L = _lib.lib()
     with on_device(dev), nvtx_range("ringrnn_linear_attention_fwd"):
         p = _problem(q, k, v, log_decay, scale, lengths, initial_state)
-        n = L.ringrnn_linear_attention_bytes(C.byref(p), None)
-        if n == _lib.INVALID_BYTES:
-            raise RuntimeError("linear_attention: batch, tokens or heads too large")
-        ws = _scratch(n, dev)
-        _lib.check(L.ringrnn_linear_attention_fwd(C.byref(p), out.data_ptr(), final.data_ptr(), ws.data_ptr(), n, stream_of(dev)))
+        n = L.ringrnn_linear_attention_bytes(p, None)
+        ws, at = _workspace(n, dev)
+        rc = L.ringrnn_linear_attention_fwd(p, out.data_ptr(), final.data_ptr(), at, n, raw_stream(dev.index))
+        if rc:
+            _lib.check(rc)
     return out, final
 
 
@@ -123,12 +132,11 @@ class LinearAttentionFunc(Function):
         L = _lib.lib()
         with on_device(dev), nvtx_range("ringrnn_linear_attention_bwd"):
             p = _problem(q, k, v, log_decay, ctx.scale, lengths, initial_state)
-            g = strided(d_out)
-            n = L.ringrnn_linear_attention_bytes(C.byref(p), C.byref(g))
-            ws = _scratch(n, dev)
-            _lib.check(L.ringrnn_linear_attention_bwd(
-                C.byref(p), C.byref(g), None if d_final is None else d_final.data_ptr(), dq.data_ptr(), dk.data_ptr(),
-                dv.data_ptr(), None if d_initial is None else d_initial.data_ptr(), ws.data_ptr(), n, stream_of(dev)))
+            g = _lib.STRIDED.pack(*strided(d_out))
+            n = L.ringrnn_linear_attention_bytes(p, g)
+            ws, at = _workspace(n, dev)
+            _lib.check(L.ringrnn_linear_attention_bwd(p, g, _ptr(d_final), dq.data_ptr(), dk.data_ptr(), dv.data_ptr(),
+                                                      _ptr(d_initial), at, n, raw_stream(dev.index)))
         need = ctx.needs_input_grad
         return (dq if need[0] else None, dk if need[1] else None, dv if need[2] else None, d_initial, None, None, None)
 
@@ -148,7 +156,7 @@ def linear_attention(q, k, v, log_decay, scale=None, initial_state=None, lengths
     Gradients: q, k, v and initial_state, from those of out and final_state.
     """
     lead, dk, dv = _check_qkv(q, k, v, log_decay, 4, MAX_WIDTH)
-    B, T, H = lead
+    B, _, H = lead
     dev = q.device
     if initial_state is not None:
         _check_state("initial_state", initial_state, (B, H, dk, dv), dev)
@@ -180,17 +188,16 @@ def linear_attention_step(q, k, v, state, log_decay, scale=None, active=None):
         _check("active", active, (B,), dev, torch.bool)
         active = active.contiguous()
     q, k, v, log_decay = last_contiguous(q), last_contiguous(k), last_contiguous(v), log_decay.contiguous()
-    out = torch.empty(B, H, dv, device=dev, dtype=q.dtype)
+    out = torch.empty((B, H, dv), device=dev, dtype=q.dtype)
     if out.numel() == 0:
         return out
+    (qb, qh, _), (kb, kh, _), (vb, vh, _) = q.stride(), k.stride(), v.stride()
+    p = _lib.LINEAR_ATTENTION.pack(B, 1, H, dk, dv, DTYPES[q.dtype], dk ** -0.5 if scale is None else float(scale), q.data_ptr(),
+                                   qb, 0, qh, k.data_ptr(), kb, 0, kh, v.data_ptr(), vb, 0, vh, log_decay.data_ptr(), 0, 0)
     with on_device(dev):
-        p = _lib.LinearAttention(B, 1, H, dk, dv, DTYPES[q.dtype], dk ** -0.5 if scale is None else float(scale),
-                                 _lib.Strided(q.data_ptr(), q.stride(0), 0, q.stride(1)),
-                                 _lib.Strided(k.data_ptr(), k.stride(0), 0, k.stride(1)),
-                                 _lib.Strided(v.data_ptr(), v.stride(0), 0, v.stride(1)), log_decay.data_ptr())
-        _lib.check(_lib.lib().ringrnn_linear_attention_step(C.byref(p), state.data_ptr(),
-                                                            None if active is None else active.data_ptr(), out.data_ptr(),
-                                                            stream_of(dev)))
+        rc = _lib.lib().ringrnn_linear_attention_step(p, state.data_ptr(), _ptr(active), out.data_ptr(), raw_stream(dev.index))
+        if rc:
+            _lib.check(rc)
     if not state.is_inference():
         torch.autograd.graph.increment_version(state)  # an in-place update that torch has to know of
     return out

@@ -4,7 +4,6 @@ For the queries and keys of ``linear_attention`` (their products then depend on 
 head turns by a fixed angle each step beside its decay, as the ring network's bump is shifted by its left and right matrices
 (train/train_general_ring_no_gain.py:102-137).  The reference has no counterpart.
 """
-import ctypes as C
 import math
 
 import torch
@@ -12,8 +11,8 @@ from torch.autograd import Function
 from torch.autograd.function import once_differentiable
 
 from . import _lib
-from .linear_attention import DTYPES, last_contiguous, strided
-from .ring_rnn_cuda import nvtx_range, on_device, stream_of
+from .linear_attention import DTYPES, last_contiguous, raw_stream, strided
+from .ring_rnn_cuda import nvtx_range, on_device
 
 
 def rotary_frequencies(dim, base=10000.0, scaling=None, factor=1.0, trained_length=None, low=1.0, high=32.0, device="cuda"):
@@ -46,23 +45,21 @@ def _call(q, k, frequencies, positions, first, interleaved, amplitude, inverse):
     """positions: None or an integer tensor [B, T]."""
     B, T, Hq, D = q.shape
     dev = q.device
-    q_out = torch.empty(B, T, Hq, D, device=dev, dtype=q.dtype)
+    q_out = torch.empty((B, T, Hq, D), device=dev, dtype=q.dtype)
     k_out = None if k is None else torch.empty(k.shape, device=dev, dtype=k.dtype)
     if q_out.numel() == 0:
         return q_out, k_out
-    p = _lib.Rotary(B, T, Hq, 0 if k is None else k.shape[2], D, 2 * frequencies.shape[0], DTYPES[q.dtype], int(interleaved),
-                    int(inverse), amplitude, strided(q))
-    if k is not None:
-        p.k = strided(k)
-        p.k_out = k_out.data_ptr()
-    p.frequency = frequencies.data_ptr()
-    p.first = first
-    if positions is not None:
-        p.positions, p.position_bytes = positions.data_ptr(), positions.element_size()
-        p.position_batch, p.position_token = positions.stride()
-    p.q_out = q_out.data_ptr()
+    if positions is None:
+        where = 0, 0, 0, 0
+    else:
+        where = positions.data_ptr(), positions.element_size(), *positions.stride()
+    p = _lib.ROTARY.pack(B, T, Hq, 0 if k is None else k.shape[2], D, 2 * frequencies.shape[0], DTYPES[q.dtype], int(interleaved),
+                         int(inverse), amplitude, *strided(q), *((0, 0, 0, 0) if k is None else strided(k)), frequencies.data_ptr(),
+                         *where, first, q_out.data_ptr(), 0 if k is None else k_out.data_ptr())
     with on_device(dev), nvtx_range("ringrnn_rotary"):
-        _lib.check(_lib.lib().ringrnn_rotary(C.byref(p), stream_of(dev)))
+        rc = _lib.lib().ringrnn_rotary(p, raw_stream(dev.index))
+        if rc:
+            _lib.check(rc)
     return q_out, k_out
 
 

@@ -1,4 +1,6 @@
 """Linear attention with decay against its definition in 64 bits: sequences, gradients, single tokens, refusals."""
+import ctypes as C
+
 import pytest
 import torch
 
@@ -119,7 +121,7 @@ def test_long_sequences_of_few_heads(dtype, B, T, H, dk, dv):
         q, k, v, l, s, n, d_out, d_final = _inputs(dtype, B, T, H, dk, dv, seed=2, lengths=lengths)
         l[0] = -1e-3
         p = _lib.LinearAttention(B, T, H, dk, dv, 0, 1.0)
-        assert _lib.lib().ringrnn_linear_attention_bytes(p, None) > 0
+        assert _lib.lib().ringrnn_linear_attention_bytes(C.byref(p), None) > 0
         got, grads = _run(q, k, v, l, 0.3, s, n, d_out, d_final)
         _check_forward(got, q, k, v, l, 0.3, s, n)
         _check_grads(grads, q, k, v, l, 0.3, s, n, d_out, d_final)
@@ -384,7 +386,6 @@ def test_captured_and_replayed(T, H):
 
 def test_first_cuda_call_of_a_host_thread():
     """The library called from threads that have not touched the GPU before, as autograd's are."""
-    import ctypes as C
     import threading
     L = _lib.lib()
     q, k, v, l, s, n, _, _ = _inputs(BF16, 1, 70, 2, 64, 64)
@@ -404,7 +405,6 @@ def test_first_cuda_call_of_a_host_thread():
 
 def test_nothing_is_written_beyond_the_outputs():
     """Exact-size outputs inside a larger block, by the C entry points: what surrounds them stays."""
-    import ctypes as C
     L = _lib.lib()
     for dtype, code, B, T, H, dk, dv in ((BF16, 1, 2, 131, 2, 24, 40), (FP32, 0, 1, 45, 3, 7, 9), (BF16, 1, 1, 140, 1, 13, 99)):
         q, k, v, l, s, n, d_out, d_final = _inputs(dtype, B, T, H, dk, dv, seed=3)

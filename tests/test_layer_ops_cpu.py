@@ -92,6 +92,24 @@ def test_rotary_and_dropout_refuse_before_any_launch(L):
         assert drop(**bad) == 1, bad
 
 
+def test_structures_as_bytes_are_the_structures():
+    for packed, ctype in ((_lib.LINEAR_ATTENTION, _lib.LinearAttention), (_lib.STRIDED, _lib.Strided), (_lib.ROTARY, _lib.Rotary)):
+        assert packed.size == C.sizeof(ctype)
+
+    def fields(x):
+        for name, _ in x._fields_:
+            v = getattr(x, name)
+            if isinstance(v, C.Structure):
+                yield from fields(v)
+            else:
+                yield v
+    for packed, ctype in ((_lib.LINEAR_ATTENTION, _lib.LinearAttention), (_lib.ROTARY, _lib.Rotary)):
+        n = len(packed.unpack(bytes(packed.size)))
+        values = list(range(1, n + 1))
+        got = list(fields(ctype.from_buffer_copy(packed.pack(*values))))
+        assert got == values
+
+
 def test_python_surfaces_refuse_host_tensors():
     q = torch.zeros(1, 2, 1, 8)
     with pytest.raises(RuntimeError, match="CUDA"):
