@@ -11,21 +11,23 @@ from torch.autograd.function import once_differentiable
 
 from . import _lib
 from .linear_attention import DTYPES, raw_stream
-from .ring_rnn_cuda import nvtx_range, on_device
+from .ring_rnn_cuda import on_device
 
 
 def _call(x, residual, p, seed, stream, first_row):
-    y = torch.empty_like(x, memory_format=torch.contiguous_format)
+    y = torch.empty_like(x)  # (x is contiguous)
     if y.numel() == 0:
         return y
     rows = x.shape[0]
     dev = x.device
     numbers = seed if torch.is_tensor(seed) else None
-    with on_device(dev), nvtx_range("ringrnn_dropout"):
-        _lib.check(_lib.lib().ringrnn_dropout(
+    with on_device(dev):
+        rc = _lib.lib().ringrnn_dropout(
             DTYPES[x.dtype], rows, x.numel() // rows, x.data_ptr(), None if residual is None else residual.data_ptr(),
             y.data_ptr(), p, 0 if numbers is not None else seed, stream, None if numbers is None else numbers.data_ptr(),
-            first_row, raw_stream(dev.index)))
+            first_row, raw_stream(dev.index))
+        if rc:
+            _lib.check(rc)
     return y
 
 

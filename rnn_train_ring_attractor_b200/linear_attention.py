@@ -26,7 +26,17 @@ def strided(t):
 
 
 def last_contiguous(t):
-    return t if t.stride(-1) == 1 or t.shape[-1] == 1 else t.contiguous()
+    return t if t.is_contiguous() or t.stride(-1) == 1 or t.shape[-1] == 1 else t.contiguous()
+
+
+def new(dev, dtype, *shape):
+    """torch.empty(*shape), in less time."""
+    n, strides = 1, []
+    for d in reversed(shape):
+        strides.append(n)
+        n *= d or 1
+    strides.reverse()
+    return torch.empty_strided(shape, strides, device=dev, dtype=dtype)
 
 
 def _check(name, t, shape, device, dtype):
@@ -48,6 +58,13 @@ def _check_state(name, t, shape, device):
 
 
 def _check_qkv(q, k, v, log_decay, dims, widest):
+    shape, dev, dtype = q.shape, q.device, q.dtype
+    if (dtype in DTYPES and len(shape) == dims and v.dim() == dims and k.shape == shape and v.shape[:-1] == shape[:-1]
+            and k.dtype is dtype and v.dtype is dtype and q.is_cuda and k.device == dev and v.device == dev
+            and log_decay.dtype is torch.float32 and log_decay.device == dev and log_decay.shape == shape[-2:-1]
+            and 1 <= shape[-1] <= widest and 1 <= v.shape[-1] <= max(widest, MAX_WIDTH) and not log_decay.requires_grad):
+        return shape[:-1], shape[-1], v.shape[-1]
+    # one of them is wrong: which
     if q.dtype not in DTYPES:
         raise RuntimeError("q must be float32, bfloat16 or float16")
     if q.dim() != dims or k.dim() != dims or v.dim() != dims:
@@ -87,8 +104,8 @@ def _workspace(n, dev):
 def _forward(q, k, v, log_decay, scale, lengths, initial_state):
     B, T, H, dk = q.shape
     dv, dev = v.shape[-1], q.device
-    out = torch.empty((B, T, H, dv), device=dev, dtype=q.dtype)
-    final = torch.empty((B, H, dk, dv), device=dev, dtype=torch.float32)
+    out = new(dev, q.dtype, B, T, H, dv)
+    final = new(dev, torch.float32, B, H, dk, dv)
     if out.numel() == 0:  # no tokens or no sequences: the state is what it was
         return out, final.copy_(initial_state) if initial_state is not None else final.zero_()
     L = _lib.lib()
@@ -188,7 +205,7 @@ def linear_attention_step(q, k, v, state, log_decay, scale=None, active=None):
         _check("active", active, (B,), dev, torch.bool)
         active = active.contiguous()
     q, k, v, log_decay = last_contiguous(q), last_contiguous(k), last_contiguous(v), log_decay.contiguous()
-    out = torch.empty((B, H, dv), device=dev, dtype=q.dtype)
+    out = new(dev, q.dtype, B, H, dv)
     if out.numel() == 0:
         return out
     (qb, qh, _), (kb, kh, _), (vb, vh, _) = q.stride(), k.stride(), v.stride()

@@ -11,8 +11,8 @@ from torch.autograd import Function
 from torch.autograd.function import once_differentiable
 
 from . import _lib
-from .linear_attention import DTYPES, last_contiguous, raw_stream, strided
-from .ring_rnn_cuda import nvtx_range, on_device
+from .linear_attention import DTYPES, last_contiguous, new, raw_stream, strided
+from .ring_rnn_cuda import on_device
 
 
 def rotary_frequencies(dim, base=10000.0, scaling=None, factor=1.0, trained_length=None, low=1.0, high=32.0, device="cuda"):
@@ -45,8 +45,8 @@ def _call(q, k, frequencies, positions, first, interleaved, amplitude, inverse):
     """positions: None or an integer tensor [B, T]."""
     B, T, Hq, D = q.shape
     dev = q.device
-    q_out = torch.empty((B, T, Hq, D), device=dev, dtype=q.dtype)
-    k_out = None if k is None else torch.empty(k.shape, device=dev, dtype=k.dtype)
+    q_out = new(dev, q.dtype, B, T, Hq, D)
+    k_out = None if k is None else new(dev, k.dtype, *k.shape)
     if q_out.numel() == 0:
         return q_out, k_out
     if positions is None:
@@ -56,7 +56,7 @@ def _call(q, k, frequencies, positions, first, interleaved, amplitude, inverse):
     p = _lib.ROTARY.pack(B, T, Hq, 0 if k is None else k.shape[2], D, 2 * frequencies.shape[0], DTYPES[q.dtype], int(interleaved),
                          int(inverse), amplitude, *strided(q), *((0, 0, 0, 0) if k is None else strided(k)), frequencies.data_ptr(),
                          *where, first, q_out.data_ptr(), 0 if k is None else k_out.data_ptr())
-    with on_device(dev), nvtx_range("ringrnn_rotary"):
+    with on_device(dev):
         rc = _lib.lib().ringrnn_rotary(p, raw_stream(dev.index))
         if rc:
             _lib.check(rc)
