@@ -1,28 +1,30 @@
 // Linear attention with decay on tensor cores: bf16, widths up to 128 (padded to 64 or 128), chunks of 128 tokens.
 //
 // One CTA takes a (job, sequence, head, segment) and goes through its chunks with the state at hand; what a job is stands in
-// linear_attention.cuh.  Everything is computed transposed, outer columns on the tensor-memory lanes, so that the state never
-// leaves them (c: this chunk of n tokens; t, s: tokens in it; weights as in the forward, "reverse" mirrors them):
+// linear_attention.cuh.  A chunk of n tokens (t, s: tokens in it; weights as in the forward, "reverse" mirrors them):
 //
-//   scores   [t x s]      = Q K^T                                     both from shared memory
-//   inter^T  [outer x t]  = bf16(S^T) Q^T  S in tensor memory
-//   intra^T  [outer x t]  = V^T P^T        P_ts = bf16(scale g^(t-s) scores_ts), s <= t
-//   delta^T  [outer x in] = V^T K'         K'_s = g^(n-1-s) k_s = hi + lo, two bf16 numbers, beside each other in shared memory
-//   out_t    = row_scale g^(t+1) inter_t + intra_t                    S = g^n S + delta
+//   scores [t x s]      = Q K^T            both from shared memory
+//   inter  [t x outer]  = Q bf16(S)        S copied to shared memory; its rows are then scaled by row_scale g^(t+1), in place
+//   out    [t x outer] += P V              P_ts = bf16(scale g^(t-s) scores_ts), s <= t, in tensor memory where the scores were
+//   delta  [in x outer] = K'^T V           K'_s = g^(n-1-s) k_s = hi + lo, two bf16 numbers, transposed into tensor memory
+//   S = g^n S + delta
 //
 // Precision: the state is fp32 (registers) and what is added to it keeps sixteen bits, so that states passed from call to call
 // and their gradients are good for what fp32 is for: 2e-6 of their size, where keys rounded to bf16 would leave 2e-3.  Where it
 // only goes into bf16 outputs the state is rounded to bf16, like P: next to the outputs' own rounding that costs a factor of 1.4
 // in their error, a second product for the rest of the state would make it 1.1 and take 512 of a chunk's cycles.
 //
-// Roles (28 warps): 0 TMA loads; 1 MMA issue; 2 TMA stores; 4-11 weight the scores and the keys (in place, the rest where q was);
-// 12-19 bring the outputs to shared memory (where P was); 20-27 keep the state, half a row each.  A scheduler has two warps of a
-// role at a time, each at its own place in the code, and waits for instructions more than for anything else
-// once that outgrows the instruction cache (13 cycles for each instruction, with everything unrolled: 96 us instead of 82 for
-// 8 x 2048 tokens of 16 heads): loops stay rolled, pairs of fp32 are computed as such, and what only a partial chunk needs is done
-// apart.  The tensor pipe's order is inter and intra of a chunk, the next one's scores, delta: the weights of the next
-// scores and keys are then formed while delta and the state follow.  Tensor memory: 4 x 128 columns, scores | inter | intra | state, where delta
-// is read from the columns that then receive the next operand.
+// What bounds it: at widths of 128 the memory (a chunk is 128 KB, 5500 cycles of an SM's share at 6.5 TB/s); then shared memory's
+// 128 bytes per cycle, which products with both operands there use up.  P and K' therefore live in tensor memory, and V is all
+// that is read beside them: 3600 cycles of shared memory per chunk, where the transposed arrangement (columns on the lanes, so that
+// the state is the operand in tensor memory, P and K' in shared memory) took 5200 and was bound by that.
+//
+// Roles (28 warps): 0 TMA loads; 1 MMA issue; 2 TMA stores; 4-11 weight the keys and the scores; 12-19 scale inter and bring the
+// outputs to shared memory (where k was); 20-27 keep the state, half a row each.  A scheduler has two warps of a role at a time,
+// each at its own place in the code, and waits for instructions more than for anything else once that outgrows the instruction
+// cache (13 cycles for each instruction, with everything unrolled): loops stay rolled, pairs of fp32 are computed as such, and
+// what only a partial chunk needs is done apart.  The tensor pipe's order is inter, delta, out, the next scores: the chain of a
+// chunk is inter, delta, state, and the rest fills its gaps.
 #include <string.h>
 
 #include "linear_attention.cuh"
@@ -34,24 +36,24 @@ namespace {
 using namespace tc;
 
 constexpr int C = LA_TC_CHUNK;
-constexpr int TILE = C * 128;  // bytes of [128 tokens x 64 columns]
+constexpr int TILE = C * 128;  // bytes of [128 rows x 64 columns]
 constexpr int LT_THREADS = 896;
 // registers of warps 0-3, 4-11, 12-19, 20-27 (setmaxnreg): no more than the block is launched with
 constexpr int REGS_ISSUE = 32, REGS_WEIGHT = 72, REGS_OUT = 64, REGS_STATE = 96;
 static_assert((4 * REGS_ISSUE + 8 * REGS_WEIGHT + 8 * REGS_OUT + 8 * REGS_STATE) * 32 <= 65536 / LT_THREADS / 8 * 8 * LT_THREADS, "registers");
-constexpr uint32_t TM_SCORES = 0, TM_INTER = 128, TM_INTRA = 256, TM_STATE = 384, TM_COLS = 512;
+// tensor memory: scores, of each 16 columns the first 8 then P; inter and outputs; delta; K' (hi, lo)
+constexpr uint32_t TM_SCORES = 0, TM_OUT = 128, TM_DELTA = 256, TM_KEYS = 384, TM_COLS = 512;
 
 template <int DI, int DO>
 struct LtCfg {
   static constexpr int WIDE = DI > DO ? DI : DO;
   static constexpr int SLOT = TILE * (WIDE / 64);
   static constexpr int SLOTS = WIDE == 128 ? 6 : 12;  // two chunks' q, k and v or four's: what it takes to keep the memory busy
-  // slots | P, then the outputs on their way.  The last v may be followed by what the MMAs read in place of rows that nobody uses,
-  // so another buffer stands behind the slots.
-  static constexpr int P = SLOT * SLOTS, BARS = P + 2 * TILE;
-  static constexpr int TABLES = BARS + (2 * SLOTS + 12) * 8 + 32;  // 128 row factors, 32 powers
+  // slots | the state as operand | barriers and tables.  A product reads 128 rows of K' whatever DI is; nobody uses what it makes of the others.
+  static constexpr int STATE = SLOT * SLOTS, BARS = STATE + 2 * TILE;
+  static constexpr int TABLES = BARS + (2 * SLOTS + 12) * 8 + 32;  // 32 powers; key weights of 64 pairs of tokens
   static_assert(TABLES % 16 == 0, "alignment");
-  static constexpr int FLAGS = TABLES + 640;
+  static constexpr int FLAGS = TABLES + 128 + 512;
   static constexpr int SMEM = FLAGS + 16;
   static_assert(SMEM <= 232448, "shared memory of a block");
 };
@@ -59,8 +61,8 @@ struct LtCfg {
 struct LtParams {
   LaLaunch L;
   int h_step[LA_MAX_JOBS][3], b_step[LA_MAX_JOBS][3];  // 0: a tensor that all heads / sequences share
-  int store[LA_MAX_JOBS];  // out can be written by TMA
-  alignas(64) CUtensorMap map[LA_MAX_JOBS][4];  // q, k, v, out
+  int store[LA_MAX_JOBS];                              // out can be written by TMA
+  alignas(64) CUtensorMap map[LA_MAX_JOBS][4];         // q, k, v, out
 };
 
 __device__ __forceinline__ void tma_load_4d(uint32_t dst, const CUtensorMap* m, uint32_t bar, int x, int t, int h, int b) {
@@ -74,11 +76,6 @@ __device__ __forceinline__ void tma_store_4d(const CUtensorMap* m, uint32_t src,
                    reinterpret_cast<uint64_t>(m)),
                "r"(src), "r"(x), "r"(t), "r"(h), "r"(b)
                : "memory");
-}
-__device__ __forceinline__ uint4 lds128(uint32_t a) {
-  uint4 v;
-  asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(a) : "memory");
-  return v;
 }
 __device__ __forceinline__ void sts128(uint32_t a, uint32_t x, uint32_t y, uint32_t z, uint32_t w) {
   asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(a), "r"(x), "r"(y), "r"(z), "r"(w) : "memory");
@@ -100,8 +97,7 @@ __device__ __forceinline__ void regs_up() { asm volatile("setmaxnreg.inc.sync.al
 template <int DI, int DO, bool STATES>
 __global__ void __launch_bounds__(LT_THREADS, 1) la_tc_kernel(const __grid_constant__ LtParams A, volatile int* host_status) {
   using Cfg = LtCfg<DI, DO>;
-  // Tiles of a chunk: (q,) k, v.  What the weighted keys leave goes where q was; forming sums, to P and the last slot in turn.
-  constexpr int NS = Cfg::SLOTS - (STATES ? 1 : 0), TILES = STATES ? 2 : 3;
+  constexpr int NS = Cfg::SLOTS, TILES = STATES ? 2 : 3;  // tiles of a chunk: (q,) k, v
   // (nothing else is in shared memory, so that this starts on a boundary of the swizzle's period; there is no room to move it)
   extern __shared__ __align__(1024) uint8_t mem[];
   const uint32_t base = smem_u32(mem);
@@ -126,12 +122,14 @@ __global__ void __launch_bounds__(LT_THREADS, 1) la_tc_kernel(const __grid_const
   auto empty = [&](int i) { return bars + 8u * (NS + i); };
   const uint32_t one = bars + 16u * NS;
   const uint32_t scores_ready = one, keys_ready = one + 8, pairs_ready = one + 16, inter_done = one + 24, delta_ready = one + 32,
-                 state_ready = one + 40, out_ready = one + 48, out_free = one + 56, all_done = one + 64, tail_ready = one + 72, staged = one + 80, stored = one + 88;
+                 state_ready = one + 40, out_ready = one + 48, out_free = one + 56, all_done = one + 64, tail_ready = one + 72,
+                 staged = one + 80, scaled = one + 88;
   // A barrier's waiter can only tell one phase from the next.  Two barriers in turn where the other side can be a chunk ahead.
   auto sum_keys_ready = [&](int c) { return c & 1 ? pairs_ready : keys_ready; };  // forming sums: keys two chunks ahead at most
   auto sum_done = [&](int c) { return c & 1 ? out_ready : inter_done; };          // and what they were added to
-  float* const row_factor = reinterpret_cast<float*>(mem + Cfg::TABLES);
-  float* const powers = row_factor + C;
+  auto sum_keys = [&](int c) { return c & 1 ? TM_SCORES : TM_KEYS; };
+  float* const powers = reinterpret_cast<float*>(mem + Cfg::TABLES);
+  uint2* const key_weights = reinterpret_cast<uint2*>(powers + 32);  // of tokens 2i and 2i + 1: what bf16 keeps of them, the rest
 
   if (warp == 0) {
     if (lane == 0) {
@@ -151,7 +149,7 @@ __global__ void __launch_bounds__(LT_THREADS, 1) la_tc_kernel(const __grid_const
       mbar_init(all_done, 1);
       mbar_init(tail_ready, 256);
       mbar_init(staged, 256);
-      mbar_init(stored, 1);
+      mbar_init(scaled, 256);
       fence_mbar_init();
     }
   } else if (warp == 1) {
@@ -194,70 +192,74 @@ __global__ void __launch_bounds__(LT_THREADS, 1) la_tc_kernel(const __grid_const
   } else if (warp == 1) {
     // ---- MMAs, issued by the whole warp (see umma_ts_warp)
     const uint32_t lead = elect_one();
-    constexpr uint32_t ID_SCORES = make_idesc_bf16(128, 128, 0, 0), ID_INTER = make_idesc_bf16(128, 128, 0, 0),
-                       ID_DELTA = make_idesc_bf16(128, DI, 1, 1), ID_INTRA = make_idesc_bf16(128, 128, 1, 0);
+    constexpr uint32_t ID_SCORES = make_idesc_bf16(128, 128, 0, 0), ID_OUT = make_idesc_bf16(128, DO, 0, 1);
     auto slot = [&](int tile) { return base + (tile % NS) * Cfg::SLOT; };
     auto loaded = [&](int tile, int code) { mbar_wait(full(tile % NS), (tile / NS) & 1, w, code); };
     // K-major operands: 16 of the 64 columns of a 128-byte row at a time
     auto k_major = [&](uint32_t tile, int ks) { return desc_sw128(desc_lo(tile + (ks >> 2) * TILE + (ks & 3) * 32, 0)); };
     // M/N-major ones: 16 rows, blocks of 64 columns a tile apart
     auto mn_major = [&](uint32_t tile, int ks) { return desc_sw128(desc_lo(tile + ks * 2048, TILE)); };
-    // inter(c - 1), intra(c - 1), scores(c), delta(c - 1); loops are left rolled where their instructions keep up (see above)
+    // inter(c - 1), delta(c - 1), out(c - 1), scores(c); loops are left rolled where their instructions keep up (see above)
 #pragma unroll 1
     for (int i = STATES ? 1 : 0; i <= chunks; ++i) {
       const int c = i - 1, kt = TILES * c + TILES - 2, vt = kt + 1;  // of the chunk before
-      if (!STATES && i > 0) {
-        mbar_wait(state_ready, c & 1, w, 112);
-        if (c > 0) mbar_wait(out_free, (c - 1) & 1, w, 113);
-        tcgen05_fence_after();
-        // the state's halves stand one behind the other, DI / 4 of DI / 2 columns each
+      if (i > 0) {
+        if (!STATES) {
+          mbar_wait(state_ready, c & 1, w, 112);
+          if (c > 0) mbar_wait(out_free, (c - 1) & 1, w, 113);
+          tcgen05_fence_after();
 #pragma unroll 2
-        for (int ks = 0; ks < DI / 16; ++ks)
-          umma_ts_warp(tm + TM_INTER, tm + TM_STATE + (ks / (DI / 32)) * (DI / 2) + (ks % (DI / 32)) * 8, k_major(slot(kt - 1), ks), ID_INTER,
-                       ks != 0, lead);
-        if (lead) umma_commit(inter_done);
-        __syncwarp();
-        loaded(vt, 115);
-        mbar_wait(pairs_ready, c & 1, w, 117);
+          for (int ks = 0; ks < DI / 16; ++ks)
+            umma_ss_warp(tm + TM_OUT, k_major(slot(kt - 1), ks), mn_major(base + Cfg::STATE, ks), ID_OUT, ks != 0, lead);
+          if (lead) {
+            umma_commit(inter_done);
+            umma_commit(empty((kt - 1) % NS));
+          }
+          __syncwarp();
+          loaded(vt, 115);
+          mbar_wait(keys_ready, c & 1, w, 114);
+        } else {
+          loaded(vt, 115);
+          mbar_wait(sum_keys_ready(c), (c >> 1) & 1, w, 114);
+        }
         tcgen05_fence_after();
+        const uint32_t keys = tm + (STATES ? sum_keys(c) : TM_KEYS), v = slot(vt);
 #pragma unroll 2
-        for (int ks = 0; ks < C / 16; ++ks)
-          umma_ss_warp(tm + TM_INTRA, mn_major(slot(vt), ks), k_major(base + Cfg::P, ks), ID_INTRA, ks != 0, lead);
-        if (lead) umma_commit(out_ready);
+        for (int x = 0; x < C / 8; ++x)
+          umma_ts_warp(tm + TM_DELTA, keys + (x & 1) * 64 + (x >> 1) * 8, mn_major(v, x >> 1), ID_OUT, (STATES && c > 0) || x != 0, lead);
+        if (lead) {
+          if (STATES) umma_commit(sum_done(c));
+          if (!STATES || c == chunks - 1) umma_commit(delta_ready);
+          if (STATES) {
+            umma_commit(empty(kt % NS));
+            umma_commit(empty(vt % NS));
+          }
+        }
         __syncwarp();
+        if (!STATES) {
+          mbar_wait(scaled, c & 1, w, 116);
+          mbar_wait(pairs_ready, c & 1, w, 117);
+          tcgen05_fence_after();
+#pragma unroll 2
+          for (int ks = 0; ks < C / 16; ++ks) umma_ts_warp(tm + TM_OUT, tm + TM_SCORES + 16 * ks, mn_major(v, ks), ID_OUT, true, lead);
+          if (lead) {
+            umma_commit(out_ready);
+            umma_commit(empty(vt % NS));
+          }
+          __syncwarp();
+        }
       }
       if (!STATES && i < chunks) {
         const uint32_t q = slot(TILES * i), k = slot(TILES * i + 1);
         loaded(TILES * i, 110);
         loaded(TILES * i + 1, 111);
         if (chunk_at(i) + C > end) mbar_wait(tail_ready, 0, w, 119);
+        // the scores go where out has just read P: no order holds between MMAs of different accumulators
+        if (i > 0) mbar_wait(out_ready, c & 1, w, 118);
         tcgen05_fence_after();
 #pragma unroll 2
         for (int ks = 0; ks < DI / 16; ++ks) umma_ss_warp(tm + TM_SCORES, k_major(q, ks), k_major(k, ks), ID_SCORES, ks != 0, lead);
         if (lead) umma_commit(scores_ready);
-        __syncwarp();
-      }
-      if (i > 0) {
-        if (STATES) {
-          loaded(vt, 115);
-          mbar_wait(sum_keys_ready(c), (c >> 1) & 1, w, 114);
-        } else {
-          mbar_wait(keys_ready, c & 1, w, 114);
-          // delta overwrites the columns that inter has read: no order holds between MMAs of different accumulators
-          mbar_wait(inter_done, c & 1, w, 116);
-        }
-        tcgen05_fence_after();
-        const uint32_t k = slot(kt), v = slot(vt), rest = STATES ? base + (c & 1 ? NS * Cfg::SLOT : Cfg::P) : slot(kt - 1);
-#pragma unroll 2
-        for (int x = 0; x < C / 8; ++x)
-          umma_ss_warp(tm + TM_STATE, mn_major(v, x >> 1), mn_major(x & 1 ? rest : k, x >> 1), ID_DELTA, (STATES && c > 0) || x != 0, lead);
-        if (lead) {
-          if (STATES) umma_commit(sum_done(c));
-          if (!STATES || c == chunks - 1) umma_commit(delta_ready);
-          umma_commit(empty(kt % NS));
-          umma_commit(empty(vt % NS));
-          if (!STATES) umma_commit(empty((kt - 1) % NS));
-        }
         __syncwarp();
       }
     }
@@ -265,26 +267,25 @@ __global__ void __launch_bounds__(LT_THREADS, 1) la_tc_kernel(const __grid_const
     if (lead) umma_commit(all_done);
     mbar_wait(all_done, 0, drain, 118);
   } else if (warp == 2) {
-    // ---- stores: outputs from where P was
+    // ---- stores: outputs from the slot that held k, which is free after that
     if (!STATES && lane == 0) {
       for (int c = 0; c < chunks; ++c) {
+        const int slot = (TILES * c + 1) % NS;
         if (!mbar_wait(staged, c & 1, w, 150)) break;
         if (A.store[ji]) {
-          for (int k = 0; k < DO / 64; ++k) tma_store_4d(A.map[ji] + 3, base + Cfg::P + k * TILE, k * 64, chunk_at(c), h, b);
+          for (int k = 0; k < DO / 64; ++k) tma_store_4d(A.map[ji] + 3, base + slot * Cfg::SLOT + k * TILE, k * 64, chunk_at(c), h, b);
           bulk_commit();
           bulk_wait_read<0>();
         }
-        mbar_arrive(stored);
+        mbar_arrive(empty(slot));
       }
       bulk_wait_all<0>();
     }
   } else if (warp >= 4 && warp < 12) {
-    // ---- keys weighted for the state, then scores weighted: a thread has half of row r of both
+    // ---- keys, transposed and weighted for the state, then scores weighted
     regs_down<REGS_WEIGHT>();
-    const int q = warp & 3, half = (warp - 4) >> 2, r = q * 32 + lane;
-    // a block of 32 keys is seen by all, some or none of this warp's 32 tokens: j to q's one side, j == q, the other side
-    auto pair_at = [&](int j) { return base + Cfg::P + (j >> 1) * TILE; };
-    const int col = half * 16;  // of each block
+    const int q = warp & 3, half = (warp - 4) >> 2, r = q * 32 + lane, a = tid - 128;
+    const int col = half * 16;  // scores: a thread has row r and these 16 of each 32 columns
     // Weights of scores, the same in every chunk.  The diagonal block's stand in registers.  Another block's are the power up to
     // its near end, a factor per token (32 tokens more: times g^32), times one within the block: all at most one.
     f32x2 diagonal[8];
@@ -294,15 +295,14 @@ __global__ void __launch_bounds__(LT_THREADS, 1) la_tc_kernel(const __grid_const
       const int far = rev ? col + s - lane : lane - col - s, far1 = rev ? far + 1 : far - 1;
       diagonal[s / 2] = pk2(far >= 0 ? J.pair_scale * g.power(far) : 0.f, far1 >= 0 ? J.pair_scale * g.power(far1) : 0.f);
     }
+    int have = 0;
 #pragma unroll 1
     for (int c = 0; c < chunks; ++c) {
       const int t0 = chunk_at(c), n = min(C, end - t0), kt = TILES * c + TILES - 2, vt = kt + 1;
-      const uint32_t k = base + (kt % NS) * Cfg::SLOT, rest = base + (STATES ? (c & 1 ? NS * Cfg::SLOT : Cfg::P) : ((kt - 1) % NS) * Cfg::SLOT);
-      const int steps = STATES ? (rev ? t0 + r - begin + 1 : end - 1 - t0 - r) : rev ? r + 1 : n - 1 - r;
-      const float wk = r < n ? J.key_scale * g.power(steps) : 0.f;
+      const uint32_t k = base + (kt % NS) * Cfg::SLOT;
+      mbar_wait(full(kt % NS), (kt / NS) & 1, w, 120);
       if (n < C) {
         // what stands behind the sequence, a NaN included, becomes zero before anybody reads it
-        mbar_wait(full(kt % NS), (kt / NS) & 1, w, 120);
         mbar_wait(full(vt % NS), (vt / NS) & 1, w, 123);
         if (r >= n) {
           const uint32_t v = base + (vt % NS) * Cfg::SLOT;
@@ -311,38 +311,83 @@ __global__ void __launch_bounds__(LT_THREADS, 1) la_tc_kernel(const __grid_const
         }
         fence_proxy_async_smem();
         if (!STATES) mbar_arrive(tail_ready);
-        else named_bar_sync(2, 256);
       }
-      if (STATES) {
-        mbar_wait(full(kt % NS), (kt / NS) & 1, w, 120);
-        // the sum of two chunks before has read its keys' rest
-        if (c > 1) mbar_wait(sum_done(c), ((c >> 1) - 1) & 1, w, 121);
-      } else {
+      if (STATES || n != have) {  // the keys' weights: they change with the number of tokens, and towards a segment's end
+        named_bar_sync(1, 256);
+        if (a < 64) {
+          float x[2], rest[2];
+          __nv_bfloat16 y[2];
+#pragma unroll
+          for (int e = 0; e < 2; ++e) {
+            const int s = 2 * a + e;
+            const int steps = STATES ? (rev ? t0 + s - begin + 1 : end - 1 - t0 - s) : rev ? s + 1 : n - 1 - s;
+            x[e] = s < n ? J.key_scale * g.power(steps) : 0.f;
+            y[e] = __float2bfloat16_rn(x[e]);
+            rest[e] = x[e] - __bfloat162float(y[e]);
+          }
+          key_weights[a] = make_uint2(pack2(x[0], x[1]), pack2(rest[0], rest[1]));
+        }
+        named_bar_sync(1, 256);
+        have = n;
+      }
+      // what read the last keys: the chunk before's delta; forming sums, of two chunks before
+      if (STATES ? c > 1 : c > 0) {
+        if (STATES) mbar_wait(sum_done(c), ((c >> 1) - 1) & 1, w, 121);
+        else mbar_wait(delta_ready, (c - 1) & 1, w, 121);
+        tcgen05_fence_after();
+      }
+      if (q * 32 < DI) {
+        // k w = hi + lo with w = w_hi + w_lo, all bf16: hi = k w_hi rounded, what that leaves is exact in bf16 (eight bits of the
+        // sixteen), lo = k w_lo + that, rounded.  Three instructions for two elements, where the way through fp32 takes eight.
+        const int row = half * 64 + (lane >> 4) * 8 + (lane & 7), in = (q & 1) * 32 + ((lane >> 3) & 1) * 8;  // matrices: two of tokens by two of columns
+        const uint32_t from = k + (q >> 1) * TILE, to = tm + (STATES ? sum_keys(c) : TM_KEYS) + ((uint32_t)(q * 32) << 16) + half * 32;
+        const uint2* kw = key_weights + half * 32 + (lane & 3);
+#pragma unroll 1
+        for (int x = 0; x < 4; ++x) {  // 16 columns by 32 tokens
+          const int i = x >> 1, j = x & 1;
+          uint32_t hi[8], lo[8];
+#pragma unroll
+          for (int m = 0; m < 2; ++m) {
+            uint32_t y[4];
+            ldmatrix_x4_trans(from + sw128_offset(row + j * 32 + m * 16, in + i * 16), y);
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+              const uint2 wt = kw[(j * 4 + m * 2 + (e >> 1)) * 4];
+              const __nv_bfloat162 wh = *reinterpret_cast<const __nv_bfloat162*>(&wt.x), wl = *reinterpret_cast<const __nv_bfloat162*>(&wt.y),
+                                   z = *reinterpret_cast<const __nv_bfloat162*>(y + e), h2 = __hmul2_rn(z, wh),
+                                   l2 = __hfma2(z, wl, __hfma2(z, wh, __hneg2(h2)));
+              hi[m * 4 + e] = *reinterpret_cast<const uint32_t*>(&h2);
+              lo[m * 4 + e] = *reinterpret_cast<const uint32_t*>(&l2);
+            }
+          }
+          tmem_st_frag4(to + ((uint32_t)(i * 16) << 16) + j * 16, hi);
+          tmem_st_frag4(to + ((uint32_t)(i * 16) << 16) + 64 + j * 16, lo);
+        }
+        tmem_st_wait();
+        tcgen05_fence_before();
+      }
+      mbar_arrive(STATES ? sum_keys_ready(c) : keys_ready);
+      if (!STATES) {
         mbar_wait(scores_ready, c & 1, w, 122);
         tcgen05_fence_after();
-        if (c > 0) mbar_wait(stored, (c - 1) & 1, w, 124);
-      }
-      if (!STATES) {
-        const uint32_t from = tm + TM_SCORES + ((uint32_t)(q * 32) << 16) + col;
-        auto put = [&](int j, const f32x2* y) {
-#pragma unroll
-          for (int e = 0; e < 8; e += 4)
-            sts128(pair_at(j) + sw128_offset(r, (j & 1) * 32 + col + 2 * e), pack2(y[e]), pack2(y[e + 1]), pack2(y[e + 2]), pack2(y[e + 3]));
-        };
+        const uint32_t mine = tm + TM_SCORES + ((uint32_t)(q * 32) << 16) + col;
         uint32_t x[16];
         f32x2 y[8];
-        tmem_ld16(from + q * 32, x);
-#pragma unroll 1
-        for (int j = rev ? q - 1 : q + 1; rev ? j >= 0 : j < 4; j += rev ? -1 : 1)  // blocks that none of this warp's tokens see
-          for (int e = 0; e < 16; e += 8) sts128(pair_at(j) + sw128_offset(r, (j & 1) * 32 + col + e), 0, 0, 0, 0);
+        auto put = [&](int j) {
+          uint32_t z[8];
+#pragma unroll
+          for (int e = 0; e < 8; ++e) z[e] = pack2(y[e]);
+          tmem_st8(mine + j * 32, z);
+        };
+        tmem_ld16(mine + q * 32, x);
         tmem_ld_wait();
 #pragma unroll
         for (int s = 0; s < 8; ++s) y[s] = mul2(pk2u(x[2 * s], x[2 * s + 1]), diagonal[s]);
-        put(q, y);
+        put(q);
         float f = near;
 #pragma unroll 1
         for (int j = rev ? q + 1 : q - 1; rev ? j < 4 : j >= 0; j += rev ? 1 : -1) {
-          tmem_ld16(from + j * 32, x);
+          tmem_ld16(mine + j * 32, x);
           const f32x2 f2 = pk2(f, f);
           f *= g32;
 #pragma unroll
@@ -354,129 +399,101 @@ __global__ void __launch_bounds__(LT_THREADS, 1) la_tc_kernel(const __grid_const
           tmem_ld_wait();
 #pragma unroll
           for (int s = 0; s < 8; ++s) y[s] = mul2(pk2u(x[2 * s], x[2 * s + 1]), y[s]);
-          put(j, y);
+          put(j);
         }
-        fence_proxy_async_smem();
+#pragma unroll
+        for (int e = 0; e < 8; ++e) x[e] = 0u;
+#pragma unroll 1
+        for (int j = rev ? q - 1 : q + 1; rev ? j >= 0 : j < 4; j += rev ? -1 : 1) tmem_st8(mine + j * 32, x);  // what none of these tokens sees
+        tmem_st_wait();
         tcgen05_fence_before();
         mbar_arrive(pairs_ready);
       }
-      if (!STATES) mbar_wait(inter_done, c & 1, w, 125);  // q has been read for the last time: the keys' rest goes there
-      // k w = hi + lo with w = w_hi + w_lo, all bf16: hi = k w_hi rounded, what that leaves is exact in bf16 (eight bits of the
-      // sixteen), lo = k w_lo + that, rounded.  Three instructions for two elements, where the way through fp32 takes eight.
-      const __nv_bfloat16 w_hi = __float2bfloat16_rn(wk);
-      const __nv_bfloat162 wh = __bfloat162bfloat162(w_hi), wl = __bfloat162bfloat162(__float2bfloat16_rn(wk - __bfloat162float(w_hi)));
-#pragma unroll 1
-      for (int i = half * (DI / 16); i < (half + 1) * (DI / 16); i += 2) {
-        const uint32_t o0 = (i >> 3) * TILE + sw128_offset(r, (i & 7) * 8), o1 = (i >> 3) * TILE + sw128_offset(r, (i & 7) * 8 + 8);
-        const uint4 x0 = lds128(k + o0), x1 = lds128(k + o1);
-        const uint32_t x[8] = {x0.x, x0.y, x0.z, x0.w, x1.x, x1.y, x1.z, x1.w};
-        uint32_t hi[8], lo[8];
-#pragma unroll
-        for (int e = 0; e < 8; ++e) {
-          const __nv_bfloat162 y = *reinterpret_cast<const __nv_bfloat162*>(x + e), h2 = __hmul2_rn(y, wh);
-          const __nv_bfloat162 l2 = __hfma2(y, wl, __hfma2(y, wh, __hneg2(h2)));
-          hi[e] = *reinterpret_cast<const uint32_t*>(&h2);
-          lo[e] = *reinterpret_cast<const uint32_t*>(&l2);
-        }
-        sts128(k + o0, hi[0], hi[1], hi[2], hi[3]);
-        sts128(k + o1, hi[4], hi[5], hi[6], hi[7]);
-        sts128(rest + o0, lo[0], lo[1], lo[2], lo[3]);
-        sts128(rest + o1, lo[4], lo[5], lo[6], lo[7]);
-      }
-      fence_proxy_async_smem();
-      mbar_arrive(STATES ? sum_keys_ready(c) : keys_ready);
     }
   } else if (warp >= 12 && warp < 20) {
-    // ---- outputs: fragments of 32 columns by 16 tokens, turned by the matrix stores: [token][column] tiles where P was;
-    // each of two warps with the same columns takes half of the tokens
+    // ---- outputs: a thread has token r and half of its columns.  Inter is scaled; later the sum goes to shared memory
     regs_down<REGS_OUT>();
     if (!STATES) {
-      const int q = warp & 3, half = (warp - 12) >> 2, r = tid - 384, i0 = half * (C / 2);
+      constexpr int N = DO / 2;
+      const int q = warp & 3, half = (warp - 12) >> 2, r = q * 32 + lane, a = tid - 384, o0 = half * N;
       const size_t ld = (size_t)L.H * J.outer;
       __nv_bfloat16* const out = static_cast<__nv_bfloat16*>(J.out) + ((size_t)b * L.T * L.H + h) * J.outer;
-      const uint32_t from = tm + ((uint32_t)(q * 32) << 16);
-      const uint32_t put = base + Cfg::P + (q >> 1) * TILE + sw128_offset(lane & 7, (q & 1) * 32 + (lane >> 3) * 8);
-      int have = 0;
+      const uint32_t mine = tm + TM_OUT + ((uint32_t)(q * 32) << 16) + o0;
 #pragma unroll 1
       for (int c = 0; c < chunks; ++c) {
         const int t0 = chunk_at(c), n = min(C, end - t0);
-        if (n != have) {  // factors of the rows: they change with the number of tokens only in reverse, and then once
-          named_bar_sync(1, 256);
-          if (r < C) row_factor[r] = r < n ? J.row_scale * g.power(rev ? n - 1 - r : r + 1) : 0.f;
-          named_bar_sync(1, 256);
-          have = n;
-        }
-        mbar_wait(out_ready, c & 1, w, 130);
+        const int slot = ((TILES * c + 1) % NS) * Cfg::SLOT;
+        const float f = r < n ? J.row_scale * g.power(rev ? n - 1 - r : r + 1) : 0.f;
+        const f32x2 f2 = pk2(f, f);
+        mbar_wait(inter_done, c & 1, w, 130);
         tcgen05_fence_after();
-        if (q * 32 < DO) {
-          uint32_t x[16], y[16];
-          auto fetch = [&](int i) {
-            tmem_ld_frag2(from + TM_INTER + i, x);
-            tmem_ld_frag2(from + (16u << 16) + TM_INTER + i, x + 8);
-            tmem_ld_frag2(from + TM_INTRA + i, y);
-            tmem_ld_frag2(from + (16u << 16) + TM_INTRA + i, y + 8);
-          };
-          fetch(i0);
 #pragma unroll 1
-          for (int i = i0; i < i0 + C / 2; i += 16) {
-            const f32x2 f0 = *reinterpret_cast<const f32x2*>(row_factor + i + 2 * (lane & 3)),
-                        f1 = *reinterpret_cast<const f32x2*>(row_factor + i + 8 + 2 * (lane & 3));
-            tmem_ld_wait();
-            uint32_t v[8];  // of 16 columns (half), 8 tokens, 8 columns: half * 4 + tokens * 2 + columns
+        for (int i = 0; i < N; i += 16) {
+          uint32_t x[16];
+          tmem_ld16(mine + i, x);
+          tmem_ld_wait();
 #pragma unroll
-            for (int e = 0; e < 8; ++e)
-              v[e] = pack2(fma2((e >> 1) & 1 ? f1 : f0, pk2u(x[2 * e], x[2 * e + 1]), pk2u(y[2 * e], y[2 * e + 1])));
-            if (i + 16 < i0 + C / 2) {
-              fetch(i + 16);
-            } else {  // all of it is in registers
-              tcgen05_fence_before();
-              mbar_arrive(out_free);
-            }
-            if (i + 16 > n) {
-#pragma unroll
-              for (int e = 0; e < 8; ++e) {
-                const int t = i + ((e >> 1) & 1) * 8 + 2 * (lane & 3);
-                if (t >= n) v[e] &= 0xffff0000u;
-                if (t + 1 >= n) v[e] &= 0x0000ffffu;
-              }
-            }
-            stmatrix_x4_trans(put + i * 128, v[0], v[1], v[4], v[5]);
-            stmatrix_x4_trans(put + i * 128 + 1024, v[2], v[3], v[6], v[7]);
+          for (int e = 0; e < 16; e += 2) {
+            float y, z;
+            upk2(mul2(f2, pk2u(x[e], x[e + 1])), y, z);
+            x[e] = __float_as_uint(y), x[e + 1] = __float_as_uint(z);
           }
-        } else {
-          mbar_arrive(out_free);
+          tmem_st8(mine + i, x);
+          tmem_st8(mine + i + 8, x + 8);
+        }
+        tmem_st_wait();
+        tcgen05_fence_before();
+        mbar_arrive(scaled);
+        mbar_wait(out_ready, c & 1, w, 131);
+        tcgen05_fence_after();
+        const uint32_t to = base + slot + (o0 >> 6) * TILE;
+#pragma unroll 1
+        for (int i = 0; i < N; i += 16) {
+          uint32_t x[16];
+          tmem_ld16(mine + i, x);
+          tmem_ld_wait();
+          if (i + 16 == N) {  // all of it is in registers
+            tcgen05_fence_before();
+            mbar_arrive(out_free);
+          }
+          uint32_t y[8];
+#pragma unroll
+          for (int e = 0; e < 8; ++e) y[e] = r < n ? pack2(__uint_as_float(x[2 * e]), __uint_as_float(x[2 * e + 1])) : 0u;
+          sts128(to + sw128_offset(r, (o0 & 63) + i), y[0], y[1], y[2], y[3]);
+          sts128(to + sw128_offset(r, (o0 & 63) + i + 8), y[4], y[5], y[6], y[7]);
         }
         if (!A.store[ji]) {  // widths and addresses that TMA does not take: element by element
-          named_bar_sync(1, 256);
-          const int o = r & 127;
+          named_bar_sync(2, 256);
+          const int o = a & 127;
 #pragma unroll 1
-          for (int t = r >> 7; t < C && t0 + t < stop; t += 2)
+          for (int t = a >> 7; t < C && t0 + t < stop; t += 2)
             if (o < J.outer)
-              out[(size_t)(t0 + t) * ld + o] = *reinterpret_cast<const __nv_bfloat16*>(mem + Cfg::P + (o >> 6) * TILE + sw128_offset(t, o & 63));
+              out[(size_t)(t0 + t) * ld + o] = *reinterpret_cast<const __nv_bfloat16*>(mem + slot + (o >> 6) * TILE + sw128_offset(t, o & 63));
         }
         fence_proxy_async_smem();
         mbar_arrive(staged);
       }
       // tokens behind the sequence, beyond its last chunk
 #pragma unroll 1
-      for (int t = begin + chunks * C + (r >> 7); t < stop; t += 2)
-        if ((r & 127) < J.outer) out[(size_t)t * ld + (r & 127)] = __float2bfloat16_rn(0.f);
+      for (int t = begin + chunks * C + (a >> 7); t < stop; t += 2)
+        if ((a & 127) < J.outer) out[(size_t)t * ld + (a & 127)] = __float2bfloat16_rn(0.f);
     }
   } else if (warp >= 20) {
-    // ---- the state: a thread has half a row of S^T
+    // ---- the state: a thread has half a row
     regs_up<REGS_STATE>();
-    constexpr int N = DI / 2;
-    const int q = warp & 3, half = (warp - 20) >> 2, o = q * 32 + lane, i0 = half * N;
-    const uint32_t mine = tm + TM_STATE + ((uint32_t)(q * 32) << 16) + half * N;
+    constexpr int N = DO / 2;
+    const int q = warp & 3, half = (warp - 20) >> 2, in = q * 32 + lane, o0 = half * N;
+    const uint32_t mine = tm + TM_DELTA + ((uint32_t)(q * 32) << 16) + o0;
+    const uint32_t to = base + Cfg::STATE + (o0 >> 6) * TILE;
     const size_t mat = (size_t)at * J.inner * J.outer;
     f32x2 S[N / 2];
     {
-      const float* from = J.init + mat + (size_t)o * J.s_out;
-      const bool given = !STATES && J.init != nullptr && o < J.outer;
+      const float* from = J.init + mat + (size_t)in * J.s_in;
+      const bool given = !STATES && J.init != nullptr && in < J.inner;
 #pragma unroll
       for (int i = 0; i < N; i += 2)
-        S[i / 2] = pk2(given && i0 + i < J.inner ? from[(size_t)(i0 + i) * J.s_in] : 0.f,
-                       given && i0 + i + 1 < J.inner ? from[(size_t)(i0 + i + 1) * J.s_in] : 0.f);
+        S[i / 2] = pk2(given && o0 + i < J.outer ? from[(size_t)(o0 + i) * J.s_out] : 0.f,
+                       given && o0 + i + 1 < J.outer ? from[(size_t)(o0 + i + 1) * J.s_out] : 0.f);
     }
     if (STATES) {
       if (chunks > 0) {
@@ -510,28 +527,26 @@ __global__ void __launch_bounds__(LT_THREADS, 1) la_tc_kernel(const __grid_const
             for (int e = 0; e < 8; ++e) S[i / 2 + e] = fma2(g_hi, S[i / 2 + e], fma2(g_lo, S[i / 2 + e], pk2u(y[2 * e], y[2 * e + 1])));
           }
         }
-        if (c < chunks) {  // the next operand
+        if (c < chunks) {  // the next operand (delta of this chunk is behind inter, which has read the last one)
+          if (in < DI) {
 #pragma unroll
-          for (int i = 0; i < N; i += 16) {
-            uint32_t x[8];
-#pragma unroll
-            for (int e = 0; e < 8; ++e) x[e] = pack2(S[i / 2 + e]);
-            tmem_st8(mine + i / 2, x);
+            for (int i = 0; i < N; i += 8)
+              sts128(to + sw128_offset(in, (o0 & 63) + i), pack2(S[i / 2]), pack2(S[i / 2 + 1]), pack2(S[i / 2 + 2]), pack2(S[i / 2 + 3]));
           }
-          tmem_st_wait();
+          fence_proxy_async_smem();
           tcgen05_fence_before();
           mbar_arrive(state_ready);
         }
       }
     }
-    if (J.fin != nullptr && o < J.outer) {
-      float* to = J.fin + mat + (size_t)o * J.s_out;
+    if (J.fin != nullptr && in < J.inner) {
+      float* fin = J.fin + mat + (size_t)in * J.s_in;
 #pragma unroll
       for (int i = 0; i < N; i += 2) {
         float x, y;
         upk2(S[i / 2], x, y);
-        if (i0 + i < J.inner) to[(size_t)(i0 + i) * J.s_in] = x;
-        if (i0 + i + 1 < J.inner) to[(size_t)(i0 + i + 1) * J.s_in] = y;
+        if (o0 + i < J.outer) fin[(size_t)(o0 + i) * J.s_out] = x;
+        if (o0 + i + 1 < J.outer) fin[(size_t)(o0 + i + 1) * J.s_out] = y;
       }
     }
   }
