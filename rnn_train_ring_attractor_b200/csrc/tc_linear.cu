@@ -89,6 +89,17 @@ __device__ __forceinline__ uint32_t pack2(f32x2 v) {
   upk2(v, a, b);
   return pack2(a, b);
 }
+// 32 bytes: a whole sector of each lane's own row
+__device__ __forceinline__ void ldg8(const float* p, float* x) {
+  asm volatile("ld.global.v8.f32 {%0, %1, %2, %3, %4, %5, %6, %7}, [%8];"
+               : "=f"(x[0]), "=f"(x[1]), "=f"(x[2]), "=f"(x[3]), "=f"(x[4]), "=f"(x[5]), "=f"(x[6]), "=f"(x[7])
+               : "l"(p));
+}
+__device__ __forceinline__ void stg8(float* p, const float* x) {
+  asm volatile("st.global.v8.f32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(p), "f"(x[0]), "f"(x[1]), "f"(x[2]), "f"(x[3]), "f"(x[4]),
+               "f"(x[5]), "f"(x[6]), "f"(x[7])
+               : "memory");
+}
 template <int REGS>
 __device__ __forceinline__ void regs_down() { asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(REGS)); }
 template <int REGS>
@@ -486,14 +497,25 @@ __global__ void __launch_bounds__(LT_THREADS, 1) la_tc_kernel(const __grid_const
     const uint32_t mine = tm + TM_DELTA + ((uint32_t)(q * 32) << 16) + o0;
     const uint32_t to = base + Cfg::STATE + (o0 >> 6) * TILE;
     const size_t mat = (size_t)at * J.inner * J.outer;
+    // rows of a state in its own order are read and written a sector at a time (the transposed ones come lane by lane)
+    auto rows_of_sectors = [&](const float* p) { return J.s_out == 1 && (J.outer & 7) == 0 && (reinterpret_cast<uintptr_t>(p) & 31) == 0; };
     f32x2 S[N / 2];
     {
-      const float* from = J.init + mat + (size_t)in * J.s_in;
-      const bool given = !STATES && J.init != nullptr && in < J.inner;
+      const float* from = J.init + mat + (size_t)in * J.s_in + (size_t)o0 * J.s_out;
+      const bool given = !STATES && J.init != nullptr && in < J.inner, sectors = rows_of_sectors(J.init);
 #pragma unroll
-      for (int i = 0; i < N; i += 2)
-        S[i / 2] = pk2(given && o0 + i < J.outer ? from[(size_t)(o0 + i) * J.s_out] : 0.f,
-                       given && o0 + i + 1 < J.outer ? from[(size_t)(o0 + i + 1) * J.s_out] : 0.f);
+      for (int i = 0; i < N; i += 8) {
+        float x[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+        if (given && sectors) {
+          if (o0 + i < J.outer) ldg8(from + i, x);
+        } else if (given) {
+#pragma unroll
+          for (int e = 0; e < 8; ++e)
+            if (o0 + i + e < J.outer) x[e] = from[(size_t)(i + e) * J.s_out];
+        }
+#pragma unroll
+        for (int e = 0; e < 8; e += 2) S[(i + e) / 2] = pk2(x[e], x[e + 1]);
+      }
     }
     if (STATES) {
       if (chunks > 0) {
@@ -540,13 +562,20 @@ __global__ void __launch_bounds__(LT_THREADS, 1) la_tc_kernel(const __grid_const
       }
     }
     if (J.fin != nullptr && in < J.inner) {
-      float* fin = J.fin + mat + (size_t)in * J.s_in;
+      float* fin = J.fin + mat + (size_t)in * J.s_in + (size_t)o0 * J.s_out;
+      const bool sectors = rows_of_sectors(J.fin);
 #pragma unroll
-      for (int i = 0; i < N; i += 2) {
-        float x, y;
-        upk2(S[i / 2], x, y);
-        if (o0 + i < J.outer) fin[(size_t)(o0 + i) * J.s_out] = x;
-        if (o0 + i + 1 < J.outer) fin[(size_t)(o0 + i + 1) * J.s_out] = y;
+      for (int i = 0; i < N; i += 8) {
+        float x[8];
+#pragma unroll
+        for (int e = 0; e < 8; e += 2) upk2(S[(i + e) / 2], x[e], x[e + 1]);
+        if (sectors) {
+          if (o0 + i < J.outer) stg8(fin + i, x);
+        } else {
+#pragma unroll
+          for (int e = 0; e < 8; ++e)
+            if (o0 + i + e < J.outer) fin[(size_t)(i + e) * J.s_out] = x[e];
+        }
       }
     }
   }
