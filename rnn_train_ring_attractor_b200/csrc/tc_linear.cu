@@ -617,7 +617,14 @@ bool la_tc_operand_ok(const LaOperand& o, int B, int T, int H) {
 }
 
 int la_tc_launch(const LaLaunch& L, bool states_only, cudaStream_t s) {
-  // jobs of one shape together
+  // Jobs of one shape together.  Where all of them fit the GPU at once, the largest shape does for all: its products take longer,
+  // a second launch more (heads of 64 and 104, 90 CTAs: TODO).
+  const bool one_launch = L.B * L.H * L.segments * L.jobs <= 148;
+  int most_in = 64, most_out = 64;
+  for (int j = 0; j < L.jobs; ++j) {
+    if (L.job[j].inner > 64) most_in = 128;
+    if (L.job[j].outer > 64) most_out = 128;
+  }
   for (int shape = 0; shape < 4; ++shape) {
     const int di = shape & 1 ? 128 : 64, d_o = shape & 2 ? 128 : 64;
     LtParams P;
@@ -626,7 +633,7 @@ int la_tc_launch(const LaLaunch& L, bool states_only, cudaStream_t s) {
     P.L.jobs = 0;
     for (int j = 0; j < L.jobs; ++j) {
       const LaJob& J = L.job[j];
-      if ((J.inner <= 64 ? 64 : 128) != di || (J.outer <= 64 ? 64 : 128) != d_o) continue;
+      if ((one_launch ? most_in : J.inner <= 64 ? 64 : 128) != di || (one_launch ? most_out : J.outer <= 64 ? 64 : 128) != d_o) continue;
       const int to = P.L.jobs++;
       P.L.job[to] = J;
       const LaOperand* ops[3] = {&J.q, &J.k, &J.v};

@@ -11,7 +11,7 @@ from torch.autograd import Function
 from torch.autograd.function import once_differentiable
 
 from . import _lib
-from .linear_attention import DTYPES, last_contiguous, new, raw_stream, strided
+from .linear_attention import DTYPES, last_contiguous, new, raw_stream
 from .ring_rnn_cuda import on_device
 
 
@@ -54,7 +54,8 @@ def _call(q, k, frequencies, positions, first, interleaved, amplitude, inverse):
     else:
         where = positions.data_ptr(), positions.element_size(), *positions.stride()
     p = _lib.ROTARY.pack(B, T, Hq, 0 if k is None else k.shape[2], D, 2 * frequencies.shape[0], DTYPES[q.dtype], int(interleaved),
-                         int(inverse), amplitude, *strided(q), *((0, 0, 0, 0) if k is None else strided(k)), frequencies.data_ptr(),
+                         int(inverse), amplitude, q.data_ptr(), *q.stride()[:3],
+                         *((0, 0, 0, 0) if k is None else (k.data_ptr(), *k.stride()[:3])), frequencies.data_ptr(),
                          *where, first, q_out.data_ptr(), 0 if k is None else k_out.data_ptr())
     with on_device(dev):
         rc = _lib.lib().ringrnn_rotary(p, raw_stream(dev.index))
