@@ -353,7 +353,7 @@ LaOperand operand(const RingRnnStrided& t) { return LaOperand{t.data, t.batch, t
 // is copied to rows of a multiple of 8 elements first.
 struct PackJobs {
   LaOperand from[4];
-  __nv_bfloat16* to[4];
+  void* to[4];
   int width[4], padded[4];
 };
 __global__ void __launch_bounds__(256) la_pack_kernel(const __grid_constant__ PackJobs p, int B, int T, int H) {
@@ -369,7 +369,7 @@ __global__ void __launch_bounds__(256) la_pack_kernel(const __grid_constant__ Pa
     unsigned short y[8];
 #pragma unroll
     for (int e = 0; e < 8; ++e) y[e] = i0 + e < width ? x[e] : (unsigned short)0;
-    reinterpret_cast<uint4*>(p.to[j])[id] = make_uint4(y[0] | (uint32_t)y[1] << 16, y[2] | (uint32_t)y[3] << 16,
+    static_cast<uint4*>(p.to[j])[id] = make_uint4(y[0] | (uint32_t)y[1] << 16, y[2] | (uint32_t)y[3] << 16,
                                                        y[4] | (uint32_t)y[5] << 16, y[6] | (uint32_t)y[7] << 16);
   }
 }
@@ -406,7 +406,7 @@ Plan make_plan(const RingRnnLinearAttention& p, const RingRnnStrided* d_out) {
   Plan l;
   memset(&l, 0, sizeof(l));
   const bool backward = d_out != nullptr;
-  l.tensor_cores = p.dtype == RINGRNN_BF16 && p.dk <= LA_TC_WIDTH && p.dv <= LA_TC_WIDTH;
+  l.tensor_cores = p.dtype != RINGRNN_F32 && p.dk <= LA_TC_WIDTH && p.dv <= LA_TC_WIDTH;
   const int chunk = l.tensor_cores ? LA_TC_CHUNK : PC, n = cut(p, l.tensor_cores, backward);
   l.segment_tokens = (int)((((long long)p.T + n - 1) / n + chunk - 1) / chunk * chunk);
   l.segments = (int)(((long long)p.T + l.segment_tokens - 1) / l.segment_tokens);
@@ -433,7 +433,7 @@ int pack(const RingRnnLinearAttention& p, Plan* l, char* at, cudaStream_t s) {
     if (l->packed[x] == 0) continue;
     const int padded = (int)align_up(l->width[x], 8);
     jobs.from[n] = l->op[x];
-    jobs.to[n] = reinterpret_cast<__nv_bfloat16*>(at);
+    jobs.to[n] = at;
     jobs.width[n] = l->width[x];
     jobs.padded[n++] = padded;
     most = padded > most ? padded : most;
@@ -462,7 +462,7 @@ int check_workspace(const Plan& l, const void* workspace, size_t bytes) {
 }
 template <bool STATES>
 int launch(const RingRnnLinearAttention& p, const Plan& l, const LaLaunch& L, cudaStream_t s) {
-  return l.tensor_cores ? la_tc_launch(L, STATES, s) : plain_launch<STATES>(p.dtype, L, s);
+  return l.tensor_cores ? la_tc_launch(L, p.dtype, STATES, s) : plain_launch<STATES>(p.dtype, L, s);
 }
 
 }  // namespace

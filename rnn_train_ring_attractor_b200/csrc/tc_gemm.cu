@@ -66,7 +66,7 @@ bool make_tmap_bf16_4d(CUtensorMap* out, const void* base, const uint64_t dims[4
   for (int i = 0; i < 4; ++i) d[i] = dims[i], bx[i] = box[i];
   for (int i = 0; i < 3; ++i) st[i] = stride_bytes[i];
   return fn(out, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 4, const_cast<void*>(base), d, st, bx, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
-            CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_128B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+            CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
 namespace {

@@ -1,18 +1,20 @@
-// Linear attention with decay on tensor cores: bf16, widths up to 128 (padded to 64 or 128), chunks of 128 tokens.
+// Linear attention with decay on tensor cores: bf16 or fp16, widths up to 128 (padded to 64 or 128), chunks of 128 tokens.
 //
 // One CTA takes a (job, sequence, head, segment) and goes through its chunks with the state at hand; what a job is stands in
 // linear_attention.cuh.  A chunk of n tokens (t, s: tokens in it; weights as in the forward, "reverse" mirrors them):
 //
 //   scores [t x s]      = Q K^T            both from shared memory
-//   inter  [t x outer]  = Q bf16(S)        S copied to shared memory; its rows are then scaled by row_scale g^(t+1), in place
-//   out    [t x outer] += P V              P_ts = bf16(scale g^(t-s) scores_ts), s <= t, in tensor memory where the scores were
-//   delta  [in x outer] = K'^T V           K'_s = g^(n-1-s) k_s = hi + lo, two bf16 numbers, transposed into tensor memory
-//   S = g^n S + delta
+//   inter  [t x outer]  = Q b(S)           S copied to shared memory; its rows are then scaled by row_scale g^(t+1), in place
+//   out    [t x outer] += P V              P_ts = b(scale g^(t-s) scores_ts), s <= t, in tensor memory where the scores were
+//   delta  [in x outer] = K'^T V           K'_s = g^(n-1-s) k_s = hi + lo, two numbers, transposed into tensor memory
+//   S = g^n S + delta                      b(): rounded to the tensors' type
 //
-// Precision: the state is fp32 (registers) and what is added to it keeps sixteen bits, so that states passed from call to call
+// Precision (of bf16): the state is fp32 (registers) and what is added to it keeps sixteen bits, so that states passed from call to call
 // and their gradients are good for what fp32 is for: 2e-6 of their size, where keys rounded to bf16 would leave 2e-3.  Where it
 // only goes into bf16 outputs the state is rounded to bf16, like P: next to the outputs' own rounding that costs a factor of 1.4
 // in their error, a second product for the rest of the state would make it 1.1 and take 512 of a chunk's cycles.
+// fp16 has three bits more and little range: the state is multiplied by the power of two that brings its largest element just
+// below 2^15 before it is rounded, and inter divided by it again.  Scores have no such power: weighted ones from 65520 on are infinite.
 //
 // What bounds it: at widths of 128 the memory (a chunk is 128 KB, 5500 cycles of an SM's share at 6.5 TB/s); then shared memory's
 // 128 bytes per cycle, which products with both operands there use up.  P and K' therefore live in tensor memory, and V is all
@@ -25,6 +27,7 @@
 // cache (13 cycles for each instruction, with everything unrolled): loops stay rolled, pairs of fp32 are computed as such, and
 // what only a partial chunk needs is done apart.  The tensor pipe's order is inter, delta, out, the next scores: the chain of a
 // chunk is inter, delta, state, and the rest fills its gaps.
+#include <cuda_fp16.h>
 #include <string.h>
 
 #include "linear_attention.cuh"
@@ -54,7 +57,8 @@ struct LtCfg {
   static constexpr int TABLES = BARS + (2 * SLOTS + 12) * 8 + 32;  // 32 powers; key weights of 64 pairs of tokens
   static_assert(TABLES % 16 == 0, "alignment");
   static constexpr int FLAGS = TABLES + 128 + 512;
-  static constexpr int SMEM = FLAGS + 16;
+  static constexpr int RANGE = FLAGS + 16;  // fp16: the state's largest element by warp; what it was divided by, of two chunks
+  static constexpr int SMEM = RANGE + 48;
   static_assert(SMEM <= 232448, "shared memory of a block");
 };
 
@@ -80,14 +84,33 @@ __device__ __forceinline__ void tma_store_4d(const CUtensorMap* m, uint32_t src,
 __device__ __forceinline__ void sts128(uint32_t a, uint32_t x, uint32_t y, uint32_t z, uint32_t w) {
   asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(a), "r"(x), "r"(y), "r"(z), "r"(w) : "memory");
 }
+// what differs between the types: pairs of elements, and the bits of an instruction descriptor that name them
+template <class E>
+struct Pair;
+template <>
+struct Pair<__nv_bfloat16> {
+  typedef __nv_bfloat162 type;
+  static constexpr uint32_t IDESC = 0;
+  static __device__ __forceinline__ type from(float a, float b) { return __floats2bfloat162_rn(a, b); }
+  static __device__ __forceinline__ float kept(float x) { return __bfloat162float(__float2bfloat16_rn(x)); }
+};
+template <>
+struct Pair<__half> {
+  typedef __half2 type;
+  static constexpr uint32_t IDESC = (1u << 7) | (1u << 10);  // taken from the bf16 descriptor
+  static __device__ __forceinline__ type from(float a, float b) { return __floats2half2_rn(a, b); }
+  static __device__ __forceinline__ float kept(float x) { return __half2float(__float2half_rn(x)); }
+};
+template <class E>
 __device__ __forceinline__ uint32_t pack2(float lo, float hi) {
-  const __nv_bfloat162 v = __floats2bfloat162_rn(lo, hi);
+  const typename Pair<E>::type v = Pair<E>::from(lo, hi);
   return *reinterpret_cast<const uint32_t*>(&v);
 }
+template <class E>
 __device__ __forceinline__ uint32_t pack2(f32x2 v) {
   float a, b;
   upk2(v, a, b);
-  return pack2(a, b);
+  return pack2<E>(a, b);
 }
 // 32 bytes: a whole sector of each lane's own row
 __device__ __forceinline__ void ldg8(const float* p, float* x) {
@@ -105,9 +128,11 @@ __device__ __forceinline__ void regs_down() { asm volatile("setmaxnreg.dec.sync.
 template <int REGS>
 __device__ __forceinline__ void regs_up() { asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(REGS)); }
 
-template <int DI, int DO, bool STATES>
+template <class E, int DI, int DO, bool STATES>
 __global__ void __launch_bounds__(LT_THREADS, 1) la_tc_kernel(const __grid_constant__ LtParams A, volatile int* host_status) {
   using Cfg = LtCfg<DI, DO>;
+  typedef typename Pair<E>::type E2;
+  constexpr bool HALF = Pair<E>::IDESC != 0;
   constexpr int NS = Cfg::SLOTS, TILES = STATES ? 2 : 3;  // tiles of a chunk: (q,) k, v
   // (nothing else is in shared memory, so that this starts on a boundary of the swizzle's period; there is no room to move it)
   extern __shared__ __align__(1024) uint8_t mem[];
@@ -203,7 +228,7 @@ __global__ void __launch_bounds__(LT_THREADS, 1) la_tc_kernel(const __grid_const
   } else if (warp == 1) {
     // ---- MMAs, issued by the whole warp (see umma_ts_warp)
     const uint32_t lead = elect_one();
-    constexpr uint32_t ID_SCORES = make_idesc_bf16(128, 128, 0, 0), ID_OUT = make_idesc_bf16(128, DO, 0, 1);
+    constexpr uint32_t ID_SCORES = make_idesc_bf16(128, 128, 0, 0) - Pair<E>::IDESC, ID_OUT = make_idesc_bf16(128, DO, 0, 1) - Pair<E>::IDESC;
     auto slot = [&](int tile) { return base + (tile % NS) * Cfg::SLOT; };
     auto loaded = [&](int tile, int code) { mbar_wait(full(tile % NS), (tile / NS) & 1, w, code); };
     // K-major operands: 16 of the 64 columns of a 128-byte row at a time
@@ -327,16 +352,14 @@ __global__ void __launch_bounds__(LT_THREADS, 1) la_tc_kernel(const __grid_const
         named_bar_sync(1, 256);
         if (a < 64) {
           float x[2], rest[2];
-          __nv_bfloat16 y[2];
 #pragma unroll
           for (int e = 0; e < 2; ++e) {
             const int s = 2 * a + e;
             const int steps = STATES ? (rev ? t0 + s - begin + 1 : end - 1 - t0 - s) : rev ? s + 1 : n - 1 - s;
             x[e] = s < n ? J.key_scale * g.power(steps) : 0.f;
-            y[e] = __float2bfloat16_rn(x[e]);
-            rest[e] = x[e] - __bfloat162float(y[e]);
+            rest[e] = x[e] - Pair<E>::kept(x[e]);
           }
-          key_weights[a] = make_uint2(pack2(x[0], x[1]), pack2(rest[0], rest[1]));
+          key_weights[a] = make_uint2(pack2<E>(x[0], x[1]), pack2<E>(rest[0], rest[1]));
         }
         named_bar_sync(1, 256);
         have = n;
@@ -348,31 +371,31 @@ __global__ void __launch_bounds__(LT_THREADS, 1) la_tc_kernel(const __grid_const
         tcgen05_fence_after();
       }
       if (q * 32 < DI) {
-        // k w = hi + lo with w = w_hi + w_lo, all bf16: hi = k w_hi rounded, what that leaves is exact in bf16 (eight bits of the
-        // sixteen), lo = k w_lo + that, rounded.  Three instructions for two elements, where the way through fp32 takes eight.
+        // k w = hi + lo with w = w_hi + w_lo, all of the tensors' type: hi = k w_hi rounded, what that leaves is exact (half of the
+        // product's bits), lo = k w_lo + that, rounded.  Three instructions for two elements, where the way through fp32 takes eight.
         const int row = half * 64 + (lane >> 4) * 8 + (lane & 7), in = (q & 1) * 32 + ((lane >> 3) & 1) * 8;  // matrices: two of tokens by two of columns
         const uint32_t from = k + (q >> 1) * TILE, to = tm + (STATES ? sum_keys(c) : TM_KEYS) + ((uint32_t)(q * 32) << 16) + half * 32;
         const uint2* kw = key_weights + half * 32 + (lane & 3);
 #pragma unroll 1
-        for (int x = 0; x < 4; ++x) {  // 16 columns by 32 tokens
-          const int i = x >> 1, j = x & 1;
-          uint32_t hi[8], lo[8];
+        for (int j = 0; j < 2; ++j) {  // 32 tokens
+          uint2 wt[4];
 #pragma unroll
-          for (int m = 0; m < 2; ++m) {
-            uint32_t y[4];
-            ldmatrix_x4_trans(from + sw128_offset(row + j * 32 + m * 16, in + i * 16), y);
+          for (int e = 0; e < 4; ++e) wt[e] = kw[(j * 4 + e) * 4];
 #pragma unroll
-            for (int e = 0; e < 4; ++e) {
-              const uint2 wt = kw[(j * 4 + m * 2 + (e >> 1)) * 4];
-              const __nv_bfloat162 wh = *reinterpret_cast<const __nv_bfloat162*>(&wt.x), wl = *reinterpret_cast<const __nv_bfloat162*>(&wt.y),
-                                   z = *reinterpret_cast<const __nv_bfloat162*>(y + e), h2 = __hmul2_rn(z, wh),
-                                   l2 = __hfma2(z, wl, __hfma2(z, wh, __hneg2(h2)));
-              hi[m * 4 + e] = *reinterpret_cast<const uint32_t*>(&h2);
-              lo[m * 4 + e] = *reinterpret_cast<const uint32_t*>(&l2);
+          for (int i = 0; i < 2; ++i) {  // 16 columns
+            uint32_t hi[8], lo[8];
+            ldmatrix_x4_trans(from + sw128_offset(row + j * 32, in + i * 16), lo);
+            ldmatrix_x4_trans(from + sw128_offset(row + j * 32 + 16, in + i * 16), lo + 4);
+#pragma unroll
+            for (int e = 0; e < 8; ++e) {
+              const E2 wh = *reinterpret_cast<const E2*>(&wt[e >> 1].x), wl = *reinterpret_cast<const E2*>(&wt[e >> 1].y),
+                       z = *reinterpret_cast<const E2*>(lo + e), h2 = __hmul2_rn(z, wh), l2 = __hfma2(z, wl, __hfma2(z, wh, __hneg2(h2)));
+              hi[e] = *reinterpret_cast<const uint32_t*>(&h2);
+              lo[e] = *reinterpret_cast<const uint32_t*>(&l2);
             }
+            tmem_st_frag4(to + ((uint32_t)(i * 16) << 16) + j * 16, hi);
+            tmem_st_frag4(to + ((uint32_t)(i * 16) << 16) + 64 + j * 16, lo);
           }
-          tmem_st_frag4(to + ((uint32_t)(i * 16) << 16) + j * 16, hi);
-          tmem_st_frag4(to + ((uint32_t)(i * 16) << 16) + 64 + j * 16, lo);
         }
         tmem_st_wait();
         tcgen05_fence_before();
@@ -387,7 +410,7 @@ __global__ void __launch_bounds__(LT_THREADS, 1) la_tc_kernel(const __grid_const
         auto put = [&](int j) {
           uint32_t z[8];
 #pragma unroll
-          for (int e = 0; e < 8; ++e) z[e] = pack2(y[e]);
+          for (int e = 0; e < 8; ++e) z[e] = pack2<E>(y[e]);
           tmem_st8(mine + j * 32, z);
         };
         tmem_ld16(mine + q * 32, x);
@@ -428,16 +451,17 @@ __global__ void __launch_bounds__(LT_THREADS, 1) la_tc_kernel(const __grid_const
       constexpr int N = DO / 2;
       const int q = warp & 3, half = (warp - 12) >> 2, r = q * 32 + lane, a = tid - 384, o0 = half * N;
       const size_t ld = (size_t)L.H * J.outer;
-      __nv_bfloat16* const out = static_cast<__nv_bfloat16*>(J.out) + ((size_t)b * L.T * L.H + h) * J.outer;
+      unsigned short* const out = static_cast<unsigned short*>(J.out) + ((size_t)b * L.T * L.H + h) * J.outer;
       const uint32_t mine = tm + TM_OUT + ((uint32_t)(q * 32) << 16) + o0;
 #pragma unroll 1
       for (int c = 0; c < chunks; ++c) {
         const int t0 = chunk_at(c), n = min(C, end - t0);
         const int slot = ((TILES * c + 1) % NS) * Cfg::SLOT;
-        const float f = r < n ? J.row_scale * g.power(rev ? n - 1 - r : r + 1) : 0.f;
-        const f32x2 f2 = pk2(f, f);
+        float f = r < n ? J.row_scale * g.power(rev ? n - 1 - r : r + 1) : 0.f;
         mbar_wait(inter_done, c & 1, w, 130);
         tcgen05_fence_after();
+        if (HALF) f *= reinterpret_cast<const volatile float*>(mem + Cfg::RANGE)[8 + (c & 1)];
+        const f32x2 f2 = pk2(f, f);
 #pragma unroll 1
         for (int i = 0; i < N; i += 16) {
           uint32_t x[16];
@@ -469,7 +493,7 @@ __global__ void __launch_bounds__(LT_THREADS, 1) la_tc_kernel(const __grid_const
           }
           uint32_t y[8];
 #pragma unroll
-          for (int e = 0; e < 8; ++e) y[e] = r < n ? pack2(__uint_as_float(x[2 * e]), __uint_as_float(x[2 * e + 1])) : 0u;
+          for (int e = 0; e < 8; ++e) y[e] = r < n ? pack2<E>(__uint_as_float(x[2 * e]), __uint_as_float(x[2 * e + 1])) : 0u;
           sts128(to + sw128_offset(r, (o0 & 63) + i), y[0], y[1], y[2], y[3]);
           sts128(to + sw128_offset(r, (o0 & 63) + i + 8), y[4], y[5], y[6], y[7]);
         }
@@ -479,7 +503,7 @@ __global__ void __launch_bounds__(LT_THREADS, 1) la_tc_kernel(const __grid_const
 #pragma unroll 1
           for (int t = a >> 7; t < C && t0 + t < stop; t += 2)
             if (o < J.outer)
-              out[(size_t)(t0 + t) * ld + o] = *reinterpret_cast<const __nv_bfloat16*>(mem + slot + (o >> 6) * TILE + sw128_offset(t, o & 63));
+              out[(size_t)(t0 + t) * ld + o] = *reinterpret_cast<const unsigned short*>(mem + slot + (o >> 6) * TILE + sw128_offset(t, o & 63));
         }
         fence_proxy_async_smem();
         mbar_arrive(staged);
@@ -487,7 +511,7 @@ __global__ void __launch_bounds__(LT_THREADS, 1) la_tc_kernel(const __grid_const
       // tokens behind the sequence, beyond its last chunk
 #pragma unroll 1
       for (int t = begin + chunks * C + (a >> 7); t < stop; t += 2)
-        if ((a & 127) < J.outer) out[(size_t)t * ld + (a & 127)] = __float2bfloat16_rn(0.f);
+        if ((a & 127) < J.outer) out[(size_t)t * ld + (a & 127)] = 0;
     }
   } else if (warp >= 20) {
     // ---- the state: a thread has half a row
@@ -550,10 +574,33 @@ __global__ void __launch_bounds__(LT_THREADS, 1) la_tc_kernel(const __grid_const
           }
         }
         if (c < chunks) {  // the next operand (delta of this chunk is behind inter, which has read the last one)
-          if (in < DI) {
+          float down = 1.f;
+          if (HALF) {  // the largest element of all, and the power of two that brings it below 2^15 but not 2^14
+            volatile float* const range = reinterpret_cast<volatile float*>(mem + Cfg::RANGE);
+            float top = 0.f;
 #pragma unroll
-            for (int i = 0; i < N; i += 8)
-              sts128(to + sw128_offset(in, (o0 & 63) + i), pack2(S[i / 2]), pack2(S[i / 2 + 1]), pack2(S[i / 2 + 2]), pack2(S[i / 2 + 3]));
+            for (int i = 0; i < N / 2; ++i) {
+              float x, y;
+              upk2(S[i], x, y);
+              top = fmaxf(top, fmaxf(fabsf(x), fabsf(y)));
+            }
+            if (in >= DI) top = 0.f;
+#pragma unroll
+            for (int e = 16; e > 0; e >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, e));
+            named_bar_sync(3, 256);  // the last chunk's have been read
+            if (lane == 0) range[warp - 20] = top;
+            named_bar_sync(3, 256);
+#pragma unroll
+            for (int e = 0; e < 8; ++e) top = fmaxf(top, range[e]);
+            const int exponent = (int)(__float_as_uint(top) >> 23) - 127 - 14;
+            if (exponent > -100 && exponent < 100) down = __uint_as_float((uint32_t)(127 - exponent) << 23);
+            if (tid == 640) range[8 + (c & 1)] = 1.f / down;
+          }
+          if (in < DI) {
+            const f32x2 down2 = pk2(down, down);
+            auto two = [&](int i) { return pack2<E>(HALF ? mul2(S[i], down2) : S[i]); };
+#pragma unroll
+            for (int i = 0; i < N; i += 8) sts128(to + sw128_offset(in, (o0 & 63) + i), two(i / 2), two(i / 2 + 1), two(i / 2 + 2), two(i / 2 + 3));
           }
           fence_proxy_async_smem();
           tcgen05_fence_before();
@@ -594,17 +641,31 @@ bool make_map(CUtensorMap* m, const LaOperand& o, int width, int B, int T, int H
   return make_tmap_bf16_4d(m, o.p, dims, strides, box);
 }
 
-template <int DI, int DO, bool STATES>
+template <class E, int DI, int DO, bool STATES>
 int launch(const LtParams& P, cudaStream_t s) {
   using Cfg = LtCfg<DI, DO>;
   volatile int* host = nullptr;
   const int rc = host_status_word(&host);
   if (rc != RINGRNN_OK) return rc;
-  RINGRNN_CUDA_TRY(cudaFuncSetAttribute(la_tc_kernel<DI, DO, STATES>, cudaFuncAttributeMaxDynamicSharedMemorySize, Cfg::SMEM));
+  RINGRNN_CUDA_TRY(cudaFuncSetAttribute(la_tc_kernel<E, DI, DO, STATES>, cudaFuncAttributeMaxDynamicSharedMemorySize, Cfg::SMEM));
   LaunchScope ls(K_LAYER, s);
-  la_tc_kernel<DI, DO, STATES><<<P.L.B * P.L.H * P.L.segments * P.L.jobs, LT_THREADS, Cfg::SMEM, s>>>(P, host);
+  la_tc_kernel<E, DI, DO, STATES><<<P.L.B * P.L.H * P.L.segments * P.L.jobs, LT_THREADS, Cfg::SMEM, s>>>(P, host);
   RINGRNN_CUDA_TRY(cudaGetLastError());
   return RINGRNN_OK;
+}
+
+template <class E>
+int launch(int di, int d_o, bool states, const LtParams& P, cudaStream_t s) {
+  switch ((di == 128 ? 1 : 0) + (d_o == 128 ? 2 : 0) + (states ? 4 : 0)) {
+    case 0: return launch<E, 64, 64, false>(P, s);
+    case 1: return launch<E, 128, 64, false>(P, s);
+    case 2: return launch<E, 64, 128, false>(P, s);
+    case 3: return launch<E, 128, 128, false>(P, s);
+    case 4: return launch<E, 64, 64, true>(P, s);
+    case 5: return launch<E, 128, 64, true>(P, s);
+    case 6: return launch<E, 64, 128, true>(P, s);
+    default: return launch<E, 128, 128, true>(P, s);
+  }
 }
 
 }  // namespace
@@ -616,7 +677,7 @@ bool la_tc_operand_ok(const LaOperand& o, int B, int T, int H) {
   return t && h && b && (reinterpret_cast<uintptr_t>(o.p) & 15) == 0;
 }
 
-int la_tc_launch(const LaLaunch& L, bool states_only, cudaStream_t s) {
+int la_tc_launch(const LaLaunch& L, int dtype, bool states_only, cudaStream_t s) {
   // Jobs of one shape together.  Where all of them fit the GPU at once, the largest shape does for all: its products take longer,
   // a second launch more (heads of 64 and 104, 90 CTAs: TODO).
   const bool one_launch = L.B * L.H * L.segments * L.jobs <= 148;
@@ -646,17 +707,7 @@ int la_tc_launch(const LaLaunch& L, bool states_only, cudaStream_t s) {
       if (P.store[to] && !make_map(&P.map[to][3], out, J.outer, L.B, L.T, L.H, unused, unused + 1)) return RINGRNN_ERR_CUDA;
     }
     if (P.L.jobs == 0) continue;
-    int rc;
-    switch (shape * 2 + (states_only ? 1 : 0)) {
-      case 0: rc = launch<64, 64, false>(P, s); break;
-      case 1: rc = launch<64, 64, true>(P, s); break;
-      case 2: rc = launch<128, 64, false>(P, s); break;
-      case 3: rc = launch<128, 64, true>(P, s); break;
-      case 4: rc = launch<64, 128, false>(P, s); break;
-      case 5: rc = launch<64, 128, true>(P, s); break;
-      case 6: rc = launch<128, 128, false>(P, s); break;
-      default: rc = launch<128, 128, true>(P, s); break;
-    }
+    const int rc = dtype == RINGRNN_F16 ? launch<__half>(di, d_o, states_only, P, s) : launch<__nv_bfloat16>(di, d_o, states_only, P, s);
     if (rc != RINGRNN_OK) return rc;
   }
   return RINGRNN_OK;

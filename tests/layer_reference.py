@@ -74,15 +74,40 @@ def attend_bounds(dtype, T, widest, tensor_cores):
 
     fp32 arithmetic: a product of two factors and a decay, summed over a head's width and over T tokens by way of chunks: at
     most T + widest + 16 roundings in a row (the decay's powers count for sixteen).
-    Tensor cores, beside those sums in fp32: scores of pairs, or the state, rounded to bf16 (2^-8; an output is a sum of products
-    of the two kinds).  A key k with its weight w is hi + lo: w as two bf16 numbers is off by 2^-8 * 2^-8 of it; hi = k w_hi
-    rounded leaves at most 2^-8, which is exact; lo, of that size, is rounded once more: 2^-8 * 2^-8 again.  Together 2^-15, with
-    a part in 2^7 for the products of these parts."""
+    Tensor cores, beside those sums in fp32: scores of pairs, or the state, rounded to the type (u = 2^-8 for bf16, 2^-11 for fp16;
+    an output is a sum of products of the two kinds).  A key k with its weight w is hi + lo: w as two numbers is off by u * u of
+    it; hi = k w_hi rounded leaves at most u, which is exact; lo, of that size, is rounded once more: u * u again.  Together
+    2 u^2, with a factor of 1 + 2 u for the products of these parts."""
     sums = (T + widest + 16) * 2.0 ** -23
     if not tensor_cores:
         return sums, sums
-    keys = 2.0 ** -15 * (1 + 2.0 ** -7)
-    return 2.0 ** -8 * (1 + 2 * keys) + keys + sums, keys + sums
+    u = U[dtype]
+    keys = 2 * u * u * (1 + 2 * u)
+    return u * (1 + 2 * keys) + keys + sums, keys + sums
+
+
+def half_floor(q, k, v, scale, lengths=None, reverse=False):
+    """What the smallest numbers of fp16 add on tensor cores: [B,T,H,dv], to be added to a bound on outputs of (q, k, v).
+
+    A score is off by at most 2^-25 more (half a step), so an output by 2^-25 sum |v_s|.  A weighted key is off by 2^-25 for each
+    of hi, what hi leaves and lo, and by 2^-25 |k| for its weight: (3 + |k|) 2^-25, with 2^-23 (1 + |k|) on the safe side.  The
+    state's largest element is brought to 2^14 or more, so others are off by 2^-39 of it; 2^-38 of the sums' largest."""
+    q, k, v = (x.double().abs() for x in (q, k, v))
+    if lengths is not None:
+        live = (torch.arange(q.shape[1], device=q.device) < lengths[:, None])[:, :, None, None]
+        q, k, v = (torch.where(live, x, 0.0) for x in (q, k, v))
+    if reverse:
+        q, k, v = (x.flip(1) for x in (q, k, v))
+    none = torch.zeros(q.shape[2], device=q.device)
+    out, state = attend(q, 1 + k * max(1.0, scale), v, none, max(1.0, scale))
+    more = 2.0 ** -23 * out + 2.0 ** -25 * v.cumsum(1) + 2.0 ** -38 * max(1.0, scale) * q.sum(-1, keepdim=True) * state.amax()
+    return more.flip(1) if reverse else more
+
+
+def half_floor_state(k, v, scale=1.0):
+    """The same for states: [B,H,dk,dv]."""
+    k, v = (x.double().abs().transpose(1, 2) for x in (k, v))
+    return 2.0 ** -23 * ((1 + k * max(1.0, scale)).transpose(-1, -2) @ v)
 
 
 def philox(counter, key):

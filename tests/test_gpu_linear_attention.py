@@ -30,7 +30,23 @@ def _inputs(dtype, B, T, H, dk, dv, seed=0, state=True, lengths=None):
 
 
 def _on_tensor_cores(dtype, dk, dv):
-    return dtype is BF16 and dk <= 128 and dv <= 128
+    return dtype is not FP32 and dk <= 128 and dv <= 128
+
+
+def _masked(x, n):
+    return x if n is None else torch.where((torch.arange(x.shape[1], device="cuda") < n[:, None])[:, :, None, None], x, 0)
+
+
+def _floors(q, k, v, scale, n, d_out=None):
+    """fp16's smallest numbers: additions to the bounds of (out, state) or of (dq, dk, dv, dstate); zeros for other types."""
+    if q.dtype is not FP16 or not _on_tensor_cores(q.dtype, q.shape[-1], v.shape[-1]):
+        return (0.0,) * 4
+    q, k, v = (_masked(x, n) for x in (q, k, v))
+    if d_out is None:
+        return ref.half_floor(q, k, v, scale, n), ref.half_floor_state(k, v)
+    d_out = _masked(d_out, n)
+    return (ref.half_floor(d_out, v, k, scale, n), ref.half_floor(v, d_out, q, scale, n, True), ref.half_floor(k, q, d_out, scale, n, True),
+            ref.half_floor_state(q, d_out, scale) + ref.half_floor_state(d_out, q, scale).transpose(-1, -2))
 
 
 def _abs(*ts):
@@ -43,8 +59,10 @@ def _check_forward(got, q, k, v, l, scale, s, n):
     f_out, f_state = ref.attend_bounds(dtype, T, max(dk, dv), _on_tensor_cores(dtype, dk, dv))
     want, want_s = ref.attend(q, k, v, l, scale, s, n)
     top, top_s = ref.attend(*_abs(q, k, v), l, scale, *_abs(s), n)
-    e = ref.worst(got[0], want, f_out * top + ref.U[dtype] * (want.abs() + f_out * top) + ref.TINY[dtype])
-    es = ref.worst(got[1], want_s, f_state * top_s + ref.TINY[FP32])
+    more, more_s = _floors(q, k, v, scale, n)[:2]
+    room = f_out * top + more
+    e = ref.worst(got[0], want, room + ref.U[dtype] * (want.abs() + room) + ref.TINY[dtype])
+    es = ref.worst(got[1], want_s, f_state * top_s + more_s + ref.TINY[FP32])
     assert e <= 1.0 and es <= 1.0, (e, es)
     return e, es
 
@@ -56,10 +74,12 @@ def _check_grads(got, q, k, v, l, scale, s, n, d_out, d_final):
     want = ref.attend_grads(q, k, v, l, scale, s, n, d_out, d_final)
     top = ref.attend_grads(*_abs(q, k, v), l, scale, *_abs(s), n, *_abs(d_out, d_final))
     worst = []
-    for x, y, m in zip(got[:3], want, top):
-        worst.append(ref.worst(x, y, f_out * m + ref.U[dtype] * (y.abs() + f_out * m) + ref.TINY[dtype]))
+    more = _floors(q, k, v, scale, n, d_out)
+    for x, y, m, add in zip(got[:3], want, top, more):
+        room = f_out * m + add
+        worst.append(ref.worst(x, y, room + ref.U[dtype] * (y.abs() + room) + ref.TINY[dtype]))
     if s is not None:
-        worst.append(ref.worst(got[3], want[3], f_state * top[3] + ref.TINY[FP32]))
+        worst.append(ref.worst(got[3], want[3], f_state * top[3] + more[3] + ref.TINY[FP32]))
     assert max(worst) <= 1.0, worst
     return worst
 
@@ -76,7 +96,8 @@ CASES = [  # dtype, B, T, H, dk, dv
     (FP16, 2, 65, 2, 64, 64), (FP16, 1, 40, 3, 33, 100), (BF16, 1, 37, 2, 160, 192), (BF16, 1, 20, 1, 256, 3),
     (BF16, 1, 1, 1, 64, 64), (BF16, 2, 2, 3, 128, 128), (BF16, 2, 127, 2, 64, 128), (BF16, 1, 128, 3, 128, 64),
     (BF16, 2, 129, 2, 128, 128), (BF16, 3, 257, 2, 72, 104), (BF16, 1, 511, 1, 8, 16), (BF16, 2, 300, 2, 13, 99), (BF16, 1, 1000, 2, 64, 64),
-    (BF16, 1, 130, 2, 1, 1), (BF16, 1, 384, 2, 127, 65)]
+    (BF16, 1, 130, 2, 1, 1), (BF16, 1, 384, 2, 127, 65),
+    (FP16, 1, 1, 2, 128, 64), (FP16, 2, 129, 2, 128, 128), (FP16, 1, 300, 3, 64, 64), (FP16, 1, 257, 2, 17, 120), (FP16, 1, 200, 1, 150, 40)]
 
 
 @pytest.mark.parametrize("dtype,B,T,H,dk,dv", CASES)
@@ -90,7 +111,8 @@ def test_forward_and_gradients(dtype, B, T, H, dk, dv, state, achieved):
     achieved(f"linear attention {str(dtype)[6:]} {B}x{T}x{H} {dk}/{dv} (of the bound)", out=e, state=es, grads=max(w))
 
 
-@pytest.mark.parametrize("dtype,T,dk,dv", [(FP32, 90, 24, 40), (BF16, 300, 64, 128), (BF16, 300, 128, 72), (BF16, 70, 200, 20)])
+@pytest.mark.parametrize("dtype,T,dk,dv", [(FP32, 90, 24, 40), (BF16, 300, 64, 128), (BF16, 300, 128, 72), (BF16, 70, 200, 20),
+                                           (FP16, 300, 64, 128)])
 def test_padded_batches_ignore_what_stands_behind_a_sequence(dtype, T, dk, dv):
     lengths = [T, 0, 1, T - 1, 128 if T > 128 else 32, T // 2]
     q, k, v, l, s, n, d_out, d_final = _inputs(dtype, len(lengths), T, 2, dk, dv, seed=5, lengths=lengths)
@@ -114,7 +136,8 @@ def test_padded_batches_ignore_what_stands_behind_a_sequence(dtype, T, dk, dv):
 
 
 @pytest.mark.parametrize("dtype,B,T,H,dk,dv", [(FP32, 1, 2500, 1, 40, 24), (BF16, 1, 5003, 1, 128, 64), (BF16, 2, 4100, 1, 64, 128),
-                                               (BF16, 1, 2600, 3, 20, 33), (FP16, 1, 3000, 1, 200, 64)])
+                                               (BF16, 1, 2600, 3, 20, 33), (FP16, 1, 3000, 1, 200, 64),
+                                               (FP16, 1, 5003, 1, 64, 128)])
 def test_long_sequences_of_few_heads(dtype, B, T, H, dk, dv):
     """Cut into segments that run at once: the same bounds, ends inside and before segments, and one call like two."""
     for lengths in (None, [T - 1001] + [7] * (B - 1)):
@@ -152,7 +175,7 @@ def test_many_chunks_in_a_segment(T, H, dk, dv):
 
 
 @pytest.mark.parametrize("decay", [0.0, -1e-5, -0.3, -5.0, -60.0, -3e38, float("-inf")])
-@pytest.mark.parametrize("dtype", [FP32, BF16])
+@pytest.mark.parametrize("dtype", [FP32, BF16, FP16])
 def test_decays_from_none_to_all(dtype, decay):
     q, k, v, l, s, n, d_out, d_final = _inputs(dtype, 1, 200, 2, 64, 64, seed=9)
     l[:] = decay
@@ -201,6 +224,17 @@ def test_gradients_of_shared_heads_and_sequences(dtype):
         # each part has its own rounding, the sum of up to three one for every addition
         y, m = y.sum(dim, keepdim=True), m.sum(dim, keepdim=True)
         assert ref.worst(got, y, (f + u * (1 + f)) * m + 3 * u * (1 + f) * m) <= 1.0
+
+
+@pytest.mark.parametrize("size", [2.0 ** 9, 2.0 ** -9])
+def test_range_of_half_states(size):
+    """States far beyond fp16's range, or far below its step, read out as exactly as others."""
+    q, k, v, l, s, n, d_out, d_final = _inputs(FP16, 1, 300, 2, 64, 128, seed=31)
+    q = (q / size).to(FP16)
+    k, v, s = (k * min(1.0, size)).to(FP16), (v * size).to(FP16), s * size ** 2
+    out, final = linear_attention(q, k, v, l, scale=0.125, initial_state=s)
+    assert bool(torch.isfinite(out).all())
+    _check_forward((out, final), q, k, v, l, 0.125, s, n)
 
 
 def test_offsets_beyond_32_bits():
