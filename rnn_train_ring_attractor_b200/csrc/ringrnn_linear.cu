@@ -10,18 +10,23 @@ namespace {
 // ---- fp32 arithmetic: any type, any width up to 256 -----------------------------------------------------------------
 // One CTA per (job, sequence, head, segment) and slice of 64 outer columns, whose part of the state lives in shared memory
 // for the whole segment.  Chunks of 32 tokens: of 16, 32 and 64, 32 has the fewest products per token next to the state's own
-// 2 * inner * 64 (64 for the pairs' scores and 64 for their values) that still leave two CTAs per SM their shared memory.
-constexpr int PC = 32, PO = 64, P_THREADS = 256, P_LD = PC + 4;
+// 2 * inner * 64 (64 for the pairs' scores and 64 for their values) that still leave several CTAs per SM their shared memory.
+// Bound by the operands' way through shared memory: 10 words of 128 bytes for 32 products a thread where the state is read.  A
+// chunk's numbers are loaded into registers while the one before is at work (widths up to 128).
+constexpr int PC = 32, PO = 64, P_THREADS = 256, P_WARPS = P_THREADS / 32, P_LD = PC + 4;
 
 __host__ __device__ constexpr int plain_row(int inner) { return (inner + 3) / 4 * 4 + 4; }  // +4: rows a bank group apart
 size_t plain_smem(int inner) {
-  return sizeof(float) * (2 * PC * plain_row(inner) + PC * PO + PC * P_LD + 2 * PC + (size_t)(plain_row(inner) - 4) * PO);
+  return sizeof(float) * (2 * PC * plain_row(inner) + PC * PO + PC * P_LD + 3 * PC + 4 + (size_t)(plain_row(inner) - 4) * PO);
 }
 
-template <class E, bool STATES>
-__global__ void __launch_bounds__(P_THREADS) la_plain_kernel(const __grid_constant__ LaLaunch L) {
+// NC: inner columns a lane loads of each row, 32 apart
+template <class E, bool STATES, int NC>
+__global__ void __launch_bounds__(P_THREADS, NC <= 4 ? 2 : 1) la_plain_kernel(const __grid_constant__ LaLaunch L) {
   extern __shared__ float sm[];
-  const int tid = threadIdx.x;
+  constexpr bool AHEAD = NC <= 4;
+  constexpr int ROWS = PC / P_WARPS;  // a warp loads rows warp, warp + 8, ...
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const int ji = (int)(blockIdx.x % L.jobs);
   const LaJob& J = L.job[ji];
   const int at = (int)(blockIdx.x / L.jobs), seg = at % L.segments, bh = at / L.segments, h = bh % L.H, b = bh / L.H;
@@ -32,17 +37,20 @@ __global__ void __launch_bounds__(P_THREADS) la_plain_kernel(const __grid_consta
   float* K = Q + PC * ld;      // [PC][ld]
   float* V = K + PC * ld;      // [PC][PO]
   float* P = V + PC * PO;      // [PC][P_LD]
-  float* wk = P + PC * P_LD;   // [PC] factor of a key in the state
+  float* pw = P + PC * P_LD;   // [PC + 4] powers of the decay
+  float* wk = pw + PC + 4;     // [PC] factor of a key in the state
   float* wr = wk + PC;         // [PC] factor of the state in a row
   float* S = wr + PC;          // [IP][PO]
-  const LaDecay g(L.log_decay[h]);
   const int len = la_length(L, b);
   const int begin = seg * L.segment_tokens, stop = min(L.T, begin + L.segment_tokens), end = min(len, stop);
   const size_t mat = (size_t)at * J.inner * J.outer;
-
-  for (int e = tid; e < IP * PO; e += P_THREADS) {
-    const int i = e / PO, o = e % PO;
-    S[e] = (!STATES && J.init != nullptr && i < I && o < on) ? J.init[mat + (size_t)i * J.s_in + (size_t)(o0 + o) * J.s_out] : 0.f;
+  if (tid <= PC) pw[tid] = LaDecay(L.log_decay[h]).power(tid);
+  {
+    const bool given = !STATES && J.init != nullptr;
+    for (int e = tid; e < IP * PO; e += P_THREADS) {
+      const int i = e / PO, o = e % PO;
+      S[e] = given && i < I && o < on ? J.init[mat + (size_t)i * J.s_in + (size_t)(o0 + o) * J.s_out] : 0.f;
+    }
   }
   const E* q = static_cast<const E*>(J.q.p) + b * J.q.sb + h * J.q.sh;
   const E* k = static_cast<const E*>(J.k.p) + b * J.k.sb + h * J.k.sh;
@@ -50,26 +58,61 @@ __global__ void __launch_bounds__(P_THREADS) la_plain_kernel(const __grid_consta
   E* out = static_cast<E*>(J.out);
 
   const int chunks = end > begin ? (end - begin + PC - 1) / PC : 0;
+  auto chunk_at = [&](int c) { return begin + (J.reverse ? chunks - 1 - c : c) * PC; };
   const LaFactor whole(L.log_decay[h], PC);
+  float qr[AHEAD ? ROWS : 1][NC], kr[AHEAD ? ROWS : 1][NC], vr[AHEAD ? ROWS : 1][2];
+  // row j of this warp's: what is not there counts as zero
+  auto load_row = [&](int t0, int n, int j, float* x, float* y, float* z) {
+    const int r = warp + j * P_WARPS;
+    const bool row = r < n;
+#pragma unroll
+    for (int i = 0; i < NC; ++i) {
+      const bool in = row && lane + 32 * i < I;
+      if (!STATES) x[i] = in ? up(q[(t0 + r) * J.q.st + lane + 32 * i]) : 0.f;
+      y[i] = in ? up(k[(t0 + r) * J.k.st + lane + 32 * i]) : 0.f;
+    }
+#pragma unroll
+    for (int i = 0; i < 2; ++i) z[i] = row && lane + 32 * i < on ? up(v[(t0 + r) * J.v.st + lane + 32 * i]) : 0.f;
+  };
+  auto store_row = [&](int j, const float* x, const float* y, const float* z) {
+    const int r = warp + j * P_WARPS;
+#pragma unroll
+    for (int i = 0; i < NC; ++i)
+      if (lane + 32 * i < IP) {
+        if (!STATES) Q[r * ld + lane + 32 * i] = x[i];
+        K[r * ld + lane + 32 * i] = y[i];
+      }
+#pragma unroll
+    for (int i = 0; i < 2; ++i) V[r * PO + lane + 32 * i] = z[i];
+  };
+  auto load_chunk = [&](int c) {
+    const int t0 = chunk_at(c), n = min(PC, end - t0);
+#pragma unroll
+    for (int j = 0; j < ROWS; ++j) load_row(t0, n, j, qr[j], kr[j], vr[j]);
+  };
+  if (AHEAD && chunks > 0) load_chunk(0);
+  auto add = [](float4& a, float x, const float4& y) {
+    a.x = fmaf(x, y.x, a.x); a.y = fmaf(x, y.y, a.y); a.z = fmaf(x, y.z, a.z); a.w = fmaf(x, y.w, a.w);
+  };
   for (int c = 0; c < chunks; ++c) {
-    const int t0 = begin + (J.reverse ? chunks - 1 - c : c) * PC, n = min(PC, end - t0);
+    const int t0 = chunk_at(c), n = min(PC, end - t0);
     __syncthreads();
-    for (int e = tid; e < PC * IP; e += P_THREADS) {
-      const int r = e / IP, i = e - r * IP;
-      const bool in = r < n && i < I;
-      if (!STATES) Q[r * ld + i] = in ? up(q[(t0 + r) * J.q.st + i]) : 0.f;
-      K[r * ld + i] = in ? up(k[(t0 + r) * J.k.st + i]) : 0.f;
+    if (AHEAD) {
+#pragma unroll
+      for (int j = 0; j < ROWS; ++j) store_row(j, qr[j], kr[j], vr[j]);
+    } else {
+      for (int j = 0; j < ROWS; ++j) {
+        load_row(t0, n, j, qr[0], kr[0], vr[0]);
+        store_row(j, qr[0], kr[0], vr[0]);
+      }
     }
-    for (int e = tid; e < PC * PO; e += P_THREADS) {
-      const int r = e / PO, o = e % PO;
-      V[e] = (r < n && o < on) ? up(v[(t0 + r) * J.v.st + o]) : 0.f;
-    }
-    if (tid < PC) wk[tid] = tid < n ? J.key_scale * g.power(J.reverse ? tid + 1 : n - 1 - tid) : 0.f;
+    if (tid < PC) wk[tid] = tid < n ? J.key_scale * pw[J.reverse ? tid + 1 : n - 1 - tid] : 0.f;
     else if (tid < 2 * PC) {
       const int r = tid - PC;
-      wr[r] = r < n ? J.row_scale * g.power(J.reverse ? n - 1 - r : r + 1) : 0.f;
+      wr[r] = r < n ? J.row_scale * pw[J.reverse ? n - 1 - r : r + 1] : 0.f;
     }
     __syncthreads();
+    if (AHEAD && c + 1 < chunks) load_chunk(c + 1);
     if (!STATES) {
       // scores of a row with four keys, eight apart: consecutive threads read consecutive rows of K
       {
@@ -86,7 +129,7 @@ __global__ void __launch_bounds__(P_THREADS) la_plain_kernel(const __grid_consta
 #pragma unroll
         for (int m = 0; m < 4; ++m) {
           const int j = j0 + 8 * m, far = J.reverse ? j - i : i - j;
-          P[i * P_LD + j] = (far >= 0 && i < n && j < n) ? acc[m] * J.pair_scale * g.power(far) : 0.f;
+          P[i * P_LD + j] = far >= 0 && i < n && j < n ? acc[m] * (J.pair_scale * pw[far]) : 0.f;
         }
       }
       __syncthreads();
@@ -94,9 +137,6 @@ __global__ void __launch_bounds__(P_THREADS) la_plain_kernel(const __grid_consta
       {
         const int r = (tid >> 4) * 2, o = (tid & 15) * 4;
         float4 a0 = make_float4(0.f, 0.f, 0.f, 0.f), a1 = a0;
-        auto add = [](float4& a, float x, const float4& y) {
-          a.x = fmaf(x, y.x, a.x); a.y = fmaf(x, y.y, a.y); a.z = fmaf(x, y.z, a.z); a.w = fmaf(x, y.w, a.w);
-        };
         for (int d = 0; d < IP; d += 4) {
           const float4 x0 = *reinterpret_cast<const float4*>(Q + r * ld + d), x1 = *reinterpret_cast<const float4*>(Q + (r + 1) * ld + d);
           const float4* s4 = reinterpret_cast<const float4*>(S + d * PO + o);
@@ -116,11 +156,12 @@ __global__ void __launch_bounds__(P_THREADS) la_plain_kernel(const __grid_consta
         }
         const float w[2][4] = {{a0.x, a0.y, a0.z, a0.w}, {a1.x, a1.y, a1.z, a1.w}};
 #pragma unroll
-        for (int m = 0; m < 2; ++m)
+        for (int m = 0; m < 2; ++m) {
+          E* to = out + (((size_t)b * L.T + t0 + r + m) * L.H + h) * J.outer + o0 + o;
 #pragma unroll
           for (int e = 0; e < 4; ++e)
-            if (r + m < n && o + e < on)
-              out[(((size_t)b * L.T + t0 + r + m) * L.H + h) * J.outer + o0 + o + e] = down<E>(w[m][e]);
+            if (r + m < n && o + e < on) to[e] = down<E>(w[m][e]);
+        }
       }
       __syncthreads();
     }
@@ -140,12 +181,20 @@ __global__ void __launch_bounds__(P_THREADS) la_plain_kernel(const __grid_consta
           float4 y = *reinterpret_cast<const float4*>(V + r * PO + o);
           y.x *= w; y.y *= w; y.z *= w; y.w *= w;
           const float4 x = *reinterpret_cast<const float4*>(K + r * ld + d);
-          const float4 z = two ? *reinterpret_cast<const float4*>(K + r * ld + d + 64) : make_float4(0.f, 0.f, 0.f, 0.f);
-          const float xs[8] = {x.x, x.y, x.z, x.w, z.x, z.y, z.z, z.w};
+          const float xs[4] = {x.x, x.y, x.z, x.w};
 #pragma unroll
-          for (int m = 0; m < 8; ++m) {
+          for (int m = 0; m < 4; ++m) {
             acc[m][0] = fmaf(xs[m], y.x, acc[m][0]); acc[m][1] = fmaf(xs[m], y.y, acc[m][1]);
             acc[m][2] = fmaf(xs[m], y.z, acc[m][2]); acc[m][3] = fmaf(xs[m], y.w, acc[m][3]);
+          }
+          if (two) {
+            const float4 z = *reinterpret_cast<const float4*>(K + r * ld + d + 64);
+            const float zs[4] = {z.x, z.y, z.z, z.w};
+#pragma unroll
+            for (int m = 0; m < 4; ++m) {
+              acc[4 + m][0] = fmaf(zs[m], y.x, acc[4 + m][0]); acc[4 + m][1] = fmaf(zs[m], y.y, acc[4 + m][1]);
+              acc[4 + m][2] = fmaf(zs[m], y.z, acc[4 + m][2]); acc[4 + m][3] = fmaf(zs[m], y.w, acc[4 + m][3]);
+            }
           }
         }
 #pragma unroll
@@ -163,8 +212,8 @@ __global__ void __launch_bounds__(P_THREADS) la_plain_kernel(const __grid_consta
   __syncthreads();
   if (!STATES) {  // rows behind the sequence
     const int first = max(begin, end), rows = stop - first;
-    for (int e = tid; e < rows * on; e += P_THREADS)
-      out[(((size_t)b * L.T + first + e / on) * L.H + h) * J.outer + o0 + e % on] = down<E>(0.f);
+    for (int e = tid; e < rows * PO; e += P_THREADS)
+      if (e % PO < on) out[(((size_t)b * L.T + first + e / PO) * L.H + h) * J.outer + o0 + e % PO] = down<E>(0.f);
   }
   if (J.fin != nullptr)
     for (int e = tid; e < I * PO; e += P_THREADS) {
@@ -173,6 +222,15 @@ __global__ void __launch_bounds__(P_THREADS) la_plain_kernel(const __grid_consta
     }
 }
 
+template <class E, bool STATES, int NC>
+int plain_launch(const LaLaunch& L, int inner, int outer, cudaStream_t s) {
+  RINGRNN_CUDA_TRY(cudaFuncSetAttribute(la_plain_kernel<E, STATES, NC>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)plain_smem(32 * NC)));
+  const dim3 grid((unsigned)(L.B * L.H * L.segments * L.jobs), (unsigned)((outer + PO - 1) / PO));
+  LaunchScope ls(K_LAYER, s);
+  la_plain_kernel<E, STATES, NC><<<grid, P_THREADS, plain_smem(inner), s>>>(L);
+  RINGRNN_CUDA_TRY(cudaGetLastError());
+  return RINGRNN_OK;
+}
 template <class E, bool STATES>
 int plain_launch(const LaLaunch& L, cudaStream_t s) {
   int inner = 0, outer = 0;
@@ -180,13 +238,9 @@ int plain_launch(const LaLaunch& L, cudaStream_t s) {
     inner = L.job[j].inner > inner ? L.job[j].inner : inner;
     outer = L.job[j].outer > outer ? L.job[j].outer : outer;
   }
-  const size_t smem = plain_smem(inner);
-  RINGRNN_CUDA_TRY(cudaFuncSetAttribute(la_plain_kernel<E, STATES>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)plain_smem(256)));
-  const dim3 grid((unsigned)(L.B * L.H * L.segments * L.jobs), (unsigned)((outer + PO - 1) / PO));
-  LaunchScope ls(K_LAYER, s);
-  la_plain_kernel<E, STATES><<<grid, P_THREADS, smem, s>>>(L);
-  RINGRNN_CUDA_TRY(cudaGetLastError());
-  return RINGRNN_OK;
+  return inner <= 64    ? plain_launch<E, STATES, 2>(L, inner, outer, s)
+         : inner <= 128 ? plain_launch<E, STATES, 4>(L, inner, outer, s)
+                        : plain_launch<E, STATES, 8>(L, inner, outer, s);
 }
 template <bool STATES>
 int plain_launch(int dtype, const LaLaunch& L, cudaStream_t s) {
@@ -385,21 +439,24 @@ struct Plan {
   size_t bytes;        // whole workspace: one set of sums (backward: two), then the copies
 };
 
-// Segments.  Forming the sums reads keys and values once more, so a sequence is only cut where that brings more CTAs to work.
-int cut(const RingRnnLinearAttention& p, bool tensor_cores, int backward) {
-  const int chunk = tensor_cores ? LA_TC_CHUNK : PC;
-  const long long bh = (long long)p.B * p.H;
-  if (!tensor_cores) {
-    // two CTAs per SM; a segment of at least eight chunks, and at least twice the CTAs
-    const long long ctas = bh * (backward ? 3 : 1) * ((p.dv + PO - 1) / PO), most = (p.T + 8 * chunk - 1) / (8 * chunk);
-    const long long n = 296 / ctas < most ? 296 / ctas : most;
-    return n < 2 ? 1 : (int)n;
+// Segments of a sequence.  Forming their sums reads keys and values once more and is a launch of its own, with the scan behind it,
+// so a sequence is only cut where that brings more CTAs to work: the number of segments with the least time by the model
+//   rounds of CTAs x (start + chunks of a segment x chunk), for n > 1 the same again with part of a chunk's time, and the scan.
+// Measured (us): tensor cores start 6, chunk 2, sums 0.7 of it, scan 7; fp32 arithmetic start 5, chunk TODO, sums TODO, scan 7.
+int cut(const RingRnnLinearAttention& p, bool tensor_cores, bool backward) {
+  const int chunk = tensor_cores ? LA_TC_CHUNK : PC, at_once = tensor_cores ? 148 : 296, jobs = backward ? 3 : 1;
+  const long long slices = tensor_cores ? 1 : ((p.dk > p.dv && backward ? p.dk : p.dv) + PO - 1) / PO;
+  const long long ctas = (long long)p.B * p.H * jobs * slices, chunks = ((long long)p.T + chunk - 1) / chunk;
+  const double start = 6, each = tensor_cores ? 2 : 4, sums = tensor_cores ? 0.7 : 0.4, scan = backward ? 10 : 7;
+  auto rounds = [&](long long n) { return (double)((ctas * n + at_once - 1) / at_once); };
+  int best = 1;
+  double least = rounds(1) * (start + chunks * each);
+  for (long long n = 2; n <= chunks / 2 && ctas * (n - 1) < 2 * at_once; ++n) {
+    const long long per = (chunks + n - 1) / n;
+    const double t = rounds(n) * (start + per * each) + (backward ? 2.0 / 3.0 : 1.0) * rounds(n) * (start + per * each * sums) + scan;
+    if (t < 0.9 * least) least = t, best = (int)n;
   }
-  const int chunks = (p.T + chunk - 1) / chunk;
-  if (bh * (backward ? 3 : 1) > 148 || chunks < 4) return 1;
-  const long long n = 148 / (bh * (backward ? 3 : 1));
-  const int most = (chunks + 1) / 2;
-  return n < 2 ? 1 : n < most ? (int)n : most;
+  return best;
 }
 
 Plan make_plan(const RingRnnLinearAttention& p, const RingRnnStrided* d_out) {
