@@ -8,16 +8,41 @@ namespace ringrnn {
 namespace {
 
 // ---- fp32 arithmetic: any type, any width up to 256 -----------------------------------------------------------------
-// One CTA per (job, sequence, head, segment) and slice of 64 outer columns, whose part of the state lives in shared memory
-// for the whole segment.  Chunks of 32 tokens: of 16, 32 and 64, 32 has the fewest products per token next to the state's own
-// 2 * inner * 64 (64 for the pairs' scores and 64 for their values) that still leave several CTAs per SM their shared memory.
-// Bound by the operands' way through shared memory: 10 words of 128 bytes for 32 products a thread where the state is read.  A
-// chunk's numbers are loaded into registers while the one before is at work (widths up to 128).
-constexpr int PC = 32, PO = 64, P_THREADS = 256, P_WARPS = P_THREADS / 32, P_LD = PC + 4;
+// One CTA per (job, sequence, head, segment) and slice of 64 outer columns, chunks of 32 tokens (of 16, 32 and 64, 32 has the
+// fewest products per token next to the state's own 2 * inner * 64 that still leave several CTAs per SM their shared memory).
+//
+// Products on the tensor cores' tf32 type, exact to fp32's own rounding: x = hi + lo with hi rounded to tf32's eleven bits, and
+// what is left fits eleven bits again, so x y = hi hi + hi lo + lo hi but for lo lo, at most 2^-24 of it.  (Infinities become
+// NaN on the way.)  The same products on the CUDA cores were bound by the operands' way through shared memory, four cycles for
+// each 16 bytes a thread reads: TODO.  A fragment's element is read once per product of 16 x 8 x 8.
+// The state stays in registers as an accumulator and is copied to shared memory once a chunk, where the outputs read it.  A chunk's
+// numbers are loaded into registers while the one before is at work (widths up to 128).
+constexpr int PC = 32, PO = 64, P_THREADS = 256, P_WARPS = P_THREADS / 32;
+constexpr int P_LD = PC + 4, V_LD = PO + 8;  // rows 4 (8) banks apart: the lanes of a fragment then read 32 different ones
 
-__host__ __device__ constexpr int plain_row(int inner) { return (inner + 3) / 4 * 4 + 4; }  // +4: rows a bank group apart
+__host__ __device__ constexpr int plain_width(int inner) { return (inner + 15) / 16 * 16; }
 size_t plain_smem(int inner) {
-  return sizeof(float) * (2 * PC * plain_row(inner) + PC * PO + PC * P_LD + 3 * PC + 4 + (size_t)(plain_row(inner) - 4) * PO);
+  return sizeof(float) * (2 * PC * (plain_width(inner) + 4) + PC * V_LD + PC * P_LD + 3 * PC + 4 + (size_t)plain_width(inner) * V_LD);
+}
+
+struct Split {
+  uint32_t hi, lo;
+  __device__ __forceinline__ explicit Split(float x) {
+    hi = (__float_as_uint(x) + 0x1000u) & 0xffffe000u;
+    lo = __float_as_uint(x - __uint_as_float(hi));
+  }
+};
+// c += a b for a 16 x 8 by 8 x 8 product; lane 4 g + t holds of a: (g, t), (g + 8, t), (g, t + 4), (g + 8, t + 4); of b: (t, g),
+// (t + 4, g); of c: (g, 2 t), (g, 2 t + 1), (g + 8, 2 t), (g + 8, 2 t + 1)
+__device__ __forceinline__ void mma_tf32(float* c, uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
+  asm volatile("mma.sync.aligned.m16n8k8.row.col.f32.tf32.tf32.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
+               : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+               : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+__device__ __forceinline__ void mma_exact(float* c, const Split* a, const Split* b) {
+  mma_tf32(c, a[0].lo, a[1].lo, a[2].lo, a[3].lo, b[0].hi, b[1].hi);
+  mma_tf32(c, a[0].hi, a[1].hi, a[2].hi, a[3].hi, b[0].lo, b[1].lo);
+  mma_tf32(c, a[0].hi, a[1].hi, a[2].hi, a[3].hi, b[0].hi, b[1].hi);
 }
 
 // NC: inner columns a lane loads of each row, 32 apart
@@ -26,31 +51,41 @@ __global__ void __launch_bounds__(P_THREADS, NC <= 4 ? 2 : 1) la_plain_kernel(co
   extern __shared__ float sm[];
   constexpr bool AHEAD = NC <= 4;
   constexpr int ROWS = PC / P_WARPS;  // a warp loads rows warp, warp + 8, ...
-  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  constexpr int MT = NC / 2;          // a warp's tiles of the state: rows 16 ((warp & 3) + 4 i), columns 32 (warp >> 2) and on
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, t = lane & 3;
   const int ji = (int)(blockIdx.x % L.jobs);
   const LaJob& J = L.job[ji];
   const int at = (int)(blockIdx.x / L.jobs), seg = at % L.segments, bh = at / L.segments, h = bh % L.H, b = bh / L.H;
   const int o0 = blockIdx.y * PO;
   if (o0 >= J.outer) return;
-  const int I = J.inner, IP = plain_row(I) - 4, ld = IP + 4, on = min(PO, J.outer - o0);
+  const int I = J.inner, IP = plain_width(I), ld = IP + 4, on = min(PO, J.outer - o0);
   float* Q = sm;               // [PC][ld]
   float* K = Q + PC * ld;      // [PC][ld]
-  float* V = K + PC * ld;      // [PC][PO]
-  float* P = V + PC * PO;      // [PC][P_LD]
+  float* V = K + PC * ld;      // [PC][V_LD]
+  float* P = V + PC * V_LD;    // [PC][P_LD]
   float* pw = P + PC * P_LD;   // [PC + 4] powers of the decay
   float* wk = pw + PC + 4;     // [PC] factor of a key in the state
   float* wr = wk + PC;         // [PC] factor of the state in a row
-  float* S = wr + PC;          // [IP][PO]
+  float* S = wr + PC;          // [IP][V_LD]
   const int len = la_length(L, b);
   const int begin = seg * L.segment_tokens, stop = min(L.T, begin + L.segment_tokens), end = min(len, stop);
   const size_t mat = (size_t)at * J.inner * J.outer;
   if (tid <= PC) pw[tid] = LaDecay(L.log_decay[h]).power(tid);
+  const int col0 = (warp >> 2) * 32;
+  float state[MT][4][4];  // tile, 8 columns, element of the fragment
+  auto state_row = [&](int i, int e) { return 16 * ((warp & 3) + 4 * i) + g + (e >> 1) * 8; };
+  auto state_col = [&](int n, int e) { return col0 + 8 * n + 2 * t + (e & 1); };
   {
     const bool given = !STATES && J.init != nullptr;
-    for (int e = tid; e < IP * PO; e += P_THREADS) {
-      const int i = e / PO, o = e % PO;
-      S[e] = given && i < I && o < on ? J.init[mat + (size_t)i * J.s_in + (size_t)(o0 + o) * J.s_out] : 0.f;
-    }
+#pragma unroll
+    for (int i = 0; i < MT; ++i)
+#pragma unroll
+      for (int n = 0; n < 4; ++n)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const int r = state_row(i, e), o = state_col(n, e);
+          state[i][n][e] = given && r < I && o < on ? J.init[mat + (size_t)r * J.s_in + (size_t)(o0 + o) * J.s_out] : 0.f;
+        }
   }
   const E* q = static_cast<const E*>(J.q.p) + b * J.q.sb + h * J.q.sh;
   const E* k = static_cast<const E*>(J.k.p) + b * J.k.sb + h * J.k.sh;
@@ -83,17 +118,22 @@ __global__ void __launch_bounds__(P_THREADS, NC <= 4 ? 2 : 1) la_plain_kernel(co
         K[r * ld + lane + 32 * i] = y[i];
       }
 #pragma unroll
-    for (int i = 0; i < 2; ++i) V[r * PO + lane + 32 * i] = z[i];
+    for (int i = 0; i < 2; ++i) V[r * V_LD + lane + 32 * i] = z[i];
   };
   auto load_chunk = [&](int c) {
     const int t0 = chunk_at(c), n = min(PC, end - t0);
 #pragma unroll
     for (int j = 0; j < ROWS; ++j) load_row(t0, n, j, qr[j], kr[j], vr[j]);
   };
-  if (AHEAD && chunks > 0) load_chunk(0);
-  auto add = [](float4& a, float x, const float4& y) {
-    a.x = fmaf(x, y.x, a.x); a.y = fmaf(x, y.y, a.y); a.z = fmaf(x, y.z, a.z); a.w = fmaf(x, y.w, a.w);
+  // fragments: a's rows are rows of memory; b's k index is a column (by_column) or a row of memory
+  auto frag_a = [&](const float* m, int stride, int k0, Split* x) {
+    x[0] = Split(m[g * stride + k0 + t]);
+    x[1] = Split(m[(g + 8) * stride + k0 + t]);
+    x[2] = Split(m[g * stride + k0 + t + 4]);
+    x[3] = Split(m[(g + 8) * stride + k0 + t + 4]);
   };
+  if (AHEAD && chunks > 0) load_chunk(0);
+#pragma unroll 1
   for (int c = 0; c < chunks; ++c) {
     const int t0 = chunk_at(c), n = min(PC, end - t0);
     __syncthreads();
@@ -106,6 +146,16 @@ __global__ void __launch_bounds__(P_THREADS, NC <= 4 ? 2 : 1) la_plain_kernel(co
         store_row(j, qr[0], kr[0], vr[0]);
       }
     }
+    if (!STATES) {
+#pragma unroll
+      for (int i = 0; i < MT; ++i)
+        if (state_row(i, 0) - g < IP)
+#pragma unroll
+          for (int n8 = 0; n8 < 4; ++n8)
+#pragma unroll
+            for (int e = 0; e < 4; e += 2)
+              *reinterpret_cast<float2*>(S + state_row(i, e) * V_LD + state_col(n8, 0)) = make_float2(state[i][n8][e], state[i][n8][e + 1]);
+    }
     if (tid < PC) wk[tid] = tid < n ? J.key_scale * pw[J.reverse ? tid + 1 : n - 1 - tid] : 0.f;
     else if (tid < 2 * PC) {
       const int r = tid - PC;
@@ -114,112 +164,100 @@ __global__ void __launch_bounds__(P_THREADS, NC <= 4 ? 2 : 1) la_plain_kernel(co
     __syncthreads();
     if (AHEAD && c + 1 < chunks) load_chunk(c + 1);
     if (!STATES) {
-      // scores of a row with four keys, eight apart: consecutive threads read consecutive rows of K
-      {
-        const int i = tid >> 3, j0 = tid & 7;
+      const int row0 = (warp & 1) * 16;
+      {  // scores: 16 tokens by 8 keys
+        const int key0 = (warp >> 1) * 8;
         float acc[4] = {0.f, 0.f, 0.f, 0.f};
-        for (int d = 0; d < IP; d += 4) {
-          const float4 x = *reinterpret_cast<const float4*>(Q + i * ld + d);
+#pragma unroll 4
+        for (int k0 = 0; k0 < IP; k0 += 8) {
+          Split x[4] = {Split(0.f), Split(0.f), Split(0.f), Split(0.f)};
+          frag_a(Q + row0 * ld, ld, k0, x);
+          const Split y[2] = {Split(K[(key0 + g) * ld + k0 + t]), Split(K[(key0 + g) * ld + k0 + t + 4])};
+          mma_exact(acc, x, y);
+        }
 #pragma unroll
-          for (int m = 0; m < 4; ++m) {
-            const float4 y = *reinterpret_cast<const float4*>(K + (j0 + 8 * m) * ld + d);
-            acc[m] = fmaf(x.x, y.x, fmaf(x.y, y.y, fmaf(x.z, y.z, fmaf(x.w, y.w, acc[m]))));
+        for (int e = 0; e < 4; ++e) {
+          const int i = row0 + g + (e >> 1) * 8, j = key0 + 2 * t + (e & 1), far = J.reverse ? j - i : i - j;
+          acc[e] = far >= 0 && i < n && j < n ? acc[e] * (J.pair_scale * pw[far]) : 0.f;
+        }
+        *reinterpret_cast<float2*>(P + (row0 + g) * P_LD + key0 + 2 * t) = make_float2(acc[0], acc[1]);
+        *reinterpret_cast<float2*>(P + (row0 + g + 8) * P_LD + key0 + 2 * t) = make_float2(acc[2], acc[3]);
+      }
+      __syncthreads();
+      {  // outputs: 16 tokens by 16 columns; the state's part, then the pairs'
+        const int o = (warp >> 1) * 16;
+        float acc[2][4] = {{0.f, 0.f, 0.f, 0.f}, {0.f, 0.f, 0.f, 0.f}};
+        auto step = [&](const float* a, int a_ld, const float* m, int k0) {
+          Split x[4] = {Split(0.f), Split(0.f), Split(0.f), Split(0.f)};
+          frag_a(a + row0 * a_ld, a_ld, k0, x);
+#pragma unroll
+          for (int n8 = 0; n8 < 2; ++n8) {
+            const Split y[2] = {Split(m[(k0 + t) * V_LD + o + 8 * n8 + g]), Split(m[(k0 + t + 4) * V_LD + o + 8 * n8 + g])};
+            mma_exact(acc[n8], x, y);
           }
-        }
+        };
+#pragma unroll 2
+        for (int k0 = 0; k0 < IP; k0 += 8) step(Q, ld, S, k0);
+        const float w0 = wr[row0 + g], w1 = wr[row0 + g + 8];
 #pragma unroll
-        for (int m = 0; m < 4; ++m) {
-          const int j = j0 + 8 * m, far = J.reverse ? j - i : i - j;
-          P[i * P_LD + j] = far >= 0 && i < n && j < n ? acc[m] * (J.pair_scale * pw[far]) : 0.f;
-        }
+        for (int n8 = 0; n8 < 2; ++n8)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) acc[n8][e] *= e < 2 ? w0 : w1;
+#pragma unroll 2
+        for (int k0 = 0; k0 < PC; k0 += 8) step(P, P_LD, V, k0);
+#pragma unroll
+        for (int n8 = 0; n8 < 2; ++n8)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            const int r = row0 + g + (e >> 1) * 8, x = o + 8 * n8 + 2 * t + (e & 1);
+            if (r < n && x < on) out[(((size_t)b * L.T + t0 + r) * L.H + h) * J.outer + o0 + x] = down<E>(acc[n8][e]);
+          }
       }
-      __syncthreads();
-      // two rows by four columns: the state's part, then the pairs'
-      {
-        const int r = (tid >> 4) * 2, o = (tid & 15) * 4;
-        float4 a0 = make_float4(0.f, 0.f, 0.f, 0.f), a1 = a0;
-        for (int d = 0; d < IP; d += 4) {
-          const float4 x0 = *reinterpret_cast<const float4*>(Q + r * ld + d), x1 = *reinterpret_cast<const float4*>(Q + (r + 1) * ld + d);
-          const float4* s4 = reinterpret_cast<const float4*>(S + d * PO + o);
-          const float4 y0 = s4[0], y1 = s4[PO / 4], y2 = s4[PO / 2], y3 = s4[3 * PO / 4];
-          add(a0, x0.x, y0); add(a0, x0.y, y1); add(a0, x0.z, y2); add(a0, x0.w, y3);
-          add(a1, x1.x, y0); add(a1, x1.y, y1); add(a1, x1.z, y2); add(a1, x1.w, y3);
-        }
-        const float w0 = wr[r], w1 = wr[r + 1];
-        a0.x *= w0; a0.y *= w0; a0.z *= w0; a0.w *= w0;
-        a1.x *= w1; a1.y *= w1; a1.z *= w1; a1.w *= w1;
-        for (int j = 0; j < PC; j += 4) {
-          const float4 p0 = *reinterpret_cast<const float4*>(P + r * P_LD + j), p1 = *reinterpret_cast<const float4*>(P + (r + 1) * P_LD + j);
-          const float4* v4 = reinterpret_cast<const float4*>(V + j * PO + o);
-          const float4 y0 = v4[0], y1 = v4[PO / 4], y2 = v4[PO / 2], y3 = v4[3 * PO / 4];
-          add(a0, p0.x, y0); add(a0, p0.y, y1); add(a0, p0.z, y2); add(a0, p0.w, y3);
-          add(a1, p1.x, y0); add(a1, p1.y, y1); add(a1, p1.z, y2); add(a1, p1.w, y3);
-        }
-        const float w[2][4] = {{a0.x, a0.y, a0.z, a0.w}, {a1.x, a1.y, a1.z, a1.w}};
-#pragma unroll
-        for (int m = 0; m < 2; ++m) {
-          E* to = out + (((size_t)b * L.T + t0 + r + m) * L.H + h) * J.outer + o0 + o;
-#pragma unroll
-          for (int e = 0; e < 4; ++e)
-            if (r + m < n && o + e < on) to[e] = down<E>(w[m][e]);
-        }
-      }
-      __syncthreads();
     }
-    // the state: blocks of 4 x 4, two of them per thread at a time where the width has that many
-    {
+    {  // the state: its rows are the keys' columns
       const LaFactor gn = n == PC ? whole : LaFactor(L.log_decay[h], n);
-      const int o = (tid & 15) * 4, d0 = (tid >> 4) * 4;
-      for (int d = d0; d < IP; d += 128) {
-        const bool two = d + 64 < IP;
-        float acc[8][4];
 #pragma unroll
-        for (int m = 0; m < 8; ++m)
+      for (int i = 0; i < MT; ++i)
 #pragma unroll
-          for (int e = 0; e < 4; ++e) acc[m][e] = 0.f;
-        for (int r = 0; r < n; ++r) {
-          const float w = wk[r];
-          float4 y = *reinterpret_cast<const float4*>(V + r * PO + o);
-          y.x *= w; y.y *= w; y.z *= w; y.w *= w;
-          const float4 x = *reinterpret_cast<const float4*>(K + r * ld + d);
-          const float xs[4] = {x.x, x.y, x.z, x.w};
+        for (int n8 = 0; n8 < 4; ++n8)
 #pragma unroll
-          for (int m = 0; m < 4; ++m) {
-            acc[m][0] = fmaf(xs[m], y.x, acc[m][0]); acc[m][1] = fmaf(xs[m], y.y, acc[m][1]);
-            acc[m][2] = fmaf(xs[m], y.z, acc[m][2]); acc[m][3] = fmaf(xs[m], y.w, acc[m][3]);
-          }
-          if (two) {
-            const float4 z = *reinterpret_cast<const float4*>(K + r * ld + d + 64);
-            const float zs[4] = {z.x, z.y, z.z, z.w};
+          for (int e = 0; e < 4; ++e) state[i][n8][e] = gn.times(state[i][n8][e], 0.f);
+#pragma unroll 1
+      for (int k0 = 0; k0 < PC; k0 += 8) {
+        const float w0 = wk[k0 + t], w1 = wk[k0 + t + 4];
+        Split y[4][2] = {{Split(0.f), Split(0.f)}, {Split(0.f), Split(0.f)}, {Split(0.f), Split(0.f)}, {Split(0.f), Split(0.f)}};
 #pragma unroll
-            for (int m = 0; m < 4; ++m) {
-              acc[4 + m][0] = fmaf(zs[m], y.x, acc[4 + m][0]); acc[4 + m][1] = fmaf(zs[m], y.y, acc[4 + m][1]);
-              acc[4 + m][2] = fmaf(zs[m], y.z, acc[4 + m][2]); acc[4 + m][3] = fmaf(zs[m], y.w, acc[4 + m][3]);
-            }
-          }
+        for (int n8 = 0; n8 < 4; ++n8) {
+          y[n8][0] = Split(w0 * V[(k0 + t) * V_LD + col0 + 8 * n8 + g]);
+          y[n8][1] = Split(w1 * V[(k0 + t + 4) * V_LD + col0 + 8 * n8 + g]);
         }
 #pragma unroll
-        for (int m = 0; m < 8; ++m) {
-          if (m >= 4 && !two) break;
-          float4* s4 = reinterpret_cast<float4*>(S + (d + (m & 3) + (m >> 2) * 64) * PO + o);
-          float4 x = *s4;
-          x.x = gn.times(x.x, acc[m][0]); x.y = gn.times(x.y, acc[m][1]);
-          x.z = gn.times(x.z, acc[m][2]); x.w = gn.times(x.w, acc[m][3]);
-          *s4 = x;
+        for (int i = 0; i < MT; ++i) {
+          const int r = 16 * ((warp & 3) + 4 * i);
+          if (r >= IP) break;
+          const Split x[4] = {Split(K[(k0 + t) * ld + r + g]), Split(K[(k0 + t) * ld + r + g + 8]), Split(K[(k0 + t + 4) * ld + r + g]),
+                              Split(K[(k0 + t + 4) * ld + r + g + 8])};
+#pragma unroll
+          for (int n8 = 0; n8 < 4; ++n8) mma_exact(state[i][n8], x, y[n8]);
         }
       }
     }
   }
-  __syncthreads();
   if (!STATES) {  // rows behind the sequence
     const int first = max(begin, end), rows = stop - first;
     for (int e = tid; e < rows * PO; e += P_THREADS)
       if (e % PO < on) out[(((size_t)b * L.T + first + e / PO) * L.H + h) * J.outer + o0 + e % PO] = down<E>(0.f);
   }
   if (J.fin != nullptr)
-    for (int e = tid; e < I * PO; e += P_THREADS) {
-      const int i = e / PO, o = e % PO;
-      if (o < on) J.fin[mat + (size_t)i * J.s_in + (size_t)(o0 + o) * J.s_out] = S[e];
-    }
+#pragma unroll
+    for (int i = 0; i < MT; ++i)
+#pragma unroll
+      for (int n8 = 0; n8 < 4; ++n8)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const int r = state_row(i, e), o = state_col(n8, e);
+          if (r < I && o < on) J.fin[mat + (size_t)r * J.s_in + (size_t)(o0 + o) * J.s_out] = state[i][n8][e];
+        }
 }
 
 template <class E, bool STATES, int NC>

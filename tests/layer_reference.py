@@ -73,17 +73,25 @@ def attend_bounds(dtype, T, widest, tensor_cores):
     """(factor on the absolute sums for q-k-v-shaped outputs before their own rounding, the same for states).
 
     fp32 arithmetic: a product of two factors and a decay, summed over a head's width and over T tokens by way of chunks: at
-    most T + widest + 16 roundings in a row (the decay's powers count for sixteen).
+    most T + widest + 16 roundings in a row (the decay's powers count for sixteen).  The products leave out at most 2^-24 of
+    themselves (both factors' parts beyond eleven bits), three times on the way from an input to an output: 2^-22.
     Tensor cores, beside those sums in fp32: scores of pairs, or the state, rounded to the type (u = 2^-8 for bf16, 2^-11 for fp16;
     an output is a sum of products of the two kinds).  A key k with its weight w is hi + lo: w as two numbers is off by u * u of
     it; hi = k w_hi rounded leaves at most u, which is exact; lo, of that size, is rounded once more: u * u again.  Together
     2 u^2, with a factor of 1 + 2 u for the products of these parts."""
     sums = (T + widest + 16) * 2.0 ** -23
     if not tensor_cores:
-        return sums, sums
+        return sums + 2.0 ** -22, sums + 2.0 ** -22
     u = U[dtype]
     keys = 2 * u * u * (1 + 2 * u)
     return u * (1 + 2 * keys) + keys + sums, keys + sums
+
+
+def single_floor(T, widest, *inputs):
+    """What the smallest numbers of fp32 add: a factor's part below 2^-126 may count as zero in a product, so each of a sum's T or
+    widest products may be off by 2^-125 of the other factor, which is at most a product of two inputs and a sum over them."""
+    top = max(1.0, *(float(x.abs().nan_to_num(0.0, 0.0, 0.0).max()) for x in inputs if x is not None))
+    return 2.0 ** -125 * (T + widest) ** 2 * top ** 3
 
 
 def half_floor(q, k, v, scale, lengths=None, reverse=False):

@@ -38,8 +38,10 @@ def _masked(x, n):
 
 
 def _floors(q, k, v, scale, n, d_out=None):
-    """fp16's smallest numbers: additions to the bounds of (out, state) or of (dq, dk, dv, dstate); zeros for other types."""
-    if q.dtype is not FP16 or not _on_tensor_cores(q.dtype, q.shape[-1], v.shape[-1]):
+    """The types' smallest numbers: additions to the bounds of (out, state) or of (dq, dk, dv, dstate)."""
+    if not _on_tensor_cores(q.dtype, q.shape[-1], v.shape[-1]):
+        return (ref.single_floor(q.shape[1], max(q.shape[-1], v.shape[-1]), q, k, v, d_out),) * 4
+    if q.dtype is BF16:
         return (0.0,) * 4
     q, k, v = (_masked(x, n) for x in (q, k, v))
     if d_out is None:
@@ -292,7 +294,8 @@ def test_same_bits_twice_and_parts_of_gradients(dtype):
             want = ref.attend_grads(q, k, v, l, 0.1, s, n, torch.zeros_like(d_out), d_final)[i]
             top = ref.attend_grads(*_abs(q, k, v), l, 0.1, *_abs(s), n, torch.zeros_like(d_out), d_final.abs())[i]
             f = ref.attend_bounds(dtype, 700, 128, _on_tensor_cores(dtype, 64, 128))[0]
-            assert ref.worst(b, want, (f + ref.U[dtype] * (1 + f)) * top + ref.TINY[dtype]) <= 1.0
+            floor = ref.single_floor(700, 128, q, k, v, s, d_final)
+            assert ref.worst(b, want, (f + ref.U[dtype] * (1 + f)) * top + floor + ref.TINY[dtype]) <= 1.0
         xs[i].requires_grad_(False)
 
 
