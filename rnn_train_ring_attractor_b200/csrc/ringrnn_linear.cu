@@ -39,11 +39,18 @@ __device__ __forceinline__ void mma_tf32(float* c, uint32_t a0, uint32_t a1, uin
                : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
                : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
-__device__ __forceinline__ void mma_exact(float* c, const Split* a, const Split* b) {
-  mma_tf32(c, a[0].lo, a[1].lo, a[2].lo, a[3].lo, b[0].hi, b[1].hi);
-  mma_tf32(c, a[0].hi, a[1].hi, a[2].hi, a[3].hi, b[0].lo, b[1].lo);
-  mma_tf32(c, a[0].hi, a[1].hi, a[2].hi, a[3].hi, b[0].hi, b[1].hi);
-}
+// The tensor cores cut a sum off instead of rounding it, 2^-24 of it and always the same way, which over the thousands of sums
+// behind a state would show (2.6e-6 of an output, where the CUDA cores leave 2e-7).  So they add up 32 products at a time, the
+// small ones apart, and the CUDA cores the rest.
+struct Sums {
+  float big[4] = {0.f, 0.f, 0.f, 0.f}, small[4] = {0.f, 0.f, 0.f, 0.f};
+  __device__ __forceinline__ void add(const Split* a, const Split* b) {
+    mma_tf32(small, a[0].lo, a[1].lo, a[2].lo, a[3].lo, b[0].hi, b[1].hi);
+    mma_tf32(big, a[0].hi, a[1].hi, a[2].hi, a[3].hi, b[0].hi, b[1].hi);
+    mma_tf32(small, a[0].hi, a[1].hi, a[2].hi, a[3].hi, b[0].lo, b[1].lo);
+  }
+  __device__ __forceinline__ float value(int e) const { return big[e] + small[e]; }
+};
 
 // NC: inner columns a lane loads of each row, 32 apart
 template <class E, bool STATES, int NC>
@@ -168,12 +175,19 @@ __global__ void __launch_bounds__(P_THREADS, NC <= 4 ? 2 : 1) la_plain_kernel(co
       {  // scores: 16 tokens by 8 keys
         const int key0 = (warp >> 1) * 8;
         float acc[4] = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll 4
-        for (int k0 = 0; k0 < IP; k0 += 8) {
-          Split x[4] = {Split(0.f), Split(0.f), Split(0.f), Split(0.f)};
-          frag_a(Q + row0 * ld, ld, k0, x);
-          const Split y[2] = {Split(K[(key0 + g) * ld + k0 + t]), Split(K[(key0 + g) * ld + k0 + t + 4])};
-          mma_exact(acc, x, y);
+#pragma unroll 1
+        for (int k32 = 0; k32 < IP; k32 += 32) {
+          Sums sums;
+#pragma unroll
+          for (int k0 = k32; k0 < k32 + 32; k0 += 8) {
+            if (k0 >= IP) break;
+            Split x[4] = {Split(0.f), Split(0.f), Split(0.f), Split(0.f)};
+            frag_a(Q + row0 * ld, ld, k0, x);
+            const Split y[2] = {Split(K[(key0 + g) * ld + k0 + t]), Split(K[(key0 + g) * ld + k0 + t + 4])};
+            sums.add(x, y);
+          }
+#pragma unroll
+          for (int e = 0; e < 4; ++e) acc[e] += sums.value(e);
         }
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
@@ -187,24 +201,32 @@ __global__ void __launch_bounds__(P_THREADS, NC <= 4 ? 2 : 1) la_plain_kernel(co
       {  // outputs: 16 tokens by 16 columns; the state's part, then the pairs'
         const int o = (warp >> 1) * 16;
         float acc[2][4] = {{0.f, 0.f, 0.f, 0.f}, {0.f, 0.f, 0.f, 0.f}};
-        auto step = [&](const float* a, int a_ld, const float* m, int k0) {
-          Split x[4] = {Split(0.f), Split(0.f), Split(0.f), Split(0.f)};
-          frag_a(a + row0 * a_ld, a_ld, k0, x);
+        auto step = [&](const float* a, int a_ld, const float* m, int k32, int end_k) {
+          Sums sums[2];
 #pragma unroll
-          for (int n8 = 0; n8 < 2; ++n8) {
-            const Split y[2] = {Split(m[(k0 + t) * V_LD + o + 8 * n8 + g]), Split(m[(k0 + t + 4) * V_LD + o + 8 * n8 + g])};
-            mma_exact(acc[n8], x, y);
+          for (int k0 = k32; k0 < k32 + 32; k0 += 8) {
+            if (k0 >= end_k) break;
+            Split x[4] = {Split(0.f), Split(0.f), Split(0.f), Split(0.f)};
+            frag_a(a + row0 * a_ld, a_ld, k0, x);
+#pragma unroll
+            for (int n8 = 0; n8 < 2; ++n8) {
+              const Split y[2] = {Split(m[(k0 + t) * V_LD + o + 8 * n8 + g]), Split(m[(k0 + t + 4) * V_LD + o + 8 * n8 + g])};
+              sums[n8].add(x, y);
+            }
           }
+#pragma unroll
+          for (int n8 = 0; n8 < 2; ++n8)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) acc[n8][e] += sums[n8].value(e);
         };
-#pragma unroll 2
-        for (int k0 = 0; k0 < IP; k0 += 8) step(Q, ld, S, k0);
+#pragma unroll 1
+        for (int k32 = 0; k32 < IP; k32 += 32) step(Q, ld, S, k32, IP);
         const float w0 = wr[row0 + g], w1 = wr[row0 + g + 8];
 #pragma unroll
         for (int n8 = 0; n8 < 2; ++n8)
 #pragma unroll
           for (int e = 0; e < 4; ++e) acc[n8][e] *= e < 2 ? w0 : w1;
-#pragma unroll 2
-        for (int k0 = 0; k0 < PC; k0 += 8) step(P, P_LD, V, k0);
+        step(P, P_LD, V, 0, PC);
 #pragma unroll
         for (int n8 = 0; n8 < 2; ++n8)
 #pragma unroll
@@ -217,29 +239,25 @@ __global__ void __launch_bounds__(P_THREADS, NC <= 4 ? 2 : 1) la_plain_kernel(co
     {  // the state: its rows are the keys' columns
       const LaFactor gn = n == PC ? whole : LaFactor(L.log_decay[h], n);
 #pragma unroll
-      for (int i = 0; i < MT; ++i)
-#pragma unroll
-        for (int n8 = 0; n8 < 4; ++n8)
-#pragma unroll
-          for (int e = 0; e < 4; ++e) state[i][n8][e] = gn.times(state[i][n8][e], 0.f);
+      for (int i = 0; i < MT; ++i) {
+        const int r = 16 * ((warp & 3) + 4 * i);
+        if (r >= IP) break;
+        Sums sums[4];
 #pragma unroll 1
-      for (int k0 = 0; k0 < PC; k0 += 8) {
-        const float w0 = wk[k0 + t], w1 = wk[k0 + t + 4];
-        Split y[4][2] = {{Split(0.f), Split(0.f)}, {Split(0.f), Split(0.f)}, {Split(0.f), Split(0.f)}, {Split(0.f), Split(0.f)}};
-#pragma unroll
-        for (int n8 = 0; n8 < 4; ++n8) {
-          y[n8][0] = Split(w0 * V[(k0 + t) * V_LD + col0 + 8 * n8 + g]);
-          y[n8][1] = Split(w1 * V[(k0 + t + 4) * V_LD + col0 + 8 * n8 + g]);
-        }
-#pragma unroll
-        for (int i = 0; i < MT; ++i) {
-          const int r = 16 * ((warp & 3) + 4 * i);
-          if (r >= IP) break;
+        for (int k0 = 0; k0 < PC; k0 += 8) {
+          const float w0 = wk[k0 + t], w1 = wk[k0 + t + 4];
           const Split x[4] = {Split(K[(k0 + t) * ld + r + g]), Split(K[(k0 + t) * ld + r + g + 8]), Split(K[(k0 + t + 4) * ld + r + g]),
                               Split(K[(k0 + t + 4) * ld + r + g + 8])};
 #pragma unroll
-          for (int n8 = 0; n8 < 4; ++n8) mma_exact(state[i][n8], x, y[n8]);
+          for (int n8 = 0; n8 < 4; ++n8) {
+            const Split y[2] = {Split(w0 * V[(k0 + t) * V_LD + col0 + 8 * n8 + g]), Split(w1 * V[(k0 + t + 4) * V_LD + col0 + 8 * n8 + g])};
+            sums[n8].add(x, y);
+          }
         }
+#pragma unroll
+        for (int n8 = 0; n8 < 4; ++n8)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) state[i][n8][e] = gn.times(state[i][n8][e], sums[n8].value(e));
       }
     }
   }

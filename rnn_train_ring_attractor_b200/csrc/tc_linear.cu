@@ -164,6 +164,8 @@ __global__ void __launch_bounds__(LT_THREADS, 1) la_tc_kernel(const __grid_const
   auto sum_keys_ready = [&](int c) { return c & 1 ? pairs_ready : keys_ready; };  // forming sums: keys two chunks ahead at most
   auto sum_done = [&](int c) { return c & 1 ? out_ready : inter_done; };          // and what they were added to
   auto sum_keys = [&](int c) { return c & 1 ? TM_SCORES : TM_KEYS; };
+  auto sum_delta = [&](int c) { return c & 1 ? TM_OUT : TM_DELTA; };
+  auto sum_read = [&](int c) { return c & 1 ? scaled : state_ready; };  // a sum of two chunks before is in registers
   float* const powers = reinterpret_cast<float*>(mem + Cfg::TABLES);
   uint2* const key_weights = reinterpret_cast<uint2*>(powers + 32);  // of tokens 2i and 2i + 1: what bf16 keeps of them, the rest
 
@@ -257,18 +259,20 @@ __global__ void __launch_bounds__(LT_THREADS, 1) la_tc_kernel(const __grid_const
         } else {
           loaded(vt, 115);
           mbar_wait(sum_keys_ready(c), (c >> 1) & 1, w, 114);
+          if (c > 1) mbar_wait(sum_read(c), ((c >> 1) - 1) & 1, w, 112);
         }
         tcgen05_fence_after();
         const uint32_t keys = tm + (STATES ? sum_keys(c) : TM_KEYS), v = slot(vt);
 #pragma unroll 2
         for (int x = 0; x < C / 8; ++x)
-          umma_ts_warp(tm + TM_DELTA, keys + (x & 1) * 64 + (x >> 1) * 8, mn_major(v, x >> 1), ID_OUT, (STATES && c > 0) || x != 0, lead);
+          umma_ts_warp(tm + (STATES ? sum_delta(c) : TM_DELTA), keys + (x & 1) * 64 + (x >> 1) * 8, mn_major(v, x >> 1), ID_OUT, x != 0, lead);
         if (lead) {
-          if (STATES) umma_commit(sum_done(c));
-          if (!STATES || c == chunks - 1) umma_commit(delta_ready);
           if (STATES) {
+            umma_commit(sum_done(c));
             umma_commit(empty(kt % NS));
             umma_commit(empty(vt % NS));
+          } else {
+            umma_commit(delta_ready);
           }
         }
         __syncwarp();
@@ -542,17 +546,22 @@ __global__ void __launch_bounds__(LT_THREADS, 1) la_tc_kernel(const __grid_const
       }
     }
     if (STATES) {
-      if (chunks > 0) {
-        mbar_wait(delta_ready, 0, w, 140);
+      // (added up here and not by the tensor cores, which cut a sum off at 2^-24 of it, over hundreds of chunks)
+#pragma unroll 1
+      for (int c = 0; c < chunks; ++c) {
+        mbar_wait(sum_done(c), (c >> 1) & 1, w, 140);
         tcgen05_fence_after();
+        const uint32_t from = mine - TM_DELTA + sum_delta(c);
 #pragma unroll
         for (int i = 0; i < N; i += 16) {
           uint32_t x[16];
-          tmem_ld16(mine + i, x);
+          tmem_ld16(from + i, x);
           tmem_ld_wait();
 #pragma unroll
-          for (int e = 0; e < 8; ++e) S[i / 2 + e] = pk2u(x[2 * e], x[2 * e + 1]);
+          for (int e = 0; e < 8; ++e) S[i / 2 + e] = fma2(pk2(1.f, 1.f), S[i / 2 + e], pk2u(x[2 * e], x[2 * e + 1]));
         }
+        tcgen05_fence_before();
+        mbar_arrive(sum_read(c));
       }
     } else {
       const int part = (end - begin) % C;  // tokens of the one chunk that is not whole, 0: there is none
