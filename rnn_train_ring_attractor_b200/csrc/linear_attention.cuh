@@ -81,6 +81,6 @@ __device__ __forceinline__ int la_length(const LaLaunch& L, int b) {
 // Tensor-core path (tc_linear.cu): bf16 and fp16, widths up to 128.  Operands need 16-byte aligned bases and strides.
 bool la_tc_operand_ok(const LaOperand& o, int B, int T, int H);
 int la_tc_launch(const LaLaunch& L, int dtype, bool states_only, cudaStream_t s);
-constexpr int LA_TC_CHUNK = 128, LA_TC_WIDTH = 128;
+constexpr int LA_TC_CHUNK = 128, LA_TC_WIDTH = 128, LA_TC_BLOCKS = 148;  // blocks: what runs at once
 
 }  // namespace ringrnn

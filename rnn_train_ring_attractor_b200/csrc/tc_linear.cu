@@ -54,7 +54,7 @@ struct LtCfg {
   static constexpr int SLOTS = WIDE == 128 ? 6 : 12;  // two chunks' q, k and v or four's: what it takes to keep the memory busy
   // slots | the state as operand | barriers and tables.  A product reads 128 rows of K' whatever DI is; nobody uses what it makes of the others.
   static constexpr int STATE = SLOT * SLOTS, BARS = STATE + 2 * TILE;
-  static constexpr int TABLES = BARS + (2 * SLOTS + 12) * 8 + 32;  // 32 powers; key weights of 64 pairs of tokens
+  static constexpr int TABLES = BARS + (2 * SLOTS + 13) * 8 + 24;  // 32 powers; key weights of 64 pairs of tokens
   static_assert(TABLES % 16 == 0, "alignment");
   static constexpr int FLAGS = TABLES + 128 + 512;
   static constexpr int RANGE = FLAGS + 16;  // fp16: the state's largest element by warp; what it was divided by, of two chunks
@@ -128,12 +128,25 @@ __device__ __forceinline__ void regs_down() { asm volatile("setmaxnreg.dec.sync.
 template <int REGS>
 __device__ __forceinline__ void regs_up() { asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(REGS)); }
 
-template <class E, int DI, int DO, bool STATES>
-__global__ void __launch_bounds__(LT_THREADS, 1) la_tc_kernel(const __grid_constant__ LtParams A, volatile int* host_status) {
+// What a block does with its chunks: outputs of a job; the sums of a segment; or the outputs of two jobs that share a state.
+//
+// The last is for gradients: dV (rows K, keys Q, values dO) and dK (rows V, keys dO, values Q) need the same E, the one as
+// K E and the other as V E^T.  A chunk of theirs is loaded once instead of one and a half times, its keys are weighted and added
+// to the state once instead of twice, and what is left, two products of scores, of state and of values, goes through the same
+// places one after the other: step 2c is dV of chunk c, step 2c + 1 is dK.
+// Such a block takes 1.4 times as long as one job's.  Measured: gradients of 8 x 2048 x 16 heads of 128, 150 us -> 137; what is left
+// of a second round is a dQ block's 57 on most processors (128 pairs and 128 dQ on 148).
+enum Mode { OUTPUTS, SUMS, GRADIENT_PAIR };
+
+template <class E, int DI, int DO, int MODE>
+__device__ __forceinline__ void la_tc_block(const LtParams& A, const int ji, const int at, volatile int* host_status) {
   using Cfg = LtCfg<DI, DO>;
+  constexpr bool STATES = MODE == SUMS, PAIR = MODE == GRADIENT_PAIR;
+  constexpr int STEPS = PAIR ? 2 : 1;  // of a chunk
   typedef typename Pair<E>::type E2;
   constexpr bool HALF = Pair<E>::IDESC != 0;
-  constexpr int NS = Cfg::SLOTS, TILES = STATES ? 2 : 3;  // tiles of a chunk: (q,) k, v
+  // Tiles of a chunk: rows, keys, values, and for a pair the second rows; forming sums keys and values.
+  constexpr int NS = Cfg::SLOTS, TILES = STATES ? 2 : PAIR ? 4 : 3, KEYS = STATES ? 0 : 1, VALUES = KEYS + 1;
   // (nothing else is in shared memory, so that this starts on a boundary of the swizzle's period; there is no room to move it)
   extern __shared__ __align__(1024) uint8_t mem[];
   const uint32_t base = smem_u32(mem);
@@ -145,13 +158,14 @@ __global__ void __launch_bounds__(LT_THREADS, 1) la_tc_kernel(const __grid_const
 
   const LaLaunch& L = A.L;
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
-  const int ji = (int)(blockIdx.x % L.jobs);
-  const LaJob& J = L.job[ji];
-  const int at = (int)(blockIdx.x / L.jobs), seg = at % L.segments, bh = at / L.segments, h = bh % L.H, b = bh / L.H;
+  const LaJob& J = L.job[ji];  // a pair's second is the next one
+  const int seg = at % L.segments, bh = at / L.segments, h = bh % L.H, b = bh / L.H;
   const bool rev = J.reverse != 0;
   const int len = la_length(L, b), begin = seg * L.segment_tokens, stop = min(L.T, begin + L.segment_tokens), end = min(len, stop);
   const int chunks = end > begin ? (end - begin + C - 1) / C : 0;
   auto chunk_at = [&](int c) { return begin + (rev ? chunks - 1 - c : c) * C; };
+
+  auto out_tile = [&](int u) { return PAIR ? TILES * (u >> 1) + 3 * (u & 1) : TILES * u + KEYS; };  // whose place a step's outputs take
 
   const uint32_t bars = base + Cfg::BARS;
   auto full = [&](int i) { return bars + 8u * i; };
@@ -159,7 +173,7 @@ __global__ void __launch_bounds__(LT_THREADS, 1) la_tc_kernel(const __grid_const
   const uint32_t one = bars + 16u * NS;
   const uint32_t scores_ready = one, keys_ready = one + 8, pairs_ready = one + 16, inter_done = one + 24, delta_ready = one + 32,
                  state_ready = one + 40, out_ready = one + 48, out_free = one + 56, all_done = one + 64, tail_ready = one + 72,
-                 staged = one + 80, scaled = one + 88;
+                 staged = one + 80, scaled = one + 88, taken = one + 96;
   // A barrier's waiter can only tell one phase from the next.  Two barriers in turn where the other side can be a chunk ahead.
   auto sum_keys_ready = [&](int c) { return c & 1 ? pairs_ready : keys_ready; };  // forming sums: keys two chunks ahead at most
   auto sum_done = [&](int c) { return c & 1 ? out_ready : inter_done; };          // and what they were added to
@@ -188,6 +202,7 @@ __global__ void __launch_bounds__(LT_THREADS, 1) la_tc_kernel(const __grid_const
       mbar_init(tail_ready, 256);
       mbar_init(staged, 256);
       mbar_init(scaled, 256);
+      mbar_init(taken, 1);
       fence_mbar_init();
     }
   } else if (warp == 1) {
@@ -204,19 +219,18 @@ __global__ void __launch_bounds__(LT_THREADS, 1) la_tc_kernel(const __grid_const
 
   if (warp < 4) regs_down<REGS_ISSUE>();
   if (warp == 0) {
-    // ---- loads: q, k, v of each chunk through a ring of slots
+    // ---- loads: each chunk's tiles through a ring of slots
     if (lane == 0) {
-      const CUtensorMap* maps = A.map[ji];
       int i = 0, round = 0;
       for (int c = 0; c < chunks; ++c) {
         const int t0 = chunk_at(c);
 #pragma unroll
-        for (int x = 3 - TILES; x < 3; ++x) {
+        for (int x = 0; x < TILES; ++x) {
           if (!mbar_wait(empty(i), (round & 1) ^ 1, w, 101)) break;
-          const int blocks = (x == 2 ? DO : DI) / 64;
+          const int blocks = (x > KEYS ? DO : DI) / 64, from = x == 3 ? ji + 1 : ji, tensor = x == 3 ? 0 : STATES ? x + 1 : x;
           mbar_arrive_expect_tx(full(i), blocks * TILE);
           for (int k = 0; k < blocks; ++k)
-            tma_load_4d(base + i * Cfg::SLOT + k * TILE, maps + x, full(i), k * 64, t0, h * A.h_step[ji][x], b * A.b_step[ji][x]);
+            tma_load_4d(base + i * Cfg::SLOT + k * TILE, &A.map[from][tensor], full(i), k * 64, t0, h * A.h_step[from][tensor], b * A.b_step[from][tensor]);
           if (++i == NS) i = 0, ++round;
         }
         if (*static_cast<volatile int*>(flags)) break;
@@ -230,75 +244,90 @@ __global__ void __launch_bounds__(LT_THREADS, 1) la_tc_kernel(const __grid_const
   } else if (warp == 1) {
     // ---- MMAs, issued by the whole warp (see umma_ts_warp)
     const uint32_t lead = elect_one();
-    constexpr uint32_t ID_SCORES = make_idesc_bf16(128, 128, 0, 0) - Pair<E>::IDESC, ID_OUT = make_idesc_bf16(128, DO, 0, 1) - Pair<E>::IDESC;
+    // (M, N, whether A and B have their rows along K)
+    constexpr uint32_t ID_SCORES = make_idesc_bf16(128, 128, 0, 0) - Pair<E>::IDESC, ID_OUT = make_idesc_bf16(128, DO, 0, 1) - Pair<E>::IDESC,
+                       ID_OUT2 = make_idesc_bf16(128, DI, 0, 1) - Pair<E>::IDESC, ID_INTER2 = make_idesc_bf16(128, DI, 0, 0) - Pair<E>::IDESC;
     auto slot = [&](int tile) { return base + (tile % NS) * Cfg::SLOT; };
     auto loaded = [&](int tile, int code) { mbar_wait(full(tile % NS), (tile / NS) & 1, w, code); };
     // K-major operands: 16 of the 64 columns of a 128-byte row at a time
     auto k_major = [&](uint32_t tile, int ks) { return desc_sw128(desc_lo(tile + (ks >> 2) * TILE + (ks & 3) * 32, 0)); };
     // M/N-major ones: 16 rows, blocks of 64 columns a tile apart
     auto mn_major = [&](uint32_t tile, int ks) { return desc_sw128(desc_lo(tile + ks * 2048, TILE)); };
-    // inter(c - 1), delta(c - 1), out(c - 1), scores(c); loops are left rolled where their instructions keep up (see above)
+    // inter, (delta,) out of step u, scores of the next; loops are left rolled where their instructions keep up (see above)
 #pragma unroll 1
-    for (int i = STATES ? 1 : 0; i <= chunks; ++i) {
-      const int c = i - 1, kt = TILES * c + TILES - 2, vt = kt + 1;  // of the chunk before
+    for (int i = STATES ? 1 : 0; i <= chunks * STEPS; ++i) {
+      const int u = i - 1, c = PAIR ? u >> 1 : u, tile = TILES * c;
+      const bool second = PAIR && (u & 1);
       if (i > 0) {
         if (!STATES) {
-          mbar_wait(state_ready, c & 1, w, 112);
-          if (c > 0) mbar_wait(out_free, (c - 1) & 1, w, 113);
+          if (!second) mbar_wait(state_ready, c & 1, w, 112);
+          if (u > 0) mbar_wait(out_free, (u - 1) & 1, w, 113);
           tcgen05_fence_after();
+          if (!second) {
 #pragma unroll 2
-          for (int ks = 0; ks < DI / 16; ++ks)
-            umma_ss_warp(tm + TM_OUT, k_major(slot(kt - 1), ks), mn_major(base + Cfg::STATE, ks), ID_OUT, ks != 0, lead);
+            for (int ks = 0; ks < DI / 16; ++ks)
+              umma_ss_warp(tm + TM_OUT, k_major(slot(tile), ks), mn_major(base + Cfg::STATE, ks), ID_OUT, ks != 0, lead);
+          } else {
+#pragma unroll 2
+            for (int ks = 0; ks < DO / 16; ++ks)
+              umma_ss_warp(tm + TM_OUT, k_major(slot(tile + 3), ks), k_major(base + Cfg::STATE, ks), ID_INTER2, ks != 0, lead);
+          }
           if (lead) {
             umma_commit(inter_done);
-            umma_commit(empty((kt - 1) % NS));
+            if (!PAIR) umma_commit(empty(tile % NS));
           }
           __syncwarp();
-          loaded(vt, 115);
-          mbar_wait(keys_ready, c & 1, w, 114);
-        } else {
-          loaded(vt, 115);
-          mbar_wait(sum_keys_ready(c), (c >> 1) & 1, w, 114);
-          if (c > 1) mbar_wait(sum_read(c), ((c >> 1) - 1) & 1, w, 112);
         }
-        tcgen05_fence_after();
-        const uint32_t keys = tm + (STATES ? sum_keys(c) : TM_KEYS), v = slot(vt);
-#pragma unroll 2
-        for (int x = 0; x < C / 8; ++x)
-          umma_ts_warp(tm + (STATES ? sum_delta(c) : TM_DELTA), keys + (x & 1) * 64 + (x >> 1) * 8, mn_major(v, x >> 1), ID_OUT, x != 0, lead);
-        if (lead) {
+        loaded(tile + VALUES, 115);
+        const uint32_t v = slot(tile + VALUES);
+        if (!PAIR || second) {
           if (STATES) {
-            umma_commit(sum_done(c));
-            umma_commit(empty(kt % NS));
-            umma_commit(empty(vt % NS));
+            mbar_wait(sum_keys_ready(c), (c >> 1) & 1, w, 114);
+            if (c > 1) mbar_wait(sum_read(c), ((c >> 1) - 1) & 1, w, 112);
           } else {
-            umma_commit(delta_ready);
+            mbar_wait(keys_ready, c & 1, w, 114);
           }
-        }
-        __syncwarp();
-        if (!STATES) {
-          mbar_wait(scaled, c & 1, w, 116);
-          mbar_wait(pairs_ready, c & 1, w, 117);
           tcgen05_fence_after();
+          const uint32_t keys = tm + (STATES ? sum_keys(c) : TM_KEYS);
 #pragma unroll 2
-          for (int ks = 0; ks < C / 16; ++ks) umma_ts_warp(tm + TM_OUT, tm + TM_SCORES + 16 * ks, mn_major(v, ks), ID_OUT, true, lead);
+          for (int x = 0; x < C / 8; ++x)
+            umma_ts_warp(tm + (STATES ? sum_delta(c) : TM_DELTA), keys + (x & 1) * 64 + (x >> 1) * 8, mn_major(v, x >> 1), ID_OUT, x != 0, lead);
+          if (lead) {
+            umma_commit(STATES ? sum_done(c) : delta_ready);
+            if (STATES) umma_commit(empty((tile + KEYS) % NS));
+            if (STATES || PAIR) umma_commit(empty((tile + VALUES) % NS));
+          }
+          __syncwarp();
+        }
+        if (!STATES) {
+          mbar_wait(scaled, u & 1, w, 116);
+          mbar_wait(pairs_ready, u & 1, w, 117);
+          tcgen05_fence_after();
+          const uint32_t values = second ? slot(tile + KEYS) : v;
+#pragma unroll 2
+          for (int ks = 0; ks < C / 16; ++ks)
+            umma_ts_warp(tm + TM_OUT, tm + TM_SCORES + 16 * ks, mn_major(values, ks), second ? ID_OUT2 : ID_OUT, true, lead);
           if (lead) {
             umma_commit(out_ready);
-            umma_commit(empty(vt % NS));
+            if (!PAIR) umma_commit(empty((tile + VALUES) % NS));
+            if (second) umma_commit(empty((tile + KEYS) % NS));
           }
           __syncwarp();
         }
       }
-      if (!STATES && i < chunks) {
-        const uint32_t q = slot(TILES * i), k = slot(TILES * i + 1);
-        loaded(TILES * i, 110);
-        loaded(TILES * i + 1, 111);
-        if (chunk_at(i) + C > end) mbar_wait(tail_ready, 0, w, 119);
+      if (!STATES && i < chunks * STEPS) {
+        const int n = PAIR ? i >> 1 : i;
+        const bool two = PAIR && (i & 1);
+        const int rows = TILES * n + (two ? 3 : 0), keys = TILES * n + (two ? VALUES : KEYS);
+        loaded(rows, 110);
+        loaded(keys, 111);
+        if (chunk_at(n) + C > end) mbar_wait(tail_ready, 0, w, 119);
         // the scores go where out has just read P: no order holds between MMAs of different accumulators
-        if (i > 0) mbar_wait(out_ready, c & 1, w, 118);
+        if (i > 0) mbar_wait(out_ready, u & 1, w, 118);
         tcgen05_fence_after();
 #pragma unroll 2
-        for (int ks = 0; ks < DI / 16; ++ks) umma_ss_warp(tm + TM_SCORES, k_major(q, ks), k_major(k, ks), ID_SCORES, ks != 0, lead);
+        for (int ks = 0; ks < (two ? DO : DI) / 16; ++ks)
+          umma_ss_warp(tm + TM_SCORES, k_major(slot(rows), ks), k_major(slot(keys), ks), ID_SCORES, ks != 0, lead);
         if (lead) umma_commit(scores_ready);
         __syncwarp();
       }
@@ -307,13 +336,15 @@ __global__ void __launch_bounds__(LT_THREADS, 1) la_tc_kernel(const __grid_const
     if (lead) umma_commit(all_done);
     mbar_wait(all_done, 0, drain, 118);
   } else if (warp == 2) {
-    // ---- stores: outputs from the slot that held k, which is free after that
+    // ---- stores: outputs from the slot that held the keys (of a pair: the rows), which is free after that
     if (!STATES && lane == 0) {
-      for (int c = 0; c < chunks; ++c) {
-        const int slot = (TILES * c + 1) % NS;
-        if (!mbar_wait(staged, c & 1, w, 150)) break;
-        if (A.store[ji]) {
-          for (int k = 0; k < DO / 64; ++k) tma_store_4d(A.map[ji] + 3, base + slot * Cfg::SLOT + k * TILE, k * 64, chunk_at(c), h, b);
+      for (int u = 0; u < chunks * STEPS; ++u) {
+        const int c = PAIR ? u >> 1 : u, job = PAIR ? ji + (u & 1) : ji, slot = out_tile(u) % NS;
+        if (!mbar_wait(staged, u & 1, w, 150)) break;
+        mbar_arrive(taken);
+        if (A.store[job]) {
+          for (int k = 0; k < (PAIR && (u & 1) ? DI : DO) / 64; ++k)
+            tma_store_4d(&A.map[job][3], base + slot * Cfg::SLOT + k * TILE, k * 64, chunk_at(c), h, b);
           bulk_commit();
           bulk_wait_read<0>();
         }
@@ -338,7 +369,7 @@ __global__ void __launch_bounds__(LT_THREADS, 1) la_tc_kernel(const __grid_const
     int have = 0;
 #pragma unroll 1
     for (int c = 0; c < chunks; ++c) {
-      const int t0 = chunk_at(c), n = min(C, end - t0), kt = TILES * c + TILES - 2, vt = kt + 1;
+      const int t0 = chunk_at(c), n = min(C, end - t0), kt = TILES * c + KEYS, vt = TILES * c + VALUES;
       const uint32_t k = base + (kt % NS) * Cfg::SLOT;
       mbar_wait(full(kt % NS), (kt / NS) & 1, w, 120);
       if (n < C) {
@@ -405,8 +436,9 @@ __global__ void __launch_bounds__(LT_THREADS, 1) la_tc_kernel(const __grid_const
         tcgen05_fence_before();
       }
       mbar_arrive(STATES ? sum_keys_ready(c) : keys_ready);
-      if (!STATES) {
-        mbar_wait(scores_ready, c & 1, w, 122);
+#pragma unroll 1
+      for (int step = 0; step < (STATES ? 0 : STEPS); ++step) {
+        mbar_wait(scores_ready, (c * STEPS + step) & 1, w, 122);
         tcgen05_fence_after();
         const uint32_t mine = tm + TM_SCORES + ((uint32_t)(q * 32) << 16) + col;
         uint32_t x[16];
@@ -452,17 +484,15 @@ __global__ void __launch_bounds__(LT_THREADS, 1) la_tc_kernel(const __grid_const
     // ---- outputs: a thread has token r and half of its columns.  Inter is scaled; later the sum goes to shared memory
     regs_down<REGS_OUT>();
     if (!STATES) {
-      constexpr int N = DO / 2;
-      const int q = warp & 3, half = (warp - 12) >> 2, r = q * 32 + lane, a = tid - 384, o0 = half * N;
-      const size_t ld = (size_t)L.H * J.outer;
-      unsigned short* const out = static_cast<unsigned short*>(J.out) + ((size_t)b * L.T * L.H + h) * J.outer;
-      const uint32_t mine = tm + TM_OUT + ((uint32_t)(q * 32) << 16) + o0;
+      const int q = warp & 3, half = (warp - 12) >> 2, r = q * 32 + lane, a = tid - 384;
 #pragma unroll 1
-      for (int c = 0; c < chunks; ++c) {
+      for (int u = 0; u < chunks * STEPS; ++u) {
+        const int c = PAIR ? u >> 1 : u, job = PAIR ? ji + (u & 1) : ji, N = (PAIR && (u & 1) ? DI : DO) / 2, o0 = half * N;
+        const uint32_t mine = tm + TM_OUT + ((uint32_t)(q * 32) << 16) + o0;
         const int t0 = chunk_at(c), n = min(C, end - t0);
-        const int slot = ((TILES * c + 1) % NS) * Cfg::SLOT;
+        const int slot = (out_tile(u) % NS) * Cfg::SLOT;
         float f = r < n ? J.row_scale * g.power(rev ? n - 1 - r : r + 1) : 0.f;
-        mbar_wait(inter_done, c & 1, w, 130);
+        mbar_wait(inter_done, u & 1, w, 130);
         tcgen05_fence_after();
         if (HALF) f *= reinterpret_cast<const volatile float*>(mem + Cfg::RANGE)[8 + (c & 1)];
         const f32x2 f2 = pk2(f, f);
@@ -483,7 +513,7 @@ __global__ void __launch_bounds__(LT_THREADS, 1) la_tc_kernel(const __grid_const
         tmem_st_wait();
         tcgen05_fence_before();
         mbar_arrive(scaled);
-        mbar_wait(out_ready, c & 1, w, 131);
+        mbar_wait(out_ready, u & 1, w, 131);
         tcgen05_fence_after();
         const uint32_t to = base + slot + (o0 >> 6) * TILE;
 #pragma unroll 1
@@ -501,21 +531,28 @@ __global__ void __launch_bounds__(LT_THREADS, 1) la_tc_kernel(const __grid_const
           sts128(to + sw128_offset(r, (o0 & 63) + i), y[0], y[1], y[2], y[3]);
           sts128(to + sw128_offset(r, (o0 & 63) + i + 8), y[4], y[5], y[6], y[7]);
         }
-        if (!A.store[ji]) {  // widths and addresses that TMA does not take: element by element
+        if (!A.store[job]) {  // widths and addresses that TMA does not take: element by element
           named_bar_sync(2, 256);
-          const int o = a & 127;
+          const int outer = L.job[job].outer, o = a & 127;
+          unsigned short* const out = static_cast<unsigned short*>(L.job[job].out) + ((size_t)b * L.T * L.H + h) * outer + o;
 #pragma unroll 1
           for (int t = a >> 7; t < C && t0 + t < stop; t += 2)
-            if (o < J.outer)
-              out[(size_t)(t0 + t) * ld + o] = *reinterpret_cast<const unsigned short*>(mem + slot + (o >> 6) * TILE + sw128_offset(t, o & 63));
+            if (o < outer)
+              out[(size_t)(t0 + t) * L.H * outer] = *reinterpret_cast<const unsigned short*>(mem + slot + (o >> 6) * TILE + sw128_offset(t, o & 63));
         }
         fence_proxy_async_smem();
+        if (u > 0) mbar_wait(taken, (u - 1) & 1, w, 132);  // a store may wait for the memory longer than a chunk takes
         mbar_arrive(staged);
       }
       // tokens behind the sequence, beyond its last chunk
 #pragma unroll 1
-      for (int t = begin + chunks * C + (a >> 7); t < stop; t += 2)
-        if ((a & 127) < J.outer) out[(size_t)t * ld + (a & 127)] = 0;
+      for (int job = ji; job < ji + STEPS; ++job) {
+        const int outer = L.job[job].outer, o = a & 127;
+        unsigned short* const out = static_cast<unsigned short*>(L.job[job].out) + ((size_t)b * L.T * L.H + h) * outer + o;
+#pragma unroll 1
+        for (int t = begin + chunks * C + (a >> 7); t < stop; t += 2)
+          if (o < outer) out[(size_t)t * L.H * outer] = 0;
+      }
     }
   } else if (warp >= 20) {
     // ---- the state: a thread has half a row
@@ -640,6 +677,19 @@ __global__ void __launch_bounds__(LT_THREADS, 1) la_tc_kernel(const __grid_const
   if (warp == 1) tmem_dealloc(tm, TM_COLS);
 }
 
+template <class E, int DI, int DO, int MODE>
+__global__ void __launch_bounds__(LT_THREADS, 1) la_tc_kernel(const __grid_constant__ LtParams A, volatile int* host_status) {
+  la_tc_block<E, DI, DO, MODE>(A, (int)(blockIdx.x % A.L.jobs), (int)(blockIdx.x / A.L.jobs), host_status);
+}
+// Gradients: jobs dQ, dV, dK.  The longer blocks first, so that the others fill the last round: dV and dK of each sequence, head and
+// segment together, then dQ (inner and outer widths exchanged).
+template <class E, int DK, int DV>
+__global__ void __launch_bounds__(LT_THREADS, 1) la_tc_gradients_kernel(const __grid_constant__ LtParams A, volatile int* host_status) {
+  const int pairs = gridDim.x / 2;
+  if ((int)blockIdx.x < pairs) la_tc_block<E, DK, DV, GRADIENT_PAIR>(A, 1, (int)blockIdx.x, host_status);
+  else la_tc_block<E, DV, DK, OUTPUTS>(A, 0, (int)blockIdx.x - pairs, host_status);
+}
+
 bool make_map(CUtensorMap* m, const LaOperand& o, int width, int B, int T, int H, int* h_step, int* b_step) {
   *h_step = H > 1 && o.sh != 0;
   *b_step = B > 1 && o.sb != 0;
@@ -650,32 +700,48 @@ bool make_map(CUtensorMap* m, const LaOperand& o, int width, int B, int T, int H
   return make_tmap_bf16_4d(m, o.p, dims, strides, box);
 }
 
-template <class E, int DI, int DO, bool STATES>
-int launch(const LtParams& P, cudaStream_t s) {
-  using Cfg = LtCfg<DI, DO>;
+int launch(void (*kernel)(LtParams, volatile int*), int smem, int blocks, const LtParams& P, cudaStream_t s) {
   volatile int* host = nullptr;
   const int rc = host_status_word(&host);
   if (rc != RINGRNN_OK) return rc;
-  RINGRNN_CUDA_TRY(cudaFuncSetAttribute(la_tc_kernel<E, DI, DO, STATES>, cudaFuncAttributeMaxDynamicSharedMemorySize, Cfg::SMEM));
+  RINGRNN_CUDA_TRY(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
   LaunchScope ls(K_LAYER, s);
-  la_tc_kernel<E, DI, DO, STATES><<<P.L.B * P.L.H * P.L.segments * P.L.jobs, LT_THREADS, Cfg::SMEM, s>>>(P, host);
+  kernel<<<blocks, LT_THREADS, smem, s>>>(P, host);
   RINGRNN_CUDA_TRY(cudaGetLastError());
   return RINGRNN_OK;
 }
-
-template <class E>
-int launch(int di, int d_o, bool states, const LtParams& P, cudaStream_t s) {
-  switch ((di == 128 ? 1 : 0) + (d_o == 128 ? 2 : 0) + (states ? 4 : 0)) {
-    case 0: return launch<E, 64, 64, false>(P, s);
-    case 1: return launch<E, 128, 64, false>(P, s);
-    case 2: return launch<E, 64, 128, false>(P, s);
-    case 3: return launch<E, 128, 128, false>(P, s);
-    case 4: return launch<E, 64, 64, true>(P, s);
-    case 5: return launch<E, 128, 64, true>(P, s);
-    case 6: return launch<E, 64, 128, true>(P, s);
-    default: return launch<E, 128, 128, true>(P, s);
+// all jobs of one shape; gradients: DI x DO is the state's shape
+template <class E, int DI, int DO>
+int launch(int mode, const LtParams& P, cudaStream_t s) {
+  constexpr int smem = LtCfg<DI, DO>::SMEM;
+  const int each = P.L.B * P.L.H * P.L.segments;
+  switch (mode) {
+    case OUTPUTS: return launch(la_tc_kernel<E, DI, DO, OUTPUTS>, smem, each * P.L.jobs, P, s);
+    case SUMS: return launch(la_tc_kernel<E, DI, DO, SUMS>, smem, each * P.L.jobs, P, s);
+    default: return launch(la_tc_gradients_kernel<E, DI, DO>, smem, each * 2, P, s);
   }
 }
+template <class E>
+int launch(int di, int d_o, int mode, const LtParams& P, cudaStream_t s) {
+  return di == 64 ? (d_o == 64 ? launch<E, 64, 64>(mode, P, s) : launch<E, 64, 128>(mode, P, s))
+                  : (d_o == 64 ? launch<E, 128, 64>(mode, P, s) : launch<E, 128, 128>(mode, P, s));
+}
+int launch(int dtype, int di, int d_o, int mode, const LtParams& P, cudaStream_t s) {
+  return dtype == RINGRNN_F16 ? launch<__half>(di, d_o, mode, P, s) : launch<__nv_bfloat16>(di, d_o, mode, P, s);
+}
+bool add_job(LtParams* P, const LaJob& J, bool sums) {
+  const LaLaunch& L = P->L;
+  const int to = P->L.jobs++;
+  P->L.job[to] = J;
+  const LaOperand* ops[3] = {&J.q, &J.k, &J.v};
+  for (int x = sums ? 1 : 0; x < 3; ++x)
+    if (!make_map(&P->map[to][x], *ops[x], x == 2 ? J.outer : J.inner, L.B, L.T, L.H, &P->h_step[to][x], &P->b_step[to][x])) return false;
+  int unused[2];
+  const LaOperand out{J.out, (long long)L.T * L.H * J.outer, (long long)L.H * J.outer, J.outer};
+  P->store[to] = !sums && J.outer % 8 == 0 && (reinterpret_cast<uintptr_t>(J.out) & 15) == 0;
+  return !P->store[to] || make_map(&P->map[to][3], out, J.outer, L.B, L.T, L.H, unused, unused + 1);
+}
+int padded(int width) { return width <= 64 ? 64 : 128; }
 
 }  // namespace
 
@@ -686,37 +752,33 @@ bool la_tc_operand_ok(const LaOperand& o, int B, int T, int H) {
   return t && h && b && (reinterpret_cast<uintptr_t>(o.p) & 15) == 0;
 }
 
-int la_tc_launch(const LaLaunch& L, int dtype, bool states_only, cudaStream_t s) {
-  // Jobs of one shape together.  Where all of them fit the GPU at once, the largest shape does for all: its products take longer,
-  // a second launch more (heads of 64 and 104, 90 CTAs: TODO).
-  const bool one_launch = L.B * L.H * L.segments * L.jobs <= 148;
+int la_tc_launch(const LaLaunch& L, int dtype, bool sums, cudaStream_t s) {
+  LtParams P;
+  memset(&P, 0, sizeof(P));
+  P.L = L;
+  P.L.jobs = 0;
+  const bool at_once = L.B * L.H * L.segments * L.jobs <= LA_TC_BLOCKS;
+  if (!sums && L.jobs == 3 && !at_once) {
+    const int order[3] = {0, 2, 1};
+    for (int j : order)
+      if (!add_job(&P, L.job[j], false)) return RINGRNN_ERR_CUDA;
+    return launch(dtype, padded(L.job[2].inner), padded(L.job[2].outer), GRADIENT_PAIR, P, s);
+  }
+  // Jobs of one shape together.  Where all of them fit the GPU at once, the largest shape does for all: its products take longer, a
+  // second launch more (gradients of 5 x 777 x 6 heads of 64 and 104, 90 CTAs: 25 us instead of 44).  So do gradients job by job.
   int most_in = 64, most_out = 64;
   for (int j = 0; j < L.jobs; ++j) {
-    if (L.job[j].inner > 64) most_in = 128;
-    if (L.job[j].outer > 64) most_out = 128;
+    most_in = padded(L.job[j].inner) > most_in ? padded(L.job[j].inner) : most_in;
+    most_out = padded(L.job[j].outer) > most_out ? padded(L.job[j].outer) : most_out;
   }
   for (int shape = 0; shape < 4; ++shape) {
     const int di = shape & 1 ? 128 : 64, d_o = shape & 2 ? 128 : 64;
-    LtParams P;
-    memset(&P, 0, sizeof(P));
-    P.L = L;
     P.L.jobs = 0;
-    for (int j = 0; j < L.jobs; ++j) {
-      const LaJob& J = L.job[j];
-      if ((one_launch ? most_in : J.inner <= 64 ? 64 : 128) != di || (one_launch ? most_out : J.outer <= 64 ? 64 : 128) != d_o) continue;
-      const int to = P.L.jobs++;
-      P.L.job[to] = J;
-      const LaOperand* ops[3] = {&J.q, &J.k, &J.v};
-      for (int x = states_only ? 1 : 0; x < 3; ++x)
-        if (!make_map(&P.map[to][x], *ops[x], x == 2 ? J.outer : J.inner, L.B, L.T, L.H, &P.h_step[to][x], &P.b_step[to][x]))
-          return RINGRNN_ERR_CUDA;
-      int unused[2];
-      const LaOperand out{J.out, (long long)L.T * L.H * J.outer, (long long)L.H * J.outer, J.outer};
-      P.store[to] = !states_only && J.outer % 8 == 0 && (reinterpret_cast<uintptr_t>(J.out) & 15) == 0;
-      if (P.store[to] && !make_map(&P.map[to][3], out, J.outer, L.B, L.T, L.H, unused, unused + 1)) return RINGRNN_ERR_CUDA;
-    }
+    for (int j = 0; j < L.jobs; ++j)
+      if (di == (at_once ? most_in : padded(L.job[j].inner)) && d_o == (at_once ? most_out : padded(L.job[j].outer)))
+        if (!add_job(&P, L.job[j], sums)) return RINGRNN_ERR_CUDA;
     if (P.L.jobs == 0) continue;
-    const int rc = dtype == RINGRNN_F16 ? launch<__half>(di, d_o, states_only, P, s) : launch<__nv_bfloat16>(di, d_o, states_only, P, s);
+    const int rc = launch(dtype, di, d_o, sums ? SUMS : OUTPUTS, P, s);
     if (rc != RINGRNN_OK) return rc;
   }
   return RINGRNN_OK;

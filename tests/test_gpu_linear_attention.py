@@ -137,6 +137,23 @@ def test_padded_batches_ignore_what_stands_behind_a_sequence(dtype, T, dk, dv):
         assert torch.equal(a, b)
 
 
+@pytest.mark.parametrize("dtype,T,dk,dv", [(BF16, 300, 64, 64), (BF16, 385, 128, 72), (BF16, 140, 40, 128), (BF16, 1000, 128, 128),
+                                           (BF16, 257, 13, 99), (FP16, 300, 128, 128), (FP16, 513, 64, 128)])
+def test_more_sequences_than_processors(dtype, T, dk, dv):
+    """Where the gradients of keys and values of a sequence are one block's work; padding with NaN behind the sequences as well."""
+    lengths, H = [T, 0, 1, T - 1, 128, T // 2, T, T], 19
+    q, k, v, l, s, n, d_out, d_final = _inputs(dtype, len(lengths), T, H, dk, dv, seed=12, lengths=lengths)
+    clean, clean_grads = _run(q, k, v, l, 0.2, s, n, d_out, d_final)
+    _check_forward(clean, q, k, v, l, 0.2, s, n)
+    _check_grads(clean_grads, q, k, v, l, 0.2, s, n, d_out, d_final)
+    for x in (q, k, v, d_out):
+        for b, m in enumerate(lengths):
+            x[b, m:] = float("nan")
+    got, grads = _run(q, k, v, l, 0.2, s, n, d_out, d_final)
+    for a, b in zip((*got, *grads), (*clean, *clean_grads)):
+        assert torch.equal(a, b)
+
+
 @pytest.mark.parametrize("dtype,B,T,H,dk,dv", [(FP32, 1, 2500, 1, 40, 24), (BF16, 1, 5003, 1, 128, 64), (BF16, 2, 4100, 1, 64, 128),
                                                (BF16, 1, 2600, 3, 20, 33), (FP16, 1, 3000, 1, 200, 64),
                                                (FP16, 1, 5003, 1, 64, 128)])
