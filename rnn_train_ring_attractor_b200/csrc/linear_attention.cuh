@@ -33,6 +33,7 @@ struct LaJob {
   const float* init;  // nullptr: zero
   float* fin;         // nullptr: not wanted
   int s_in, s_out;
+  int precise;  // the state keeps 24 bits of what is added, for somebody sees it (tensor cores; sums always do)
 };
 
 constexpr int LA_MAX_JOBS = 3;

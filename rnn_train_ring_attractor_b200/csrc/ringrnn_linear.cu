@@ -639,6 +639,7 @@ extern "C" int ringrnn_linear_attention_fwd(const RingRnnLinearAttention* p, voi
   } else {
     j.init = p->initial_state;
     j.fin = final_state;
+    j.precise = 1;
   }
   return launch<false>(*p, l, L, s);
 }
@@ -689,6 +690,8 @@ extern "C" int ringrnn_linear_attention_bwd(const RingRnnLinearAttention* p, con
     jq.init = p->initial_state;
     jk.init = jv.init = d_final;
     jv.fin = d_initial;
+    // (not by d_initial alone: gradients have the same bits whichever of them are asked for)
+    jv.precise = p->initial_state != nullptr || d_initial != nullptr;
   }
   return launch<false>(*p, l, L, s);
 }

@@ -6,13 +6,15 @@
 //   scores [t x s]      = Q K^T            both from shared memory
 //   inter  [t x outer]  = Q b(S)           S copied to shared memory; its rows are then scaled by row_scale g^(t+1), in place
 //   out    [t x outer] += P V              P_ts = b(scale g^(t-s) scores_ts), s <= t, in tensor memory where the scores were
-//   delta  [in x outer] = K'^T V           K'_s = g^(n-1-s) k_s = hi + lo, two numbers, transposed into tensor memory
+//   delta  [in x outer] = K'^T V           K'_s = g^(n-1-s) k_s = hi + lo, two numbers, transposed into tensor memory (+ the rest)
 //   S = g^n S + delta                      b(): rounded to the tensors' type
 //
-// Precision (of bf16): the state is fp32 (registers) and what is added to it keeps sixteen bits, so that states passed from call to call
-// and their gradients are good for what fp32 is for: 2e-6 of their size, where keys rounded to bf16 would leave 2e-3.  Where it
-// only goes into bf16 outputs the state is rounded to bf16, like P: next to the outputs' own rounding that costs a factor of 1.4
-// in their error, a second product for the rest of the state would make it 1.1 and take 512 of a chunk's cycles.
+// Precision (of bf16): the state is fp32, in registers, and chunks are added to it there.  hi and lo keep sixteen bits of what is
+// added, which is plenty where a state only goes into bf16 outputs (it is rounded to bf16 for those, like P: next to the outputs' own
+// rounding that costs a factor of 1.4 in their error; a second product for the rest of the state would make it 1.1 and take 512
+// of a chunk's cycles).  A state that a caller sees, or that sums of segments make, is good for what fp32 is for: there a third part of
+// K' follows, so that all 24 bits of the product count.  Measured against 64 bits: 6e-7 of the state's size instead of 3.8e-6,
+// for 65 us instead of 58 (forward of 8 x 2048 x 16 heads of 128; nothing at widths of 64 or where segments are summed).
 // fp16 has three bits more and little range: the state is multiplied by the power of two that brings its largest element just
 // below 2^15 before it is rounded, and inter divided by it again.  Scores have no such power: weighted ones from 65520 on are infinite.
 //
@@ -46,6 +48,8 @@ constexpr int REGS_ISSUE = 32, REGS_WEIGHT = 72, REGS_OUT = 64, REGS_STATE = 96;
 static_assert((4 * REGS_ISSUE + 8 * REGS_WEIGHT + 8 * REGS_OUT + 8 * REGS_STATE) * 32 <= 65536 / LT_THREADS / 8 * 8 * LT_THREADS, "registers");
 // tensor memory: scores, of each 16 columns the first 8 then P; inter and outputs; delta; K' (hi, lo)
 constexpr uint32_t TM_SCORES = 0, TM_OUT = 128, TM_DELTA = 256, TM_KEYS = 384, TM_COLS = 512;
+// forming sums: K' (hi, lo, rest) in turn at two places, and delta
+constexpr uint32_t TM_SUM_KEYS = 192, TM_SUM_DELTA = 384;
 
 template <int DI, int DO>
 struct LtCfg {
@@ -54,9 +58,9 @@ struct LtCfg {
   static constexpr int SLOTS = WIDE == 128 ? 6 : 12;  // two chunks' q, k and v or four's: what it takes to keep the memory busy
   // slots | the state as operand | barriers and tables.  A product reads 128 rows of K' whatever DI is; nobody uses what it makes of the others.
   static constexpr int STATE = SLOT * SLOTS, BARS = STATE + 2 * TILE;
-  static constexpr int TABLES = BARS + (2 * SLOTS + 13) * 8 + 24;  // 32 powers; key weights of 64 pairs of tokens
+  static constexpr int TABLES = BARS + (2 * SLOTS + 15) * 8 + 8;  // 32 powers; key weights of 64 pairs of tokens, twice
   static_assert(TABLES % 16 == 0, "alignment");
-  static constexpr int FLAGS = TABLES + 128 + 512;
+  static constexpr int FLAGS = TABLES + 128 + 512 + 512;
   static constexpr int RANGE = FLAGS + 16;  // fp16: the state's largest element by warp; what it was divided by, of two chunks
   static constexpr int SMEM = RANGE + 48;
   static_assert(SMEM <= 232448, "shared memory of a block");
@@ -84,6 +88,9 @@ __device__ __forceinline__ void tma_store_4d(const CUtensorMap* m, uint32_t src,
 __device__ __forceinline__ void sts128(uint32_t a, uint32_t x, uint32_t y, uint32_t z, uint32_t w) {
   asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(a), "r"(x), "r"(y), "r"(z), "r"(w) : "memory");
 }
+__device__ __forceinline__ void lds128(uint32_t a, uint32_t* x) {
+  asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];" : "=r"(x[0]), "=r"(x[1]), "=r"(x[2]), "=r"(x[3]) : "r"(a) : "memory");
+}
 // what differs between the types: pairs of elements, and the bits of an instruction descriptor that name them
 template <class E>
 struct Pair;
@@ -101,11 +108,14 @@ struct Pair<__half> {
   static __device__ __forceinline__ type from(float a, float b) { return __floats2half2_rn(a, b); }
   static __device__ __forceinline__ float kept(float x) { return __half2float(__float2half_rn(x)); }
 };
+template <class E2>
+__device__ __forceinline__ uint32_t bits(E2 v) { return *reinterpret_cast<const uint32_t*>(&v); }
 template <class E>
 __device__ __forceinline__ uint32_t pack2(float lo, float hi) {
-  const typename Pair<E>::type v = Pair<E>::from(lo, hi);
-  return *reinterpret_cast<const uint32_t*>(&v);
+  return bits(Pair<E>::from(lo, hi));
 }
+// two bf16 as fp32
+__device__ __forceinline__ f32x2 wide(uint32_t pair) { return pk2u(pair << 16, pair & 0xffff0000u); }
 template <class E>
 __device__ __forceinline__ uint32_t pack2(f32x2 v) {
   float a, b;
@@ -146,7 +156,7 @@ __device__ __forceinline__ void la_tc_block(const LtParams& A, const int ji, con
   typedef typename Pair<E>::type E2;
   constexpr bool HALF = Pair<E>::IDESC != 0;
   // Tiles of a chunk: rows, keys, values, and for a pair the second rows; forming sums keys and values.
-  constexpr int NS = Cfg::SLOTS, TILES = STATES ? 2 : PAIR ? 4 : 3, KEYS = STATES ? 0 : 1, VALUES = KEYS + 1;
+  constexpr int NS = Cfg::SLOTS, TILES = STATES ? 2 : PAIR ? 4 : 3, KEYS = PAIR ? 1 : 0, ROWS = PAIR ? 0 : 1, VALUES = STATES ? 1 : 2;
   // (nothing else is in shared memory, so that this starts on a boundary of the swizzle's period; there is no room to move it)
   extern __shared__ __align__(1024) uint8_t mem[];
   const uint32_t base = smem_u32(mem);
@@ -165,7 +175,8 @@ __device__ __forceinline__ void la_tc_block(const LtParams& A, const int ji, con
   const int chunks = end > begin ? (end - begin + C - 1) / C : 0;
   auto chunk_at = [&](int c) { return begin + (rev ? chunks - 1 - c : c) * C; };
 
-  auto out_tile = [&](int u) { return PAIR ? TILES * (u >> 1) + 3 * (u & 1) : TILES * u + KEYS; };  // whose place a step's outputs take
+  const bool rest = !HALF && !PAIR && (STATES || J.precise);  // K' in three parts
+  auto out_tile = [&](int u) { return PAIR ? TILES * (u >> 1) + 3 * (u & 1) : TILES * u + ROWS; };  // whose place a step's outputs take
 
   const uint32_t bars = base + Cfg::BARS;
   auto full = [&](int i) { return bars + 8u * i; };
@@ -173,15 +184,14 @@ __device__ __forceinline__ void la_tc_block(const LtParams& A, const int ji, con
   const uint32_t one = bars + 16u * NS;
   const uint32_t scores_ready = one, keys_ready = one + 8, pairs_ready = one + 16, inter_done = one + 24, delta_ready = one + 32,
                  state_ready = one + 40, out_ready = one + 48, out_free = one + 56, all_done = one + 64, tail_ready = one + 72,
-                 staged = one + 80, scaled = one + 88, taken = one + 96;
+                 staged = one + 80, scaled = one + 88, taken = one + 96, rest_ready = one + 104, keys_free = one + 112;
   // A barrier's waiter can only tell one phase from the next.  Two barriers in turn where the other side can be a chunk ahead.
   auto sum_keys_ready = [&](int c) { return c & 1 ? pairs_ready : keys_ready; };  // forming sums: keys two chunks ahead at most
   auto sum_done = [&](int c) { return c & 1 ? out_ready : inter_done; };          // and what they were added to
-  auto sum_keys = [&](int c) { return c & 1 ? TM_SCORES : TM_KEYS; };
-  auto sum_delta = [&](int c) { return c & 1 ? TM_OUT : TM_DELTA; };
-  auto sum_read = [&](int c) { return c & 1 ? scaled : state_ready; };  // a sum of two chunks before is in registers
+  auto sum_keys = [&](int c) { return (c & 1) * TM_SUM_KEYS; };
   float* const powers = reinterpret_cast<float*>(mem + Cfg::TABLES);
   uint2* const key_weights = reinterpret_cast<uint2*>(powers + 32);  // of tokens 2i and 2i + 1: what bf16 keeps of them, the rest
+  float* const key_weights32 = reinterpret_cast<float*>(key_weights + 64);
 
   if (warp == 0) {
     if (lane == 0) {
@@ -203,6 +213,8 @@ __device__ __forceinline__ void la_tc_block(const LtParams& A, const int ji, con
       mbar_init(staged, 256);
       mbar_init(scaled, 256);
       mbar_init(taken, 1);
+      mbar_init(rest_ready, 256);
+      mbar_init(keys_free, 1);
       fence_mbar_init();
     }
   } else if (warp == 1) {
@@ -227,7 +239,7 @@ __device__ __forceinline__ void la_tc_block(const LtParams& A, const int ji, con
 #pragma unroll
         for (int x = 0; x < TILES; ++x) {
           if (!mbar_wait(empty(i), (round & 1) ^ 1, w, 101)) break;
-          const int blocks = (x > KEYS ? DO : DI) / 64, from = x == 3 ? ji + 1 : ji, tensor = x == 3 ? 0 : STATES ? x + 1 : x;
+          const int blocks = (x >= VALUES ? DO : DI) / 64, from = x == 3 ? ji + 1 : ji, tensor = x == KEYS ? 1 : x == VALUES ? 2 : 0;
           mbar_arrive_expect_tx(full(i), blocks * TILE);
           for (int k = 0; k < blocks; ++k)
             tma_load_4d(base + i * Cfg::SLOT + k * TILE, &A.map[from][tensor], full(i), k * 64, t0, h * A.h_step[from][tensor], b * A.b_step[from][tensor]);
@@ -246,7 +258,7 @@ __device__ __forceinline__ void la_tc_block(const LtParams& A, const int ji, con
     const uint32_t lead = elect_one();
     // (M, N, whether A and B have their rows along K)
     constexpr uint32_t ID_SCORES = make_idesc_bf16(128, 128, 0, 0) - Pair<E>::IDESC, ID_OUT = make_idesc_bf16(128, DO, 0, 1) - Pair<E>::IDESC,
-                       ID_OUT2 = make_idesc_bf16(128, DI, 0, 1) - Pair<E>::IDESC, ID_INTER2 = make_idesc_bf16(128, DI, 0, 0) - Pair<E>::IDESC;
+                       ID_OUT2 = make_idesc_bf16(128, DI, 0, 1) - Pair<E>::IDESC, ID_INTER2 = make_idesc_bf16(128, DI, 0, 0) - Pair<E>::IDESC, ID_REST = make_idesc_bf16(128, DO, 1, 1) - Pair<E>::IDESC;
     auto slot = [&](int tile) { return base + (tile % NS) * Cfg::SLOT; };
     auto loaded = [&](int tile, int code) { mbar_wait(full(tile % NS), (tile / NS) & 1, w, code); };
     // K-major operands: 16 of the 64 columns of a 128-byte row at a time
@@ -266,24 +278,23 @@ __device__ __forceinline__ void la_tc_block(const LtParams& A, const int ji, con
           if (!second) {
 #pragma unroll 2
             for (int ks = 0; ks < DI / 16; ++ks)
-              umma_ss_warp(tm + TM_OUT, k_major(slot(tile), ks), mn_major(base + Cfg::STATE, ks), ID_OUT, ks != 0, lead);
+              umma_ss_warp(tm + TM_OUT, k_major(slot(tile + ROWS), ks), mn_major(base + Cfg::STATE, ks), ID_OUT, ks != 0, lead);
           } else {
 #pragma unroll 2
             for (int ks = 0; ks < DO / 16; ++ks)
               umma_ss_warp(tm + TM_OUT, k_major(slot(tile + 3), ks), k_major(base + Cfg::STATE, ks), ID_INTER2, ks != 0, lead);
           }
-          if (lead) {
-            umma_commit(inter_done);
-            if (!PAIR) umma_commit(empty(tile % NS));
-          }
+          if (lead) umma_commit(inter_done);
           __syncwarp();
         }
         loaded(tile + VALUES, 115);
         const uint32_t v = slot(tile + VALUES);
-        if (!PAIR || second) {
+        const bool add = !PAIR || second;
+        const uint32_t delta = tm + (STATES ? TM_SUM_DELTA : TM_DELTA);
+        if (add) {
           if (STATES) {
             mbar_wait(sum_keys_ready(c), (c >> 1) & 1, w, 114);
-            if (c > 1) mbar_wait(sum_read(c), ((c >> 1) - 1) & 1, w, 112);
+            if (c > 0) mbar_wait(state_ready, (c - 1) & 1, w, 112);
           } else {
             mbar_wait(keys_ready, c & 1, w, 114);
           }
@@ -291,11 +302,20 @@ __device__ __forceinline__ void la_tc_block(const LtParams& A, const int ji, con
           const uint32_t keys = tm + (STATES ? sum_keys(c) : TM_KEYS);
 #pragma unroll 2
           for (int x = 0; x < C / 8; ++x)
-            umma_ts_warp(tm + (STATES ? sum_delta(c) : TM_DELTA), keys + (x & 1) * 64 + (x >> 1) * 8, mn_major(v, x >> 1), ID_OUT, x != 0, lead);
+            umma_ts_warp(delta, keys + (x & 1) * 64 + (x >> 1) * 8, mn_major(v, x >> 1), ID_OUT, x != 0, lead);
+          if (STATES && rest) {
+#pragma unroll 2
+            for (int ks = 0; ks < C / 16; ++ks) umma_ts_warp(delta, keys + 128 + ks * 8, mn_major(v, ks), ID_OUT, true, lead);
+          }
           if (lead) {
-            umma_commit(STATES ? sum_done(c) : delta_ready);
-            if (STATES) umma_commit(empty((tile + KEYS) % NS));
-            if (STATES || PAIR) umma_commit(empty((tile + VALUES) % NS));
+            if (STATES) {
+              umma_commit(sum_done(c));
+              umma_commit(empty((tile + KEYS) % NS));
+              umma_commit(empty((tile + VALUES) % NS));
+            } else {
+              umma_commit(keys_free);
+              if (!rest) umma_commit(delta_ready);
+            }
           }
           __syncwarp();
         }
@@ -307,10 +327,19 @@ __device__ __forceinline__ void la_tc_block(const LtParams& A, const int ji, con
 #pragma unroll 2
           for (int ks = 0; ks < C / 16; ++ks)
             umma_ts_warp(tm + TM_OUT, tm + TM_SCORES + 16 * ks, mn_major(values, ks), second ? ID_OUT2 : ID_OUT, true, lead);
-          if (lead) {
-            umma_commit(out_ready);
-            if (!PAIR) umma_commit(empty((tile + VALUES) % NS));
-            if (second) umma_commit(empty((tile + KEYS) % NS));
+          if (lead) umma_commit(out_ready);
+          __syncwarp();
+          if (rest) {
+            mbar_wait(rest_ready, c & 1, w, 114);
+            tcgen05_fence_after();
+#pragma unroll 2
+            for (int ks = 0; ks < C / 16; ++ks) umma_ss_warp(delta, mn_major(slot(tile + KEYS), ks), mn_major(v, ks), ID_REST, true, lead);
+            if (lead) umma_commit(delta_ready);
+            __syncwarp();
+          }
+          if (add && lead) {
+            umma_commit(empty((tile + KEYS) % NS));
+            umma_commit(empty((tile + VALUES) % NS));
           }
           __syncwarp();
         }
@@ -318,7 +347,7 @@ __device__ __forceinline__ void la_tc_block(const LtParams& A, const int ji, con
       if (!STATES && i < chunks * STEPS) {
         const int n = PAIR ? i >> 1 : i;
         const bool two = PAIR && (i & 1);
-        const int rows = TILES * n + (two ? 3 : 0), keys = TILES * n + (two ? VALUES : KEYS);
+        const int rows = TILES * n + (two ? 3 : ROWS), keys = TILES * n + (two ? VALUES : KEYS);
         loaded(rows, 110);
         loaded(keys, 111);
         if (chunk_at(n) + C > end) mbar_wait(tail_ready, 0, w, 119);
@@ -336,7 +365,7 @@ __device__ __forceinline__ void la_tc_block(const LtParams& A, const int ji, con
     if (lead) umma_commit(all_done);
     mbar_wait(all_done, 0, drain, 118);
   } else if (warp == 2) {
-    // ---- stores: outputs from the slot that held the keys (of a pair: the rows), which is free after that
+    // ---- stores: outputs from the slot that held the rows, which is free after that
     if (!STATES && lane == 0) {
       for (int u = 0; u < chunks * STEPS; ++u) {
         const int c = PAIR ? u >> 1 : u, job = PAIR ? ji + (u & 1) : ji, slot = out_tile(u) % NS;
@@ -386,15 +415,16 @@ __device__ __forceinline__ void la_tc_block(const LtParams& A, const int ji, con
       if (STATES || n != have) {  // the keys' weights: they change with the number of tokens, and towards a segment's end
         named_bar_sync(1, 256);
         if (a < 64) {
-          float x[2], rest[2];
+          float x[2], left[2];
 #pragma unroll
           for (int e = 0; e < 2; ++e) {
             const int s = 2 * a + e;
             const int steps = STATES ? (rev ? t0 + s - begin + 1 : end - 1 - t0 - s) : rev ? s + 1 : n - 1 - s;
             x[e] = s < n ? J.key_scale * g.power(steps) : 0.f;
-            rest[e] = x[e] - Pair<E>::kept(x[e]);
+            left[e] = x[e] - Pair<E>::kept(x[e]);
           }
-          key_weights[a] = make_uint2(pack2<E>(x[0], x[1]), pack2<E>(rest[0], rest[1]));
+          key_weights[a] = make_uint2(pack2<E>(x[0], x[1]), pack2<E>(left[0], left[1]));
+          key_weights32[2 * a] = x[0], key_weights32[2 * a + 1] = x[1];
         }
         named_bar_sync(1, 256);
         have = n;
@@ -402,9 +432,11 @@ __device__ __forceinline__ void la_tc_block(const LtParams& A, const int ji, con
       // what read the last keys: the chunk before's delta; forming sums, of two chunks before
       if (STATES ? c > 1 : c > 0) {
         if (STATES) mbar_wait(sum_done(c), ((c >> 1) - 1) & 1, w, 121);
-        else mbar_wait(delta_ready, (c - 1) & 1, w, 121);
+        else mbar_wait(keys_free, (c - 1) & 1, w, 121);
         tcgen05_fence_after();
       }
+      // in fp32, of bf16 products: z w - hi - lo, rounded
+      auto remains = [](uint32_t z, f32x2 w32, E2 hi, E2 lo) { return pack2<E>(add2(fma2(wide(z), w32, wide(bits(__hneg2(hi)))), wide(bits(__hneg2(lo))))); };
       if (q * 32 < DI) {
         // k w = hi + lo with w = w_hi + w_lo, all of the tensors' type: hi = k w_hi rounded, what that leaves is exact (half of the
         // product's bits), lo = k w_lo + that, rounded.  Three instructions for two elements, where the way through fp32 takes eight.
@@ -418,23 +450,50 @@ __device__ __forceinline__ void la_tc_block(const LtParams& A, const int ji, con
           for (int e = 0; e < 4; ++e) wt[e] = kw[(j * 4 + e) * 4];
 #pragma unroll
           for (int i = 0; i < 2; ++i) {  // 16 columns
-            uint32_t hi[8], lo[8];
+            uint32_t hi[8], lo[8], left[8];
             ldmatrix_x4_trans(from + sw128_offset(row + j * 32, in + i * 16), lo);
             ldmatrix_x4_trans(from + sw128_offset(row + j * 32 + 16, in + i * 16), lo + 4);
 #pragma unroll
             for (int e = 0; e < 8; ++e) {
               const E2 wh = *reinterpret_cast<const E2*>(&wt[e >> 1].x), wl = *reinterpret_cast<const E2*>(&wt[e >> 1].y),
                        z = *reinterpret_cast<const E2*>(lo + e), h2 = __hmul2_rn(z, wh), l2 = __hfma2(z, wl, __hfma2(z, wh, __hneg2(h2)));
-              hi[e] = *reinterpret_cast<const uint32_t*>(&h2);
-              lo[e] = *reinterpret_cast<const uint32_t*>(&l2);
+              if (STATES && !HALF) {
+                const float2 w32 = *reinterpret_cast<const float2*>(key_weights32 + 2 * (half * 32 + (lane & 3) + (j * 4 + (e >> 1)) * 4));
+                left[e] = remains(lo[e], pk2(w32.x, w32.y), h2, l2);
+              }
+              hi[e] = bits(h2);
+              lo[e] = bits(l2);
             }
             tmem_st_frag4(to + ((uint32_t)(i * 16) << 16) + j * 16, hi);
             tmem_st_frag4(to + ((uint32_t)(i * 16) << 16) + 64 + j * 16, lo);
+            if (STATES && !HALF) tmem_st_frag4(to + ((uint32_t)(i * 16) << 16) + 128 + j * 16, left);
           }
         }
         tmem_st_wait();
         tcgen05_fence_before();
       }
+      // What hi and lo leave of k w in fp32, in k's place, once nobody reads that any more (tensor memory has no room for it).
+      auto leave_rest = [&] {
+        named_bar_sync(1, 256);
+#pragma unroll 2
+        for (int at0 = 0; at0 < 128 * DI / 8; at0 += 256) {
+          const int i = at0 + a;
+          const int s = (i >> 3) & 127;  // eight elements of one token
+          const uint32_t at = k + (i >> 10) * TILE + sw128_offset(s, (i & 7) * 8);
+          const float x = key_weights32[s], kept = Pair<E>::kept(x);
+          const uint32_t wh_bits = pack2<E>(kept, kept), wl_bits = pack2<E>(x - kept, x - kept);
+          const E2 wh = *reinterpret_cast<const E2*>(&wh_bits), wl = *reinterpret_cast<const E2*>(&wl_bits);
+          uint32_t y[4];
+          lds128(at, y);
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            const E2 z = *reinterpret_cast<const E2*>(y + e), h2 = __hmul2_rn(z, wh), l2 = __hfma2(z, wl, __hfma2(z, wh, __hneg2(h2)));
+            y[e] = remains(y[e], pk2(x, x), h2, l2);
+          }
+          sts128(at, y[0], y[1], y[2], y[3]);
+        }
+        fence_proxy_async_smem();
+      };
       mbar_arrive(STATES ? sum_keys_ready(c) : keys_ready);
 #pragma unroll 1
       for (int step = 0; step < (STATES ? 0 : STEPS); ++step) {
@@ -478,6 +537,10 @@ __device__ __forceinline__ void la_tc_block(const LtParams& A, const int ji, con
         tmem_st_wait();
         tcgen05_fence_before();
         mbar_arrive(pairs_ready);
+      }
+      if (!STATES && !HALF && !PAIR && rest) {
+        leave_rest();
+        mbar_arrive(rest_ready);
       }
     }
   } else if (warp >= 12 && warp < 20) {
@@ -588,7 +651,7 @@ __device__ __forceinline__ void la_tc_block(const LtParams& A, const int ji, con
       for (int c = 0; c < chunks; ++c) {
         mbar_wait(sum_done(c), (c >> 1) & 1, w, 140);
         tcgen05_fence_after();
-        const uint32_t from = mine - TM_DELTA + sum_delta(c);
+        const uint32_t from = mine - TM_DELTA + TM_SUM_DELTA;
 #pragma unroll
         for (int i = 0; i < N; i += 16) {
           uint32_t x[16];
@@ -598,7 +661,7 @@ __device__ __forceinline__ void la_tc_block(const LtParams& A, const int ji, con
           for (int e = 0; e < 8; ++e) S[i / 2 + e] = fma2(pk2(1.f, 1.f), S[i / 2 + e], pk2u(x[2 * e], x[2 * e + 1]));
         }
         tcgen05_fence_before();
-        mbar_arrive(sum_read(c));
+        mbar_arrive(state_ready);
       }
     } else {
       const int part = (end - begin) % C;  // tokens of the one chunk that is not whole, 0: there is none
@@ -758,7 +821,7 @@ int la_tc_launch(const LaLaunch& L, int dtype, bool sums, cudaStream_t s) {
   P.L = L;
   P.L.jobs = 0;
   const bool at_once = L.B * L.H * L.segments * L.jobs <= LA_TC_BLOCKS;
-  if (!sums && L.jobs == 3 && !at_once) {
+  if (!sums && L.jobs == 3 && !at_once && !L.job[2].precise) {  // (a pair needs its keys to the end of a chunk: no room for their rest)
     const int order[3] = {0, 2, 1};
     for (int j : order)
       if (!add_job(&P, L.job[j], false)) return RINGRNN_ERR_CUDA;

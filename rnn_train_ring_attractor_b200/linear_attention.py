@@ -72,10 +72,6 @@ def _check_qkv(q, k, v, log_decay, dims, widest):
     return lead, dk, dv
 
 
-def _ptr(t):
-    return 0 if t is None else t.data_ptr()
-
-
 def _problem(q, k, v, log_decay, scale, lengths, initial_state):
     B, T, H, dk = q.shape
     qb, qt, qh, _ = q.stride()
@@ -168,8 +164,10 @@ def linear_attention(q, k, v, log_decay, scale=None, initial_state=None, lengths
     ``lengths`` [B] int32: sequences end after that many tokens (0 to T); outputs beyond are zero, and what q, k and v hold
     there has no influence.  A NaN or an infinity inside a sequence may reach up to 127 tokens before it.
 
-    Sums and states are fp32.  float32 and float16 inputs are multiplied in fp32; bfloat16 ones of widths up to 128 on tensor
-    cores, the state to sixteen bits and the scores of pairs rounded to bfloat16.
+    Sums and states are fp32.  bfloat16 and float16 of widths up to 128 are multiplied on tensor cores: products of q and k, and the
+    state where it goes into outputs, are rounded to that type (float16: weighted products of q and k from 65520 on are infinite;
+    the state is scaled by a power of two first), what is added to the state keeps 22 bits or more.  Everything else is
+    multiplied to fp32's precision; an infinity among the inputs may come out as NaN.
     Gradients: q, k, v and initial_state, from those of out and final_state.
     """
     lead, dk, dv = _check_qkv(q, k, v, log_decay, 4, MAX_WIDTH)

@@ -78,13 +78,14 @@ def attend_bounds(dtype, T, widest, tensor_cores):
     Tensor cores, beside those sums in fp32: scores of pairs, or the state, rounded to the type (u = 2^-8 for bf16, 2^-11 for fp16;
     an output is a sum of products of the two kinds).  A key k with its weight w is hi + lo: w as two numbers is off by u * u of
     it; hi = k w_hi rounded leaves at most u, which is exact; lo, of that size, is rounded once more: u * u again.  Together
-    2 u^2, with a factor of 1 + 2 u for the products of these parts."""
+    2 u^2, with a factor of 1 + 2 u for the products of these parts.  States that the caller sees have a third part in bf16, of
+    2 u^2 at most, rounded to u of it, with w to 2^-24: 2 u^3 + 2^-24, 2^-22 on the safe side."""
     sums = (T + widest + 16) * 2.0 ** -23
     if not tensor_cores:
         return sums + 2.0 ** -22, sums + 2.0 ** -22
     u = U[dtype]
     keys = 2 * u * u * (1 + 2 * u)
-    return u * (1 + 2 * keys) + keys + sums, keys + sums
+    return u * (1 + 2 * keys) + keys + sums, (2.0 ** -22 if dtype is torch.bfloat16 else keys) + sums
 
 
 def single_floor(T, widest, *inputs):
