@@ -313,9 +313,10 @@ typedef struct RingRnnStrided {
  *   lengths [B] int32 device, NULL = T each; values are clamped to 0..T.  out beyond a sequence's length is zero, and the
  *     inputs there have no influence, whatever they hold
  *   initial_state, final_state [B,H,dk,dv] fp32 contiguous, NULL = zero / not wanted
- * Sums and states are held in fp32.  With fp32 and fp16 tensors all products are fp32 too.  With bf16 tensors and widths up to
- * 128 they run on tensor cores: keys weighted by their decay and states keep sixteen bits as sums of two bf16 numbers, the
- * weighted scores q.k are rounded to bf16. */
+ * Sums and states are held in fp32.  bf16 and fp16 tensors of widths up to 128 run on tensor cores: weighted scores q.k, and the
+ * state where it goes into outputs, are rounded to their type (fp16: scores from 65520 on are infinite; the state is scaled by
+ * a power of two first); what is added to a state keeps 22 bits or more, sixteen inside a gradient.  All else is multiplied
+ * to fp32's precision; an infinity among the inputs may come out as NaN. */
 typedef struct RingRnnLinearAttention {
   int B, T, H, dk, dv;
   int dtype; /* RINGRNN_F32 ... */

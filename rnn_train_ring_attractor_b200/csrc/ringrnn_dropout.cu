@@ -3,7 +3,9 @@
 // Philox4x32-10 (Salmon, Moraes, Dror, Shaw: "Parallel random numbers: as easy as 1, 2, 3", 2011): ten rounds of two 32 x 32 ->
 // 64-bit products on a counter of four words, each giving four random words, one per element.  Bound by the memory: x (and the
 // residual) read, y written.  A counter costs 20 wide products and about as many three-input logic operations for 4 elements,
-// which at bf16 is the next bound, not far behind: see the launch.
+// which at bf16 is the next bound, not far behind.  Measured, 67 M elements: bf16 71 us (3.8 TB/s, bound by those instructions),
+// with a residual 78 (5.2 TB/s), fp32 with a residual 141 (5.7 TB/s).  Rows that are not a multiple of 16 bytes go element by
+// element: bf16 178 us.
 #include <math.h>
 
 #include "element.cuh"

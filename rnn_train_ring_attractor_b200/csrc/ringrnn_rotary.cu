@@ -13,8 +13,9 @@ namespace ringrnn {
 namespace {
 
 constexpr int THREADS = 128;
-// threads per SM that heads are shared out for; measured at the sizes below, 1536: 62.5 us, 3072: 61.5
-constexpr long long WANTED = 3072;
+// threads per SM that heads are shared out for; measured at the sizes below, adjacent pairs and halves (us): 1536: 62.5, 2560: 61.4
+// and 67.6, 2944: 61.5 and 63.5, 4096: 71.7 and 69.7
+constexpr long long WANTED = 2944;
 
 struct RotaryArgs {
   int T, Hq, Hk, D, half;  // half = rotated / 2
