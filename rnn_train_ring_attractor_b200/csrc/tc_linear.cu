@@ -148,7 +148,7 @@ __device__ __forceinline__ void regs_up() { asm volatile("setmaxnreg.inc.sync.al
 // of a second round is a dQ block's 57 on most processors (128 pairs and 128 dQ on 148).
 enum Mode { OUTPUTS, SUMS, GRADIENT_PAIR };
 
-template <class E, int DI, int DO, int MODE>
+template <class E, int DI, int DO, int MODE, bool PRECISE>
 __device__ __forceinline__ void la_tc_block(const LtParams& A, const int ji, const int at, volatile int* host_status) {
   using Cfg = LtCfg<DI, DO>;
   constexpr bool STATES = MODE == SUMS, PAIR = MODE == GRADIENT_PAIR;
@@ -175,7 +175,7 @@ __device__ __forceinline__ void la_tc_block(const LtParams& A, const int ji, con
   const int chunks = end > begin ? (end - begin + C - 1) / C : 0;
   auto chunk_at = [&](int c) { return begin + (rev ? chunks - 1 - c : c) * C; };
 
-  const bool rest = !HALF && !PAIR && (STATES || J.precise);  // K' in three parts
+  const bool rest = PRECISE && !HALF && !PAIR && (STATES || J.precise);  // K' in three parts
   auto out_tile = [&](int u) { return PAIR ? TILES * (u >> 1) + 3 * (u & 1) : TILES * u + ROWS; };  // whose place a step's outputs take
 
   const uint32_t bars = base + Cfg::BARS;
@@ -538,7 +538,7 @@ __device__ __forceinline__ void la_tc_block(const LtParams& A, const int ji, con
         tcgen05_fence_before();
         mbar_arrive(pairs_ready);
       }
-      if (!STATES && !HALF && !PAIR && rest) {
+      if (PRECISE && !STATES && rest) {
         leave_rest();
         mbar_arrive(rest_ready);
       }
@@ -742,15 +742,15 @@ __device__ __forceinline__ void la_tc_block(const LtParams& A, const int ji, con
 
 template <class E, int DI, int DO, int MODE>
 __global__ void __launch_bounds__(LT_THREADS, 1) la_tc_kernel(const __grid_constant__ LtParams A, volatile int* host_status) {
-  la_tc_block<E, DI, DO, MODE>(A, (int)(blockIdx.x % A.L.jobs), (int)(blockIdx.x / A.L.jobs), host_status);
+  la_tc_block<E, DI, DO, MODE, true>(A, (int)(blockIdx.x % A.L.jobs), (int)(blockIdx.x / A.L.jobs), host_status);
 }
 // Gradients: jobs dQ, dV, dK.  The longer blocks first, so that the others fill the last round: dV and dK of each sequence, head and
 // segment together, then dQ (inner and outer widths exchanged).
 template <class E, int DK, int DV>
 __global__ void __launch_bounds__(LT_THREADS, 1) la_tc_gradients_kernel(const __grid_constant__ LtParams A, volatile int* host_status) {
   const int pairs = gridDim.x / 2;
-  if ((int)blockIdx.x < pairs) la_tc_block<E, DK, DV, GRADIENT_PAIR>(A, 1, (int)blockIdx.x, host_status);
-  else la_tc_block<E, DV, DK, OUTPUTS>(A, 0, (int)blockIdx.x - pairs, host_status);
+  if ((int)blockIdx.x < pairs) la_tc_block<E, DK, DV, GRADIENT_PAIR, false>(A, 1, (int)blockIdx.x, host_status);
+  else la_tc_block<E, DV, DK, OUTPUTS, false>(A, 0, (int)blockIdx.x - pairs, host_status);
 }
 
 bool make_map(CUtensorMap* m, const LaOperand& o, int width, int B, int T, int H, int* h_step, int* b_step) {
