@@ -20,7 +20,7 @@
 //
 // What bounds it: at widths of 128 the memory (a chunk is 128 KB, 5500 cycles of an SM's share at 6.5 TB/s); then shared memory's
 // 128 bytes per cycle, which products with both operands there use up.  P and K' therefore live in tensor memory, and V is all
-// that is read beside them: 3600 cycles of shared memory per chunk, where the transposed arrangement (columns on the lanes, so that
+// that is read beside them: 3600 cycles of shared memory per chunk (4500 with K' in three parts), where the transposed arrangement (columns on the lanes, so that
 // the state is the operand in tensor memory, P and K' in shared memory) took 5200 and was bound by that.
 //
 // Roles (28 warps): 0 TMA loads; 1 MMA issue; 2 TMA stores; 4-11 weight the keys and the scores; 12-19 scale inter and bring the

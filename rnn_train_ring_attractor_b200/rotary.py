@@ -98,7 +98,7 @@ def rotary(q, k, frequencies, positions=0, interleaved=False, amplitude=1.0):
     heads of their own; one launch for both.  ``frequencies`` [R/2] float64 (``rotary_frequencies``), R <= D.  ``positions``: the
     position of the first token, or an int32 / int64 tensor [B,T] (an expanded one will do) with each token's.  Pairs are
     elements (2i, 2i+1) if ``interleaved``, else (i, i + R/2).  ``amplitude`` multiplies the turned elements.  Angles are formed
-    in 64 bits, so that positions of millions are as exact as small ones."""
+    in 64 bits, so that positions of millions are as exact as small ones.  Gradients: q and k."""
     if q.dtype not in DTYPES:
         raise RuntimeError("q must be float32, bfloat16 or float16")
     dev = q.device
@@ -112,6 +112,8 @@ def rotary(q, k, frequencies, positions=0, interleaved=False, amplitude=1.0):
     if (frequencies.dtype != torch.float64 or frequencies.dim() != 1 or frequencies.device != dev
             or not 1 <= frequencies.shape[0] <= q.shape[3] // 2):
         raise RuntimeError("frequencies must be float64 [rotated / 2] on q's device, rotated <= width")
+    if frequencies.requires_grad and torch.is_grad_enabled():
+        raise RuntimeError("frequencies have no gradient: they are constants of the layer (pass frequencies.detach())")
     frequencies = frequencies.detach().contiguous()
     first = 0
     if torch.is_tensor(positions):

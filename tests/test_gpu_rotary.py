@@ -138,3 +138,12 @@ def test_refusals_and_empty_calls():
             rotary(*bad)
     a, b = rotary(q[:, :0], k[:, :0], f)
     assert a.shape == (2, 0, 2, 8) and b.shape == (2, 0, 1, 8)
+
+
+def test_frequencies_that_ask_for_a_gradient_are_refused():
+    q = torch.randn(1, 3, 2, 8, device="cuda")
+    f = rotary_frequencies(8).requires_grad_()
+    with pytest.raises(RuntimeError, match="frequencies have no gradient"):
+        rotary(q, None, f)
+    with torch.no_grad():
+        assert torch.equal(rotary(q, None, f)[0], rotary(q, None, f.detach())[0])
