@@ -24,7 +24,7 @@
 // the state is the operand in tensor memory, P and K' in shared memory) took 5200 and was bound by that.
 //
 // Roles (28 warps): 0 TMA loads; 1 MMA issue; 2 TMA stores; 4-11 weight the keys and the scores; 12-19 scale inter and bring the
-// outputs to shared memory (where k was); 20-27 keep the state, half a row each.  A scheduler has two warps of a role at a time,
+// outputs to shared memory (where q was); 20-27 keep the state, half a row each.  A scheduler has two warps of a role at a time,
 // each at its own place in the code, and waits for instructions more than for anything else once that outgrows the instruction
 // cache (13 cycles for each instruction, with everything unrolled): loops stay rolled, pairs of fp32 are computed as such, and
 // what only a partial chunk needs is done apart.  The tensor pipe's order is inter, delta, out, the next scores: the chain of a
