@@ -508,20 +508,21 @@ struct Plan {
 // Segments of a sequence.  Forming their sums reads keys and values once more and is a launch of its own, with the scan behind it,
 // so a sequence is only cut where that brings more CTAs to work: the number of segments with the least time by the model
 //   rounds of CTAs x (start + chunks of a segment x chunk), for n > 1 the same again with part of a chunk's time, and the scan.
-// Measured (us): tensor cores start 6, chunk 2, sums 0.7 of it, scan 7; fp32 arithmetic start 6, chunk 4, sums 0.4 of it, scan 7.
-// 10 for the two scans of gradients, which are three CTAs a segment, or two where those of keys and values go together (1.4 of a
+// Measured (us): tensor cores start 6, chunk 3, sums 0.55 of it; fp32 arithmetic start 6, chunk 4, sums 0.4 of it; a scan with the
+// gaps between launches 10.  (64 heads of 64, 16384 tokens, forward: cut in two 258 us, whole 311; 48 heads of 2048 tokens in three
+// 66, whole 62.)  12 for the two scans of gradients, which are three CTAs a segment, or two where those of keys and values go together (1.55 of a
 // CTA's time): those first, then the others on what is free.
 int cut(const RingRnnLinearAttention& p, bool tensor_cores, bool backward) {
   const int chunk = tensor_cores ? LA_TC_CHUNK : PC, at_once = tensor_cores ? LA_TC_BLOCKS : 296;
   const long long slices = tensor_cores ? 1 : ((p.dk > p.dv && backward ? p.dk : p.dv) + PO - 1) / PO;
   const long long each_job = (long long)p.B * p.H * slices, chunks = ((long long)p.T + chunk - 1) / chunk;
-  const double start = 6, each = tensor_cores ? 2 : 4, sums = tensor_cores ? 0.7 : 0.4, scan = backward ? 10 : 7;
+  const double start = 6, each = tensor_cores ? 3 : 4, sums = tensor_cores ? 0.55 : 0.4, scan = backward ? 12 : 10;
   auto rounds = [&](long long ctas) { return (double)((ctas + at_once - 1) / at_once); };
   auto rounds_of_all = [&](long long n) {
     const long long ctas = each_job * n;
     if (!backward || !tensor_cores || 3 * ctas <= at_once) return rounds((backward ? 3 : 1) * ctas);
     const long long full = ctas / at_once, more = ctas % at_once;  // after the pairs, `more` are free a pair's time after the others
-    const double pair = 1.4, free[2] = {pair * full, pair * (full + 1)};
+    const double pair = 1.55, free[2] = {pair * full, pair * (full + 1)};
     auto whole = [](double x) { return x < 0 ? 0 : (long long)(x + 1e-9); };
     double least = more > 0 ? free[1] : free[0], end = 1e30;
     for (double from : free)
@@ -534,11 +535,11 @@ int cut(const RingRnnLinearAttention& p, bool tensor_cores, bool backward) {
     return end > least ? end : least;
   };
   int best = 1;
-  double least = rounds_of_all(1) * (start + chunks * each);
+  double least = 0.9 * rounds_of_all(1) * (start + chunks * each);  // (a model: it has to promise a tenth)
   for (long long n = 2; n <= chunks / 2 && each_job * (backward ? 3 : 1) * (n - 1) < 2 * at_once; ++n) {
     const long long per = (chunks + n - 1) / n;
     const double t = rounds_of_all(n) * (start + per * each) + rounds((backward ? 2 : 1) * each_job * n) * (start + per * each * sums) + scan;
-    if (t < 0.9 * least) least = t, best = (int)n;
+    if (t < least) least = t, best = (int)n;
   }
   return best;
 }

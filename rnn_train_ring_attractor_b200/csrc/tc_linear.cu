@@ -144,7 +144,7 @@ __device__ __forceinline__ void regs_up() { asm volatile("setmaxnreg.inc.sync.al
 // K E and the other as V E^T.  A chunk of theirs is loaded once instead of one and a half times, its keys are weighted and added
 // to the state once instead of twice, and what is left, two products of scores, of state and of values, goes through the same
 // places one after the other: step 2c is dV of chunk c, step 2c + 1 is dK.
-// Such a block takes 1.4 times as long as one job's.  Measured: gradients of 8 x 2048 x 16 heads of 128, 150 us -> 137; what is left
+// Such a block takes 1.55 times as long as one job's.  Measured: gradients of 8 x 2048 x 16 heads of 128, 150 us -> 137; what is left
 // of a second round is a dQ block's 57 on most processors (128 pairs and 128 dQ on 148).
 enum Mode { OUTPUTS, SUMS, GRADIENT_PAIR };
 
