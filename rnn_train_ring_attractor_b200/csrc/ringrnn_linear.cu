@@ -509,9 +509,9 @@ struct Plan {
 // so a sequence is only cut where that brings more CTAs to work: the number of segments with the least time by the model
 //   rounds of CTAs x (start + chunks of a segment x chunk), for n > 1 the same again with part of a chunk's time, and the scan.
 // Measured (us): tensor cores start 6, chunk 3, sums 0.55 of it; fp32 arithmetic start 6, chunk 4, sums 0.4 of it; a scan with the
-// gaps between launches 10.  (64 heads of 64, 16384 tokens, forward: cut in two 258 us, whole 311; 48 heads of 2048 tokens in three
-// 66, whole 62.)  12 for the two scans of gradients, which are three CTAs a segment, or two where those of keys and values go together (1.55 of a
-// CTA's time): those first, then the others on what is free.
+// gaps between launches 10, the two scans of gradients 12.  (64 heads of 64, 16384 tokens, forward: cut in two 258 us, whole 311;
+// 48 heads of 128, 2048 tokens: in three 66, whole 62.)  Gradients are three CTAs a segment, or two where those of keys and values
+// go together (1.55 of a CTA's time): those first, then the others on what is free.
 int cut(const RingRnnLinearAttention& p, bool tensor_cores, bool backward) {
   const int chunk = tensor_cores ? LA_TC_CHUNK : PC, at_once = tensor_cores ? LA_TC_BLOCKS : 296;
   const long long slices = tensor_cores ? 1 : ((p.dk > p.dv && backward ? p.dk : p.dv) + PO - 1) / PO;

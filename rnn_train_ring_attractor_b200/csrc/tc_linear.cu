@@ -18,10 +18,12 @@
 // fp16 has three bits more and little range: the state is multiplied by the power of two that brings its largest element just
 // below 2^15 before it is rounded, and inter divided by it again.  Scores have no such power: weighted ones from 65520 on are infinite.
 //
-// What bounds it: at widths of 128 the memory (a chunk is 128 KB, 5500 cycles of an SM's share at 6.5 TB/s); then shared memory's
-// 128 bytes per cycle, which products with both operands there use up.  P and K' therefore live in tensor memory, and V is all
-// that is read beside them: 3600 cycles of shared memory per chunk (4500 with K' in three parts), where the transposed arrangement (columns on the lanes, so that
-// the state is the operand in tensor memory, P and K' in shared memory) took 5200 and was bound by that.
+// What bounds it: at widths of 128 the memory's share (a chunk is 128 KB, 5500 cycles of an SM's share at 6.5 TB/s when all SMs
+// read), then shared memory's 128 bytes per cycle, which products with both operands there use up.  P and K' therefore live in tensor
+// memory, and V is all that is read beside them: 3600 cycles of shared memory per chunk (4500 with K' in three parts), where the
+// transposed arrangement (columns on the lanes, so that the state is the operand in tensor memory, P and K' in shared memory) took
+// 5200 and was bound by that.  What a chunk takes is 5500 cycles (6100), the chain from one state to the next: products wait for
+// shared memory, and the roles for one another's instructions.
 //
 // Roles (28 warps): 0 TMA loads; 1 MMA issue; 2 TMA stores; 4-11 weight the keys and the scores; 12-19 scale inter and bring the
 // outputs to shared memory (where q was); 20-27 keep the state, half a row each.  A scheduler has two warps of a role at a time,
@@ -242,7 +244,8 @@ __device__ __forceinline__ void la_tc_block(const LtParams& A, const int ji, con
           const int blocks = (x >= VALUES ? DO : DI) / 64, from = x == 3 ? ji + 1 : ji, tensor = x == KEYS ? 1 : x == VALUES ? 2 : 0;
           mbar_arrive_expect_tx(full(i), blocks * TILE);
           for (int k = 0; k < blocks; ++k)
-            tma_load_4d(base + i * Cfg::SLOT + k * TILE, &A.map[from][tensor], full(i), k * 64, t0, h * A.h_step[from][tensor], b * A.b_step[from][tensor]);
+            tma_load_4d(base + i * Cfg::SLOT + k * TILE, &A.map[from][tensor], full(i), k * 64, t0, h * A.h_step[from][tensor],
+                        b * A.b_step[from][tensor]);
           if (++i == NS) i = 0, ++round;
         }
         if (*static_cast<volatile int*>(flags)) break;
@@ -258,7 +261,8 @@ __device__ __forceinline__ void la_tc_block(const LtParams& A, const int ji, con
     const uint32_t lead = elect_one();
     // (M, N, whether A and B have their rows along K)
     constexpr uint32_t ID_SCORES = make_idesc_bf16(128, 128, 0, 0) - Pair<E>::IDESC, ID_OUT = make_idesc_bf16(128, DO, 0, 1) - Pair<E>::IDESC,
-                       ID_OUT2 = make_idesc_bf16(128, DI, 0, 1) - Pair<E>::IDESC, ID_INTER2 = make_idesc_bf16(128, DI, 0, 0) - Pair<E>::IDESC, ID_REST = make_idesc_bf16(128, DO, 1, 1) - Pair<E>::IDESC;
+                       ID_OUT2 = make_idesc_bf16(128, DI, 0, 1) - Pair<E>::IDESC, ID_INTER2 = make_idesc_bf16(128, DI, 0, 0) - Pair<E>::IDESC,
+                       ID_REST = make_idesc_bf16(128, DO, 1, 1) - Pair<E>::IDESC;
     auto slot = [&](int tile) { return base + (tile % NS) * Cfg::SLOT; };
     auto loaded = [&](int tile, int code) { mbar_wait(full(tile % NS), (tile / NS) & 1, w, code); };
     // K-major operands: 16 of the 64 columns of a 128-byte row at a time
