@@ -54,6 +54,23 @@ def test_mask_values_and_gradients(dtype, rows, n, p, numbers):
     assert torch.equal(only, d)
 
 
+@pytest.mark.parametrize("dtype", [FP32, BF16, FP16])
+@pytest.mark.parametrize("rows,n", [(1, 1), (700, 1), (333, 3), (50, 7), (41, 9), (64, 31), (300, 250), (19, 1001), (7, 65537), (2, 3000006), (600, 12)])
+def test_rows_of_any_length_and_offset_draw_like_whole_vectors(dtype, rows, n):
+    """An element's number is its row's and its own: the same as where every row is padded to whole vectors."""
+    wide = (n + 7) // 8 * 8
+    x, r = _randn(rows, wide, dtype=dtype, seed=1), _randn(rows, wide, dtype=dtype, seed=2)
+    numbers = torch.tensor([5, 9], device="cuda")
+    want, more = dropout(x, 0.3, 5, stream=9, first_row=11)[:, :n], dropout(x, 0.3, 5, stream=9, first_row=11, residual=r)[:, :n]
+    for at, at_r in ((0, 0), (1, 1), (3, 3), (1, 2), (0, 5)):
+        flat, flat_r = torch.empty(rows * n + 8, device="cuda", dtype=dtype), torch.empty(rows * n + 8, device="cuda", dtype=dtype)
+        y, z = flat[at:at + rows * n].view(rows, n), flat_r[at_r:at_r + rows * n].view(rows, n)
+        y.copy_(x[:, :n]), z.copy_(r[:, :n])
+        assert torch.equal(dropout(y, 0.3, 5, stream=9, first_row=11), want)
+        assert torch.equal(dropout(y, 0.3, 5, stream=9, first_row=11, residual=z), more)
+        assert torch.equal(dropout(y, 0.3, numbers, first_row=11, residual=z), more)
+
+
 def test_rows_draw_the_same_in_every_batch():
     x = _randn(12, 3, 50, dtype=BF16)
     whole = dropout(x, 0.4, 77, stream=5, first_row=1000)
