@@ -362,24 +362,27 @@ int scan_launch(const LaLaunch& L, int elems, int reverse, const float* init, fl
 // VEC = 4: a thread owns 4 columns of every THREADS / 8th row; VEC = 1 (odd widths or addresses): 1 column of every THREADS / 32nd.
 // Threads: as many as leave each four rows, all of them under way at once; a block for each 32 x 64 of a small state would be
 // half idle with 256 (256 sequences of 32 heads of 64: 62 us, and 47 with 128, 5.7 TB/s; heads of 128: 174 us, 6.2 TB/s).
+// WHOLE: a CTA takes all columns, its threads a few rows of them, which lie one behind the other; for widths that are no multiple of
+// 32, whose slices would share sectors and leave the last one half empty, where there are states enough for the GPU (256 sequences
+// of 32 heads of 100: 108 us, in slices 223; of 101: 156 and 249).
 constexpr int STEP_COLS = 32, STEP_MAX_DK = 1024;
-template <class E, int VEC, int STEP_THREADS>
+template <class E, int VEC, int STEP_THREADS, bool WHOLE>
 __global__ void __launch_bounds__(STEP_THREADS) la_step_kernel(int H, int dk, int dv, float scale, LaOperand q, LaOperand k,
                                                                LaOperand v, const float* __restrict__ log_decay,
                                                                const unsigned char* __restrict__ active,
                                                                float* __restrict__ state, E* __restrict__ out) {
-  constexpr int CG = STEP_COLS / VEC, ROWS = STEP_THREADS / CG;
+  const int COLS = WHOLE ? dv : STEP_COLS, CG = COLS / VEC, ROWS = STEP_THREADS / CG;
   __shared__ float sq[STEP_MAX_DK], sk[STEP_MAX_DK];
-  __shared__ float part[ROWS][STEP_COLS];
+  __shared__ float part[STEP_THREADS * VEC];  // [ROWS][COLS]
   const int tid = threadIdx.x, bh = blockIdx.x, h = bh % H, b = bh / H;
-  const int cg = tid % CG, row = tid / CG, col = blockIdx.y * STEP_COLS + cg * VEC;
+  const int cg = tid % CG, row = tid / CG, col = blockIdx.y * COLS + cg * VEC;
   if (active != nullptr && active[b] == 0) {
     if (row == 0)
       for (int e = 0; e < VEC; ++e)
         if (col + e < dv) out[(size_t)bh * dv + col + e] = down<E>(0.f);
     return;
   }
-  const bool in = col < dv;  // VEC == 4: dv is a multiple of 4
+  const bool in = col < dv && row < ROWS;  // VEC == 4: dv is a multiple of 4
   float* S = state + (size_t)bh * dk * dv + col;
   // the state's first rows are under way while q and k come in
   constexpr int AHEAD = VEC == 4 ? 4 : 8;
@@ -430,29 +433,34 @@ __global__ void __launch_bounds__(STEP_THREADS) la_step_kernel(int H, int dk, in
         if (i0 + (AHEAD + a) * ROWS < dk) fetch(s0[a], i0 + (AHEAD + a) * ROWS);
     }
   }
+  if (row < ROWS) {
 #pragma unroll
-  for (int e = 0; e < VEC; ++e) part[row][cg * VEC + e] = acc[e];
+    for (int e = 0; e < VEC; ++e) part[row * COLS + cg * VEC + e] = acc[e];
+  }
   __syncthreads();
-  if (tid < STEP_COLS && blockIdx.y * STEP_COLS + tid < dv) {
+  for (int o = tid; o < COLS && blockIdx.y * COLS + o < dv; o += STEP_THREADS) {
     float x = 0.f;
 #pragma unroll 8
-    for (int r = 0; r < ROWS; ++r) x += part[r][tid];
-    out[(size_t)bh * dv + blockIdx.y * STEP_COLS + tid] = down<E>(scale * x);
+    for (int r = 0; r < ROWS; ++r) x += part[r * COLS + o];
+    out[(size_t)bh * dv + blockIdx.y * COLS + o] = down<E>(scale * x);
   }
 }
-template <class E, int VEC, int THREADS>
+template <class E, int VEC, int THREADS, bool WHOLE = false>
 int step_launch(const RingRnnLinearAttention& p, const LaOperand& q, const LaOperand& k, const LaOperand& v, float* state,
                 const unsigned char* active, void* out, cudaStream_t s) {
-  const dim3 grid(p.B * p.H, (p.dv + STEP_COLS - 1) / STEP_COLS);
+  const dim3 grid(p.B * p.H, WHOLE ? 1 : (p.dv + STEP_COLS - 1) / STEP_COLS);
   LaunchScope ls(K_LAYER, s);
-  la_step_kernel<E, VEC, THREADS><<<grid, THREADS, 0, s>>>(p.H, p.dk, p.dv, p.scale, q, k, v, p.log_decay, active, state, static_cast<E*>(out));
+  la_step_kernel<E, VEC, THREADS, WHOLE><<<grid, THREADS, 0, s>>>(p.H, p.dk, p.dv, p.scale, q, k, v, p.log_decay, active, state, static_cast<E*>(out));
   RINGRNN_CUDA_TRY(cudaGetLastError());
   return RINGRNN_OK;
 }
 template <class E>
 int step_launch(const RingRnnLinearAttention& p, const LaOperand& q, const LaOperand& k, const LaOperand& v, float* state,
                 const unsigned char* active, void* out, cudaStream_t s) {
-  if (p.dv % 4 != 0 || (reinterpret_cast<uintptr_t>(state) & 15) != 0) return step_launch<E, 1, 256>(p, q, k, v, state, active, out, s);
+  const int vec = p.dv % 4 != 0 || (reinterpret_cast<uintptr_t>(state) & 15) != 0 ? 1 : 4;
+  if (p.dv % STEP_COLS != 0 && p.dv / vec <= 256 && (long long)p.B * p.H >= 2 * 148)
+    return vec == 1 ? step_launch<E, 1, 256, true>(p, q, k, v, state, active, out, s) : step_launch<E, 4, 256, true>(p, q, k, v, state, active, out, s);
+  if (vec == 1) return step_launch<E, 1, 256>(p, q, k, v, state, active, out, s);
   return p.dk <= 64 ? step_launch<E, 4, 128>(p, q, k, v, state, active, out, s) : step_launch<E, 4, 256>(p, q, k, v, state, active, out, s);
 }
 

@@ -332,7 +332,10 @@ def test_empty_calls():
 
 # ---- one token -----------------------------------------------------------------------------------------------------------
 @pytest.mark.parametrize("dtype,B,H,dk,dv", [(FP32, 1, 1, 1, 1), (BF16, 3, 2, 128, 128), (FP16, 2, 3, 64, 96), (BF16, 2, 2, 33, 50),
-                                             (FP32, 2, 1, 1024, 36), (BF16, 1, 2, 200, 333), (BF16, 5, 1, 8, 2)])
+                                             (FP32, 2, 1, 1024, 36), (BF16, 1, 2, 200, 333), (BF16, 5, 1, 8, 2),
+                                             # states enough to go row by row
+                                             (BF16, 20, 17, 100, 100), (FP32, 30, 10, 33, 33), (FP16, 37, 8, 128, 50), (BF16, 300, 1, 5, 1),
+                                             (BF16, 60, 5, 64, 1000), (FP32, 99, 3, 70, 256), (BF16, 75, 4, 3, 255)])
 def test_step(dtype, B, H, dk, dv, achieved):
     q, k, v, l, s, _, _, _ = _inputs(dtype, B, 1, H, dk, dv, seed=dk)
     l = l - 0.01
@@ -385,6 +388,24 @@ def test_step_strides():
 
 
 # ---- streams, graphs, refusals ----------------------------------------------------------------------------------------------
+@pytest.mark.parametrize("B,H,dk,dv", [(300, 2, 12, 100), (150, 2, 20, 33)])
+def test_step_of_many_narrow_states(B, H, dk, dv):
+    """Row by row like column by column (a state that starts off a 16-byte boundary); inactive ones stay; nothing beside is written."""
+    q, k, v, l, s, _, _, _ = _inputs(BF16, B, 1, H, dk, dv, seed=3)
+    active = torch.rand(B, device="cuda", generator=_gen(4)) < 0.7
+    one = s.clone()
+    flat = torch.full((s.numel() + 9,), 7.0, device="cuda")
+    two = flat[5:5 + s.numel()].view(s.shape)
+    two.copy_(s)
+    a, b = (linear_attention_step(q[:, 0], k[:, 0], v[:, 0], x, l, active=active) for x in (one, two))
+    few = torch.cat([linear_attention_step(q[i:i + 10, 0], k[i:i + 10, 0], v[i:i + 10, 0], s[i:i + 10], l, active=active[i:i + 10]) for i in range(0, B, 10)])
+    assert torch.equal(one, two) and torch.equal(one, s)
+    assert not a[~active].any() and not b[~active].any() and not few[~active].any()
+    room = dk * 2.0 ** -20 * (q[:, 0].float().abs().unsqueeze(-1) * s.abs()).sum(-2) + 2.0 ** -7 * few.float().abs() + 1e-30
+    assert ((a.float() - few.float()).abs() <= room).all() and ((b.float() - few.float()).abs() <= room).all()
+    assert (flat[:5] == 7.0).all() and (flat[5 + s.numel():] == 7.0).all()
+
+
 @pytest.mark.parametrize("T,H", [(300, 2), (4100, 1)])
 def test_two_streams_at_once(T, H):
     sets = [_inputs(BF16, 1, T, H, 64, 64, seed=i) for i in range(2)]
