@@ -478,27 +478,55 @@ LaOperand operand(const RingRnnStrided& t) { return LaOperand{t.data, t.batch, t
 
 // ---- operands for the tensor cores ------------------------------------------------------------------------------------
 // A tensor that TMA cannot read as it is (a stride or an address that is not a multiple of 16 bytes, tokens that share a row)
-// is copied to rows of a multiple of 8 elements first.
+// is copied to rows of a multiple of 8 elements first, as many elements at a time as addresses and strides allow.  A thread writes
+// eight and goes on by a fixed distance, kept as a number of packs, heads, tokens and sequences, where dividing for each pack cost
+// as much as the copy.  Forward of 8 x 2048 x 16 heads in bf16, with this copy: of 60 100 us (165 before), of 121, where elements
+// go one by one, 226.
 struct PackJobs {
   LaOperand from[4];
   void* to[4];
-  int width[4], padded[4];
+  int width[4], per[4], vec[4];  // packs of a row; elements that are read at a time
+  int step[4][4];                // the distance: packs, heads, tokens, sequences
 };
-__global__ void __launch_bounds__(256) la_pack_kernel(const __grid_constant__ PackJobs p, int B, int T, int H) {
-  const int j = blockIdx.y, width = p.width[j], per = p.padded[j] / 8;
-  const LaOperand o = p.from[j];
-  const size_t total = (size_t)B * T * H * per;
-  for (size_t id = blockIdx.x * (size_t)256 + threadIdx.x; id < total; id += (size_t)gridDim.x * 256) {
-    const size_t row = id / per;
-    const int i0 = (int)(id - row * per) * 8, h = (int)(row % H);
-    const size_t bt = row / H;
-    const int t = (int)(bt % T), b = (int)(bt / T);
-    const unsigned short* x = static_cast<const unsigned short*>(o.p) + b * o.sb + t * o.st + h * o.sh + i0;
-    unsigned short y[8];
+template <int VEC>
+__device__ __forceinline__ uint4 pack_of_8(const unsigned short* x, int left) {
+  typedef Pack<unsigned short, VEC> P;
+  Pack<unsigned short, 8> y;
 #pragma unroll
-    for (int e = 0; e < 8; ++e) y[e] = i0 + e < width ? x[e] : (unsigned short)0;
-    static_cast<uint4*>(p.to[j])[id] = make_uint4(y[0] | (uint32_t)y[1] << 16, y[2] | (uint32_t)y[3] << 16,
-                                                       y[4] | (uint32_t)y[5] << 16, y[6] | (uint32_t)y[7] << 16);
+  for (int e = 0; e < 8; e += VEC) {
+    P z;
+    if (e < left) {  // left is a multiple of VEC
+      z = *reinterpret_cast<const P*>(x + e);
+    } else {
+#pragma unroll
+      for (int i = 0; i < VEC; ++i) z.v[i] = 0;
+    }
+#pragma unroll
+    for (int i = 0; i < VEC; ++i) y.v[e + i] = z.v[i];
+  }
+  return *reinterpret_cast<const uint4*>(&y);
+}
+__global__ void __launch_bounds__(256) la_pack_kernel(const __grid_constant__ PackJobs p, int B, int T, int H) {
+  const int j = blockIdx.y, per = p.per[j], vec = p.vec[j];
+  const LaOperand o = p.from[j];
+  const size_t total = (size_t)B * T * H * per, step = (size_t)gridDim.x * 256;
+  size_t id = blockIdx.x * (size_t)256 + threadIdx.x;
+  const size_t row = id / per, bt = row / H;
+  int i = (int)(id - row * per), h = (int)(row % H), t = (int)(bt % T), b = (int)(bt / T);
+  for (; id < total; id += step) {
+    const unsigned short* x = static_cast<const unsigned short*>(o.p) + b * o.sb + t * o.st + h * o.sh + i * 8;
+    const int left = p.width[j] - i * 8;
+    static_cast<uint4*>(p.to[j])[id] = vec == 4 ? pack_of_8<4>(x, left) : vec == 2 ? pack_of_8<2>(x, left) : pack_of_8<1>(x, left);
+    i += p.step[j][0];
+    const int ci = i >= per;
+    i -= ci ? per : 0;
+    h += p.step[j][1] + ci;
+    const int ch = h >= H;
+    h -= ch ? H : 0;
+    t += p.step[j][2] + ch;
+    const int ct = t >= T;
+    t -= ct ? T : 0;
+    b += p.step[j][3] + ct;
   }
 }
 
@@ -585,15 +613,24 @@ int pack(const RingRnnLinearAttention& p, Plan* l, char* at, cudaStream_t s) {
     jobs.from[n] = l->op[x];
     jobs.to[n] = at;
     jobs.width[n] = l->width[x];
-    jobs.padded[n++] = padded;
+    jobs.per[n++] = padded / 8;
     most = padded > most ? padded : most;
     l->op[x] = LaOperand{at, (long long)p.T * p.H * padded, (long long)p.H * padded, padded};
     at += l->packed[x];
   }
   if (n == 0) return RINGRNN_OK;
-  const size_t blocks = ((size_t)p.B * p.T * p.H * (most / 8) + 255) / 256;
+  const size_t need = ((size_t)p.B * p.T * p.H * (most / 8) + 255) / 256, blocks = need < 148 * 16 ? need : 148 * 16;
+  for (int x = 0; x < n; ++x) {
+    const LaOperand& o = jobs.from[x];
+    const long long all = (long long)(reinterpret_cast<uintptr_t>(o.p) / 2) | jobs.width[x] | (p.B > 1 ? o.sb : 0) | (p.T > 1 ? o.st : 0) | (p.H > 1 ? o.sh : 0);
+    jobs.vec[x] = reinterpret_cast<uintptr_t>(o.p) % 2 != 0 ? 1 : all % 4 == 0 ? 4 : all % 2 == 0 ? 2 : 1;
+    size_t step = blocks * 256;
+    const int sizes[3] = {jobs.per[x], p.H, p.T};
+    for (int y = 0; y < 3; ++y) jobs.step[x][y] = (int)(step % sizes[y]), step /= sizes[y];
+    jobs.step[x][3] = (int)step;
+  }
   LaunchScope ls(K_LAYER, s);
-  la_pack_kernel<<<dim3((unsigned)(blocks < 148 * 16 ? blocks : 148 * 16), n), 256, 0, s>>>(jobs, p.B, p.T, p.H);
+  la_pack_kernel<<<dim3((unsigned)blocks, n), 256, 0, s>>>(jobs, p.B, p.T, p.H);
   RINGRNN_CUDA_TRY(cudaGetLastError());
   return RINGRNN_OK;
 }

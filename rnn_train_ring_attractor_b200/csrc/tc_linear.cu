@@ -598,14 +598,24 @@ __device__ __forceinline__ void la_tc_block(const LtParams& A, const int ji, con
           sts128(to + sw128_offset(r, (o0 & 63) + i), y[0], y[1], y[2], y[3]);
           sts128(to + sw128_offset(r, (o0 & 63) + i + 8), y[4], y[5], y[6], y[7]);
         }
-        if (!A.store[job]) {  // widths and addresses that TMA does not take: element by element
+        if (!A.store[job]) {  // widths and addresses that TMA does not take: as many elements at a time as they allow
           named_bar_sync(2, 256);
-          const int outer = L.job[job].outer, o = a & 127;
-          unsigned short* const out = static_cast<unsigned short*>(L.job[job].out) + ((size_t)b * L.T * L.H + h) * outer + o;
-#pragma unroll 1
-          for (int t = a >> 7; t < C && t0 + t < stop; t += 2)
-            if (o < outer)
-              out[(size_t)(t0 + t) * L.H * outer] = *reinterpret_cast<const unsigned short*>(mem + slot + (o >> 6) * TILE + sw128_offset(t, o & 63));
+          const int outer = L.job[job].outer;
+          unsigned short* const out = static_cast<unsigned short*>(L.job[job].out) + ((size_t)b * L.T * L.H + h) * outer;
+          auto copy = [&](auto vector) {
+            typedef decltype(vector) P;
+            constexpr int LANES = 128 * 2 / sizeof(P);  // to a row
+            const int o = (a & (LANES - 1)) * (int)(sizeof(P) / 2);
+#pragma unroll 2
+            for (int t = a / LANES; t < C && t0 + t < stop; t += 256 / LANES)
+              if (o < outer)
+                *reinterpret_cast<P*>(out + (size_t)(t0 + t) * L.H * outer + o) =
+                    *reinterpret_cast<const P*>(mem + slot + (o >> 6) * TILE + sw128_offset(t, o & 63));
+          };
+          const uintptr_t boundary = reinterpret_cast<uintptr_t>(L.job[job].out) | (uintptr_t)outer * 2;
+          if (boundary % 8 == 0) copy(uint2());
+          else if (boundary % 4 == 0) copy(uint32_t());
+          else copy((unsigned short)0);
         }
         fence_proxy_async_smem();
         if (u > 0) mbar_wait(taken, (u - 1) & 1, w, 132);  // a store may wait for the memory longer than a chunk takes
