@@ -600,18 +600,27 @@ __device__ __forceinline__ void la_tc_block(const LtParams& A, const int ji, con
         }
         if (!A.store[job]) {  // widths and addresses that TMA does not take: as many elements at a time as they allow
           named_bar_sync(2, 256);
-          const int outer = L.job[job].outer;
-          unsigned short* const out = static_cast<unsigned short*>(L.job[job].out) + ((size_t)b * L.T * L.H + h) * outer;
-          auto copy = [&](auto vector) {
-            typedef decltype(vector) P;
-            constexpr int LANES = 128 * 2 / sizeof(P);  // to a row
-            const int o = (a & (LANES - 1)) * (int)(sizeof(P) / 2);
-#pragma unroll 2
-            for (int t = a / LANES; t < C && t0 + t < stop; t += 256 / LANES)
-              if (o < outer)
-                *reinterpret_cast<P*>(out + (size_t)(t0 + t) * L.H * outer + o) =
-                    *reinterpret_cast<const P*>(mem + slot + (o >> 6) * TILE + sw128_offset(t, o & 63));
+          const int outer = L.job[job].outer, rows = min(C, stop - t0);
+          const size_t pitch = (size_t)L.H * outer;
+          unsigned short* const out = static_cast<unsigned short*>(L.job[job].out) + (((size_t)b * L.T + t0) * L.H + h) * outer;
+          auto copy = [&](auto word) {  // four rows' words under way at a time
+            typedef decltype(word) P;
+            constexpr int N = sizeof(P) / 2, LANES = 128 / N, PER = 256 / LANES;
+            const int o = (a & (LANES - 1)) * N;
+#pragma unroll 1
+            for (int r0 = a / LANES; r0 < rows; r0 += 4 * PER) {
+              P z[4];
+#pragma unroll
+              for (int j = 0; j < 4; ++j)
+                if (r0 + j * PER < rows && o < outer)
+                  z[j] = *reinterpret_cast<const P*>(mem + slot + (o >> 6) * TILE + sw128_offset(r0 + j * PER, o & 63));
+#pragma unroll
+              for (int j = 0; j < 4; ++j)
+                if (r0 + j * PER < rows && o < outer) *reinterpret_cast<P*>(out + (r0 + j * PER) * pitch + o) = z[j];
+            }
           };
+          // (odd widths by words, with the rows' two kinds of boundary told apart, took longer: forward of 8 x 2048 x 16 heads of 121
+          // 306 us, so 176)
           const uintptr_t boundary = reinterpret_cast<uintptr_t>(L.job[job].out) | (uintptr_t)outer * 2;
           if (boundary % 8 == 0) copy(uint2());
           else if (boundary % 4 == 0) copy(uint32_t());

@@ -478,14 +478,16 @@ def test_first_cuda_call_of_a_host_thread():
     assert got == [0, 0, 0] and torch.equal(out, want)
 
 
-def test_nothing_is_written_beyond_the_outputs():
-    """Exact-size outputs inside a larger block, by the C entry points: what surrounds them stays."""
+@pytest.mark.parametrize("pad", [64, 65, 66])
+def test_nothing_is_written_beyond_the_outputs(pad):
+    """Exact-size outputs inside a larger block, at any boundary, by the C entry points: what surrounds them stays."""
     L = _lib.lib()
-    for dtype, code, B, T, H, dk, dv in ((BF16, 1, 2, 131, 2, 24, 40), (FP32, 0, 1, 45, 3, 7, 9), (BF16, 1, 1, 140, 1, 13, 99)):
+    for dtype, code, B, T, H, dk, dv in ((BF16, 1, 2, 131, 2, 24, 40), (FP32, 0, 1, 45, 3, 7, 9), (BF16, 1, 1, 140, 1, 13, 99),
+                                       (BF16, 1, 1, 200, 3, 64, 128), (BF16, 1, 2, 131, 1, 128, 127), (FP16, 2, 1, 140, 3, 30, 61),
+                                       (BF16, 1, 4, 131, 17, 127, 128)):
         q, k, v, l, s, n, d_out, d_final = _inputs(dtype, B, T, H, dk, dv, seed=3)
         sd = lambda t: _lib.Strided(t.data_ptr(), *t.stride()[:3])  # noqa: E731
         p = _lib.LinearAttention(B, T, H, dk, dv, code, 0.2, sd(q), sd(k), sd(v), l.data_ptr(), None, s.data_ptr())
-        pad = 64
 
         def block(numel, dt):
             t = torch.full((numel + 2 * pad,), 77.0, device="cuda", dtype=dt)
