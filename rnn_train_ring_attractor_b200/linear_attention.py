@@ -164,10 +164,11 @@ def linear_attention(q, k, v, log_decay, scale=None, initial_state=None, lengths
     ``lengths`` [B] int32: sequences end after that many tokens (0 to T); outputs beyond are zero, and what q, k and v hold
     there has no influence.  A NaN or an infinity inside a sequence may reach up to 127 tokens before it.
 
-    Sums and states are fp32.  bfloat16 and float16 of widths up to 128 are multiplied on tensor cores: products of q and k, and the
-    state where it goes into outputs, are rounded to that type (float16: weighted products of q and k from 65520 on are infinite;
-    the state is scaled by a power of two first), what is added to the state keeps 22 bits or more.  Everything else is
-    multiplied to fp32's precision; an infinity among the inputs may come out as NaN.
+    Sums and states are fp32.  bfloat16 and float16 of widths up to 128 are multiplied on tensor cores (but for a few sequences
+    of up to 32 tokens): products of q and k, and the state where it goes into outputs, are rounded to that type (float16:
+    weighted products of q and k from 65520 on are infinite; the state is scaled by a power of two first), what is added to the
+    state keeps 22 bits or more.  Everything else is multiplied to fp32's precision; an infinity among the inputs may come out
+    as NaN.
     Gradients: q, k, v and initial_state, from those of out and final_state.
     """
     lead, dk, dv = _check_qkv(q, k, v, log_decay, 4, MAX_WIDTH)
