@@ -406,7 +406,7 @@ def test_step_of_many_narrow_states(B, H, dk, dv):
     assert (flat[:5] == 7.0).all() and (flat[5 + s.numel():] == 7.0).all()
 
 
-@pytest.mark.parametrize("T,H", [(300, 2), (4100, 1)])
+@pytest.mark.parametrize("T,H", [(20, 2), (300, 2), (4100, 1), (300, 60)])
 def test_two_streams_at_once(T, H):
     sets = [_inputs(BF16, 1, T, H, 64, 64, seed=i) for i in range(2)]
     want = [_run(*x[:4], 0.1, *x[4:]) for x in sets]
@@ -424,7 +424,7 @@ def test_two_streams_at_once(T, H):
                 assert torch.equal(a, b)
 
 
-@pytest.mark.parametrize("T,H", [(300, 2), (4100, 1)])
+@pytest.mark.parametrize("T,H", [(20, 2), (300, 2), (4100, 1), (300, 60)])
 def test_captured_and_replayed(T, H):
     q, k, v, l, s, n, d_out, d_final = _inputs(BF16, 1, T, H, 64, 64, seed=1, lengths=[T - 5])
     state = s.clone()
