@@ -10,7 +10,7 @@ from torch.autograd import Function
 from torch.autograd.function import once_differentiable
 
 from . import _lib
-from .linear_attention import DTYPES, raw_stream
+from .linear_attention import DTYPES, raw_stream, refuse_tangents
 from .ring_rnn_cuda import on_device
 
 
@@ -44,6 +44,7 @@ class DropoutFunc(Function):
     @staticmethod
     @once_differentiable
     def backward(ctx, d_y):
+        refuse_tangents("the gradient of dropout", d_y)
         p, seed, stream, first_row = ctx.args
         seed = ctx.saved_tensors[0] if seed is None else seed
         d_x = _call(d_y.contiguous(), None, p, seed, stream, first_row) if ctx.needs_input_grad[0] else None
@@ -57,7 +58,9 @@ def dropout(x, p, seed, stream=0, first_row=0, residual=None):
     ``seed``: an integer of 64 bits; ``stream`` (32 bits) tells apart what shares a seed, such as layers and steps.  Or ``seed`` is
     an int64 tensor [2] = (seed, stream) on the device, read when the kernel runs: a captured graph draws new numbers each time
     it is replayed if the tensor is advanced between.  ``first_row``: number of x's first row in the whole batch.  p = 1 drops
-    everything.  What is dropped has no influence, infinities and NaN included.  float32, bfloat16 or float16, contiguous."""
+    everything.  What is dropped has no influence, infinities and NaN included.  float32, bfloat16 or float16, contiguous.
+    Gradients: x and residual; forward-mode derivatives are refused."""
+    refuse_tangents("dropout", x, residual)
     if x.dtype not in DTYPES:
         raise RuntimeError("x must be float32, bfloat16 or float16")
     if x.dim() < 1:

@@ -9,7 +9,7 @@ train/train_causal_transformer.py).
 """
 import torch
 from torch._C import _cuda_getCurrentRawStream as raw_stream
-from torch.autograd import Function
+from torch.autograd import Function, forward_ad
 from torch.autograd.function import once_differentiable
 
 from . import _lib
@@ -28,6 +28,12 @@ def new(dev, dtype, a, b, c, d):
     c_step = d or 1
     b_step = (c or 1) * c_step
     return torch.empty_strided((a, b, c, d), ((b or 1) * b_step, b_step, c_step, 1), device=dev, dtype=dtype)
+
+
+def refuse_tangents(name, *tensors):
+    """The kernels compute no forward-mode derivatives, and an output without a tangent would count as a constant."""
+    if forward_ad._current_level >= 0 and any(t is not None and forward_ad.unpack_dual(t).tangent is not None for t in tensors):
+        raise RuntimeError(f"{name} has no forward-mode derivative (an argument carries a tangent)")
 
 
 def _check(name, t, shape, device, dtype):
@@ -124,6 +130,7 @@ class LinearAttentionFunc(Function):
     @staticmethod
     @once_differentiable
     def backward(ctx, d_out, d_final):
+        refuse_tangents("the gradient of linear_attention", d_out, d_final)
         q, k, v, initial_state, log_decay, lengths = ctx.saved_tensors
         if d_out is None and d_final is None:
             return (None,) * 7
@@ -169,8 +176,9 @@ def linear_attention(q, k, v, log_decay, scale=None, initial_state=None, lengths
     weighted products of q and k from 65520 on are infinite; the state is scaled by a power of two first), what is added to the
     state keeps 22 bits or more.  Everything else is multiplied to fp32's precision; an infinity among the inputs may come out
     as NaN.
-    Gradients: q, k, v and initial_state, from those of out and final_state.
+    Gradients: q, k, v and initial_state, from those of out and final_state.  Forward-mode derivatives are refused.
     """
+    refuse_tangents("linear_attention", q, k, v, log_decay, initial_state)
     lead, dk, dv = _check_qkv(q, k, v, log_decay, 4, MAX_WIDTH)
     B, _, H = lead
     dev = q.device
@@ -193,7 +201,8 @@ def linear_attention_step(q, k, v, state, log_decay, scale=None, active=None):
 
     ``q``, ``k`` [B,H,dk], ``v`` [B,H,dv], any strides; widths of keys up to 1024.  ``active`` [B] bool: sequences that are False
     keep their state and get an output of zero (the unused rows of a batch of fixed size).  For inference: refused for tensors
-    that require a gradient while gradients are recorded."""
+    that require a gradient while gradients are recorded, or carry a forward-mode tangent."""
+    refuse_tangents("linear_attention_step", q, k, v, state, log_decay)
     lead, dk, dv = _check_qkv(q, k, v, log_decay, 3, 1024)
     B, H = lead
     dev = q.device

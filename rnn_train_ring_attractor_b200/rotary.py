@@ -11,7 +11,7 @@ from torch.autograd import Function
 from torch.autograd.function import once_differentiable
 
 from . import _lib
-from .linear_attention import DTYPES, last_contiguous, new, raw_stream
+from .linear_attention import DTYPES, last_contiguous, new, raw_stream, refuse_tangents
 from .ring_rnn_cuda import on_device
 
 
@@ -78,6 +78,7 @@ class RotaryFunc(Function):
     @staticmethod
     @once_differentiable
     def backward(ctx, d_q, d_k):
+        refuse_tangents("the gradient of rotary", d_q, d_k)
         frequencies, positions = ctx.saved_tensors
         first, interleaved, amplitude = ctx.args
         got = [None, None]
@@ -98,7 +99,8 @@ def rotary(q, k, frequencies, positions=0, interleaved=False, amplitude=1.0):
     heads of their own; one launch for both.  ``frequencies`` [R/2] float64 (``rotary_frequencies``), R <= D.  ``positions``: the
     position of the first token, or an int32 / int64 tensor [B,T] (an expanded one will do) with each token's.  Pairs are
     elements (2i, 2i+1) if ``interleaved``, else (i, i + R/2).  ``amplitude`` multiplies the turned elements.  Angles are formed
-    in 64 bits, so that positions of millions are as exact as small ones.  Gradients: q and k."""
+    in 64 bits, so that positions of millions are as exact as small ones.  Gradients: q and k; forward-mode derivatives are refused."""
+    refuse_tangents("rotary", q, k, frequencies)
     if q.dtype not in DTYPES:
         raise RuntimeError("q must be float32, bfloat16 or float16")
     dev = q.device
