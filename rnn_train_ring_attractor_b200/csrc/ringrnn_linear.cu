@@ -264,9 +264,9 @@ __global__ void __launch_bounds__(P_THREADS, NC <= 4 ? 2 : 1) la_plain_kernel(co
     }
   }
   if (!STATES) {  // rows behind the sequence
-    const int first = max(begin, end), rows = stop - first;
-    for (int e = tid; e < rows * PO; e += P_THREADS)
-      if (e % PO < on) out[(((size_t)b * L.T + first + e / PO) * L.H + h) * J.outer + o0 + e % PO] = down<E>(0.f);
+    // (by rows: rows times columns may not fit 31 bits)
+    for (int r = max(begin, end) + tid / PO; r < stop; r += P_THREADS / PO)
+      if (tid % PO < on) out[(((size_t)b * L.T + r) * L.H + h) * J.outer + o0 + tid % PO] = down<E>(0.f);
   }
   if (J.fin != nullptr)
 #pragma unroll
