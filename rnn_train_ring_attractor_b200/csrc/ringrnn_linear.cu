@@ -12,8 +12,8 @@ namespace {
 // fewest products per token next to the state's own 2 * inner * 64 that still leave several CTAs per SM their shared memory).
 //
 // Products on the tensor cores' tf32 type, exact to fp32's own rounding: x = hi + lo with hi rounded to tf32's eleven bits, and
-// what is left fits eleven bits again, so x y = hi hi + hi lo + lo hi but for lo lo, at most 2^-24 of it.  (Infinities become
-// NaN on the way.)  The same products on the CUDA cores were bound by the operands' way through shared memory, four cycles for
+// what is left fits eleven bits again, so x y = hi hi + hi lo + lo hi but for lo lo, at most 2^-24 of it.  (Infinities
+// may become NaN on the way.)  The same products on the CUDA cores were bound by the operands' way through shared memory, four cycles for
 // each 16 bytes a thread reads; a fragment's element is read once per product of 16 x 8 x 8.  Measured in fp32, 16 x 512 x 16 heads
 // of 64, on CUDA cores and now: forward 183 and 119 us, backward 532 and 340 (the memory alone 21 and 36 us: what bounds it is
 // three products for one, on mma.sync, and their fragments' way from shared memory).
@@ -30,7 +30,8 @@ size_t plain_smem(int inner) {
 struct Split {
   uint32_t hi, lo;
   __device__ __forceinline__ explicit Split(float x) {
-    hi = (__float_as_uint(x) + 0x1000u) & 0xffffe000u;
+    // (to the largest number of eleven bits at most: plain rounding makes infinities of what lies above it, and NaN of those)
+    asm("cvt.rn.satfinite.tf32.f32 %0, %1;" : "=r"(hi) : "f"(x));
     lo = __float_as_uint(x - __uint_as_float(hi));
   }
 };
