@@ -11,12 +11,14 @@ namespace {
 // One CTA per (job, sequence, head, segment) and slice of 64 outer columns, chunks of 32 tokens (of 16, 32 and 64, 32 has the
 // fewest products per token next to the state's own 2 * inner * 64 that still leave several CTAs per SM their shared memory).
 //
-// Products on the tensor cores' tf32 type, exact to fp32's own rounding: x = hi + lo with hi rounded to tf32's eleven bits, and
-// what is left fits eleven bits again, so x y = hi hi + hi lo + lo hi but for lo lo, at most 2^-24 of it.  (Infinities
-// may become NaN on the way.)  The same products on the CUDA cores were bound by the operands' way through shared memory, four cycles for
-// each 16 bytes a thread reads; a fragment's element is read once per product of 16 x 8 x 8.  Measured in fp32, 16 x 512 x 16 heads
-// of 64, on CUDA cores and now: forward 183 and 119 us, backward 532 and 340 (the memory alone 21 and 36 us: what bounds it is
-// three products for one, on mma.sync, and their fragments' way from shared memory).
+// Products on the tensor cores' tf32 type: x = hi + lo with hi rounded to tf32's eleven bits; what is left, of up to twelve bits, goes
+// in as it is, and the tensor cores take eleven of them, so a factor is off by a unit of fp32's last place at most (2^-23).
+// x y = hi hi + hi lo + lo hi but for lo lo, at most 2^-22 of it: together 2^-21 of a product, where fp32 rounds to 2^-24 (a state of one
+// product, with its sums: 8.8 * 2^-24 measured); over a long sum, with either sign, 3e-7 of it where plain fp32 leaves 2e-7.
+// (Infinities may become NaN on the way.)  The same products on the CUDA cores were bound by the operands' way through shared
+// memory, four cycles for each 16 bytes a thread reads; a fragment's element is read once per product of 16 x 8 x 8.  Measured in
+// fp32, 16 x 512 x 16 heads of 64, on CUDA cores and so: forward 183 and 119 us, backward 532 and 340 (the memory alone 21 and
+// 36 us: what bounds it is three products for one, on mma.sync, and their fragments' way from shared memory).
 // The state stays in registers as an accumulator and is copied to shared memory once a chunk, where the outputs read it.  A chunk's
 // numbers are loaded into registers while the one before is at work (widths up to 128).
 constexpr int PC = 32, PO = 64, P_THREADS = 256, P_WARPS = P_THREADS / 32;

@@ -1,4 +1,4 @@
-"""The fp32 kernel at the largest numbers of the type."""
+"""The fp32 kernel's products by themselves, and the largest numbers of the type."""
 import pytest
 import torch
 
@@ -8,11 +8,30 @@ from rnn_train_ring_attractor_b200.linear_attention import linear_attention
 pytestmark = pytest.mark.gpu
 
 FP32 = torch.float32
+# A factor is taken as two numbers of eleven bits and is off by one unit of its last place at most (2^-23), and the product of the two
+# second numbers (2^-12 of a factor each, and a little) is left out: 2 * 2^-23 + 2^-22 of a product, and parts in 2^-11 of that.
+PRODUCT = 2.0 ** -21 * (1 + 2.0 ** -10)
 
 
 def _full(*shape, seed, lo=1.0, hi=2.0):
     g = torch.Generator(device="cuda").manual_seed(seed)
     return torch.rand(*shape, device="cuda", generator=g) * (hi - lo) + lo
+
+
+@pytest.mark.parametrize("lo,hi", [(1.0, 1.01), (1.0, 2.0), (-2.0, 2.0)])
+def test_one_product(lo, hi, achieved):
+    """One token of heads of one element: no sum that a product's error could hide in."""
+    B, H = 4096, 64
+    q, k, v = (_full(B, 1, H, 1, seed=s, lo=lo, hi=hi) for s in (1, 2, 3))
+    l = torch.full((H,), -0.1, device="cuda")
+    out, final = linear_attention(q, k, v, l, scale=1.0)
+    want = q.double() * k.double() * v.double()
+    want_s = (k.double() * v.double())[:, 0, :, :, None]
+    e, es = float(((out.double() - want) / want).abs().max()), float(((final.double() - want_s) / want_s).abs().max())
+    achieved(f"one fp32 product of {lo:g} to {hi:g}, in 2^-24", out=e * 2 ** 24, state=es * 2 ** 24)
+    # sums of two parts, of zero and the product, the scale and the power: a rounding or a cut of 2^-23 each
+    assert es <= PRODUCT + 4 * 2.0 ** -23
+    assert e <= 2 * PRODUCT + 10 * 2.0 ** -23
 
 
 @pytest.mark.parametrize("top", [torch.finfo(FP32).max, torch.finfo(FP32).min, 3.4e38, -(2.0 ** 128 - 2.0 ** 116)])
