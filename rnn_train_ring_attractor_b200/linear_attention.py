@@ -169,7 +169,8 @@ def linear_attention(q, k, v, log_decay, scale=None, initial_state=None, lengths
     shrinks each step (``log(1 - alpha)`` for a leak of alpha); it has no gradient.  ``scale`` defaults to ``dk ** -0.5``.
     ``initial_state`` [B,H,dk,dv] fp32, or None for zero: pass the final state of one call to continue with the next.
     ``lengths`` [B] int32: sequences end after that many tokens (0 to T); outputs beyond are zero, and what q, k and v hold
-    there has no influence.  A NaN or an infinity inside a sequence may reach up to 127 tokens before it.
+    there has no influence.  A NaN or an infinity inside a sequence reaches, beside what follows it, up to 127 tokens before it
+    (31 where the arithmetic is fp32), and in the gradients of k and v as many behind it; no other sequence or head.
 
     Sums and states are fp32.  bfloat16 and float16 of widths up to 128 are multiplied on tensor cores (but for a few sequences
     of up to 32 tokens): products of q and k, and the state where it goes into outputs, are rounded to that type (float16:
