@@ -314,10 +314,10 @@ typedef struct RingRnnStrided {
  *     inputs there have no influence, whatever they hold
  *   initial_state, final_state [B,H,dk,dv] fp32 contiguous, NULL = zero / not wanted
  * Sums and states are held in fp32.  bf16 and fp16 tensors of widths up to 128 (but for a few sequences of up to 32 tokens) run
- * on tensor cores: weighted scores q.k, and the state where it goes into outputs, are rounded to their type (fp16: scores from
- * 65520 on are infinite; the state is scaled by a power of two first); what is added to a state keeps 22 bits or more, sixteen
- * inside a gradient.  All else is multiplied in fp32, products to 2^-21 of themselves or better; an infinity among the inputs
- * may come out as NaN. */
+ * on tensor cores: weighted scores q.k, and the state where it goes into outputs, are rounded to their type (fp16: multiplied
+ * by a power of two of each 128 tokens first); what is added to a state keeps 22 bits or more (fp16: or 2^-38 of the largest of 128
+ * tokens; bf16: sixteen inside a gradient).  All else is multiplied in fp32, products to 2^-21 of themselves or better; an
+ * infinity among the inputs may come out as NaN. */
 typedef struct RingRnnLinearAttention {
   int B, T, H, dk, dv;
   int dtype; /* RINGRNN_F32 ... */

@@ -15,8 +15,12 @@
 // of a chunk's cycles).  A state that a caller sees, or that sums of segments make, is good for what fp32 is for: there a third part of
 // K' follows, so that all 24 bits of the product count.  Measured against 64 bits: 6e-7 of the state's size instead of 3.8e-6,
 // for 65 us instead of 58 (forward of 8 x 2048 x 16 heads of 128; nothing at widths of 64 or where segments are summed).
-// fp16 has three bits more and little range: the state is multiplied by the power of two that brings its largest element just
-// below 2^15 before it is rounded, and inter divided by it again.  Scores have no such power: weighted ones from 65520 on are infinite.
+// fp16 has three bits more and little range: what is rounded to it is multiplied by a power of two first that brings a chunk's largest
+// number just below 2^15, and its product divided by it again.  The state's largest element; that of the keys times their weights, by
+// way of fp32 (hi and lo keep 22 bits, and what is 2^-17 of the largest or less a share of 2^-39 of it); for scores their bound, the width
+// times the largest elements of rows and keys.  Two passes over the operands in shared memory find those.  Forward and gradients of
+// 8 x 2048 x 16 heads of 128: 64 and 160 us, without the powers of keys and scores 58 and 143, but small numbers lost their bits (keys
+// of 1e-3: state off by 5e-5; gradients of 1e-5: by 2e-2) and scores from 65520 on were infinite.
 //
 // What bounds it: at widths of 128 the memory's share (a chunk is 128 KB, 5500 cycles of an SM's share at 6.5 TB/s when all SMs
 // read), then shared memory's 128 bytes per cycle, which products with both operands there use up.  P and K' therefore live in tensor
@@ -63,8 +67,10 @@ struct LtCfg {
   static constexpr int TABLES = BARS + (2 * SLOTS + 15) * 8 + 8;  // 32 powers; key weights of 64 pairs of tokens, twice
   static_assert(TABLES % 16 == 0, "alignment");
   static constexpr int FLAGS = TABLES + 128 + 512 + 512;
-  static constexpr int RANGE = FLAGS + 16;  // fp16: the state's largest element by warp; what it was divided by, of two chunks
-  static constexpr int SMEM = RANGE + 48;
+  // fp16: the state's largest element by warp, and what it was divided by, of two chunks; the same of keys and rows (three by warp, in
+  // turn at two places); what weighted keys were multiplied by, inverse, of four chunks; and scores, of two chunks' two steps
+  static constexpr int RANGE = FLAGS + 16, TOPS = RANGE + 48, KEY_DOWN = TOPS + 256, SCORE_UP = KEY_DOWN + 16;
+  static constexpr int SMEM = SCORE_UP + 16;
   static_assert(SMEM <= 232448, "shared memory of a block");
 };
 
@@ -123,6 +129,16 @@ __device__ __forceinline__ uint32_t pack2(f32x2 v) {
   float a, b;
   upk2(v, a, b);
   return pack2<E>(a, b);
+}
+__device__ __forceinline__ f32x2 wide_half(uint32_t pair) {
+  const float2 x = __half22float2(*reinterpret_cast<const __half2*>(&pair));
+  return pk2(x.x, x.y);
+}
+// The power of two, of at most 2^most, that brings a number below 2^15 but not below 2^14; one for zero.
+__device__ __forceinline__ float below_2_15(float top, int most) {
+  int up = __float_as_uint(top) < 0x800000u ? 0 : 127 + 14 - (int)(__float_as_uint(top) >> 23);
+  up = up > most ? most : up < -100 ? -100 : up;
+  return __uint_as_float((uint32_t)(127 + up) << 23);
 }
 // 32 bytes: a whole sector of each lane's own row
 __device__ __forceinline__ void ldg8(const float* p, float* x) {
@@ -399,7 +415,35 @@ __device__ __forceinline__ void la_tc_block(const LtParams& A, const int ji, con
       const int far = rev ? col + s - lane : lane - col - s, far1 = rev ? far + 1 : far - 1;
       diagonal[s / 2] = pk2(far >= 0 ? J.pair_scale * g.power(far) : 0.f, far1 >= 0 ? J.pair_scale * g.power(far1) : 0.f);
     }
-    int have = 0;
+    int have = 0, turn = 0;
+    // fp16: the largest element of this thread's half of row r (an infinity has no part in what the others are scaled by)
+    auto row_top = [&](int tile, int width, int n) {
+      mbar_wait(full(tile % NS), (tile / NS) & 1, w, 124);
+      const uint32_t from = base + (tile % NS) * Cfg::SLOT;
+      __half2 top = __float2half2_rn(0.f);
+      if (r < n)
+#pragma unroll 4
+        for (int i = half; i < width / 8; i += 2) {
+          uint32_t x[4];
+          lds128(from + (i >> 3) * TILE + sw128_offset(r, (i & 7) * 8), x);
+#pragma unroll
+          for (int e = 0; e < 4; ++e) top = __hmax2(top, __habs2(*reinterpret_cast<const __half2*>(x + e)));
+        }
+      const float x = __half2float(__hmax(__low2half(top), __high2half(top)));
+      return x < 65536.f ? x : 0.f;
+    };
+    // the largest of all threads' numbers (not negative: their order is that of their bits)
+    auto largest = [&](float x, float y, float z) {
+      uint4* const tops = reinterpret_cast<uint4*>(mem + Cfg::TOPS) + turn;
+      turn ^= 8;
+      auto top = [](uint32_t bits) { return __reduce_max_sync(0xffffffffu, bits); };
+      const uint4 mine = make_uint4(top(__float_as_uint(x)), top(__float_as_uint(y)), top(__float_as_uint(z)), 0u);
+      if (lane == 0) tops[warp - 4] = mine;
+      named_bar_sync(1, 256);
+      const uint4 all = tops[lane & 7];
+      return make_float3(__uint_as_float(top(all.x)), __uint_as_float(top(all.y)), __uint_as_float(top(all.z)));
+    };
+    const float grows = fmaxf(1.f, g.power(C - 1));
 #pragma unroll 1
     for (int c = 0; c < chunks; ++c) {
       const int t0 = chunk_at(c), n = min(C, end - t0), kt = TILES * c + KEYS, vt = TILES * c + VALUES;
@@ -427,11 +471,19 @@ __device__ __forceinline__ void la_tc_block(const LtParams& A, const int ji, con
             x[e] = s < n ? J.key_scale * g.power(steps) : 0.f;
             left[e] = x[e] - Pair<E>::kept(x[e]);
           }
-          key_weights[a] = make_uint2(pack2<E>(x[0], x[1]), pack2<E>(left[0], left[1]));
+          if (!HALF) key_weights[a] = make_uint2(pack2<E>(x[0], x[1]), pack2<E>(left[0], left[1]));
           key_weights32[2 * a] = x[0], key_weights32[2 * a + 1] = x[1];
         }
         named_bar_sync(1, 256);
         have = n;
+      }
+      float keys_up = 1.f, keys_top = 0.f, rows_top = 0.f;
+      if constexpr (HALF) {  // each thread has read its row's weight: the weights may be of the chunk before, and are the same then
+        const float top = row_top(kt, DI, n);
+        const float3 all = largest(top * fabsf(key_weights32[r]), top, STATES ? 0.f : row_top(TILES * c + ROWS, DI, n));
+        keys_up = below_2_15(all.x, 100);
+        keys_top = all.y, rows_top = all.z;
+        if (a == 0) reinterpret_cast<float*>(mem + Cfg::KEY_DOWN)[c & 3] = 1.f / keys_up;
       }
       // what read the last keys: the chunk before's delta; forming sums, of two chunks before
       if (STATES ? c > 1 : c > 0) {
@@ -450,8 +502,16 @@ __device__ __forceinline__ void la_tc_block(const LtParams& A, const int ji, con
 #pragma unroll 1
         for (int j = 0; j < 2; ++j) {  // 32 tokens
           uint2 wt[4];
+          f32x2 wt32[4];
 #pragma unroll
-          for (int e = 0; e < 4; ++e) wt[e] = kw[(j * 4 + e) * 4];
+          for (int e = 0; e < 4; ++e) {
+            if (HALF) {
+              const float2 x = *reinterpret_cast<const float2*>(key_weights32 + 2 * (half * 32 + (lane & 3) + (j * 4 + e) * 4));
+              wt32[e] = mul2(pk2(x.x, x.y), pk2(keys_up, keys_up));
+            } else {
+              wt[e] = kw[(j * 4 + e) * 4];
+            }
+          }
 #pragma unroll
           for (int i = 0; i < 2; ++i) {  // 16 columns
             uint32_t hi[8], lo[8], left[8];
@@ -459,6 +519,13 @@ __device__ __forceinline__ void la_tc_block(const LtParams& A, const int ji, con
             ldmatrix_x4_trans(from + sw128_offset(row + j * 32 + 16, in + i * 16), lo + 4);
 #pragma unroll
             for (int e = 0; e < 8; ++e) {
+              if constexpr (HALF) {
+                // the type's small numbers have few bits, so by way of fp32, with the chunk's largest product just below 2^15
+                const f32x2 p = mul2(wide_half(lo[e]), wt32[e >> 1]);
+                hi[e] = pack2<E>(p);
+                lo[e] = pack2<E>(fma2(wide_half(hi[e]), pk2(-1.f, -1.f), p));
+                continue;
+              }
               const E2 wh = *reinterpret_cast<const E2*>(&wt[e >> 1].x), wl = *reinterpret_cast<const E2*>(&wt[e >> 1].y),
                        z = *reinterpret_cast<const E2*>(lo + e), h2 = __hmul2_rn(z, wh), l2 = __hfma2(z, wl, __hfma2(z, wh, __hneg2(h2)));
               if (STATES && !HALF) {
@@ -501,6 +568,16 @@ __device__ __forceinline__ void la_tc_block(const LtParams& A, const int ji, con
       mbar_arrive(STATES ? sum_keys_ready(c) : keys_ready);
 #pragma unroll 1
       for (int step = 0; step < (STATES ? 0 : STEPS); ++step) {
+        float up = 1.f;
+        if constexpr (HALF) {
+          // Scores are brought below 2^15 by what bounds them: the width times the largest elements of rows and keys.
+          if (step > 0) {
+            const float3 all = largest(0.f, row_top(vt, DO, n), row_top(TILES * c + 3, DO, n));
+            keys_top = all.y, rows_top = all.z;
+          }
+          up = below_2_15((step > 0 ? J.outer : J.inner) * rows_top * keys_top * fabsf(J.pair_scale) * grows, 64);
+          if (a == 0) reinterpret_cast<float*>(mem + Cfg::SCORE_UP)[(c & 1) * 2 + step] = up;
+        }
         mbar_wait(scores_ready, (c * STEPS + step) & 1, w, 122);
         tcgen05_fence_after();
         const uint32_t mine = tm + TM_SCORES + ((uint32_t)(q * 32) << 16) + col;
@@ -515,9 +592,12 @@ __device__ __forceinline__ void la_tc_block(const LtParams& A, const int ji, con
         tmem_ld16(mine + q * 32, x);
         tmem_ld_wait();
 #pragma unroll
-        for (int s = 0; s < 8; ++s) y[s] = mul2(pk2u(x[2 * s], x[2 * s + 1]), diagonal[s]);
+        for (int s = 0; s < 8; ++s) {
+          y[s] = mul2(pk2u(x[2 * s], x[2 * s + 1]), diagonal[s]);
+          if (HALF) y[s] = mul2(y[s], pk2(up, up));
+        }
         put(q);
-        float f = near;
+        float f = HALF ? near * up : near;
 #pragma unroll 1
         for (int j = rev ? q + 1 : q - 1; rev ? j < 4 : j >= 0; j += rev ? 1 : -1) {
           tmem_ld16(mine + j * 32, x);
@@ -561,8 +641,14 @@ __device__ __forceinline__ void la_tc_block(const LtParams& A, const int ji, con
         float f = r < n ? J.row_scale * g.power(rev ? n - 1 - r : r + 1) : 0.f;
         mbar_wait(inter_done, u & 1, w, 130);
         tcgen05_fence_after();
-        if (HALF) f *= reinterpret_cast<const volatile float*>(mem + Cfg::RANGE)[8 + (c & 1)];
-        const f32x2 f2 = pk2(f, f);
+        float down = 1.f;
+        if (HALF) {
+          mbar_wait(pairs_ready, u & 1, w, 133);  // (what the scores were multiplied by is known then)
+          const float up = reinterpret_cast<const volatile float*>(mem + Cfg::SCORE_UP)[(c & 1) * 2 + u % STEPS];
+          f *= reinterpret_cast<const volatile float*>(mem + Cfg::RANGE)[8 + (c & 1)] * up;
+          down = 1.f / up;
+        }
+        const f32x2 f2 = pk2(f, f), down2 = pk2(down, down);
 #pragma unroll 1
         for (int i = 0; i < N; i += 16) {
           uint32_t x[16];
@@ -594,7 +680,10 @@ __device__ __forceinline__ void la_tc_block(const LtParams& A, const int ji, con
           }
           uint32_t y[8];
 #pragma unroll
-          for (int e = 0; e < 8; ++e) y[e] = r < n ? pack2<E>(__uint_as_float(x[2 * e]), __uint_as_float(x[2 * e + 1])) : 0u;
+          for (int e = 0; e < 8; ++e) {
+            const f32x2 z = pk2u(x[2 * e], x[2 * e + 1]);
+            y[e] = r < n ? pack2<E>(HALF ? mul2(z, down2) : z) : 0u;
+          }
           sts128(to + sw128_offset(r, (o0 & 63) + i), y[0], y[1], y[2], y[3]);
           sts128(to + sw128_offset(r, (o0 & 63) + i + 8), y[4], y[5], y[6], y[7]);
         }
@@ -675,13 +764,14 @@ __device__ __forceinline__ void la_tc_block(const LtParams& A, const int ji, con
         mbar_wait(sum_done(c), (c >> 1) & 1, w, 140);
         tcgen05_fence_after();
         const uint32_t from = mine - TM_DELTA + TM_SUM_DELTA;
+        const float times = HALF ? reinterpret_cast<const volatile float*>(mem + Cfg::KEY_DOWN)[c & 3] : 1.f;
 #pragma unroll
         for (int i = 0; i < N; i += 16) {
           uint32_t x[16];
           tmem_ld16(from + i, x);
           tmem_ld_wait();
 #pragma unroll
-          for (int e = 0; e < 8; ++e) S[i / 2 + e] = fma2(pk2(1.f, 1.f), S[i / 2 + e], pk2u(x[2 * e], x[2 * e + 1]));
+          for (int e = 0; e < 8; ++e) S[i / 2 + e] = fma2(pk2(times, times), pk2u(x[2 * e], x[2 * e + 1]), S[i / 2 + e]);
         }
         tcgen05_fence_before();
         mbar_arrive(state_ready);
@@ -696,13 +786,18 @@ __device__ __forceinline__ void la_tc_block(const LtParams& A, const int ji, con
           const f32x2 g_hi = all ? pk2(whole.hi, whole.hi) : pk2(rest.hi, rest.hi), g_lo = all ? pk2(whole.lo, whole.lo) : pk2(rest.lo, rest.lo);
           mbar_wait(delta_ready, (c - 1) & 1, w, 141);
           tcgen05_fence_after();
+          const float times = HALF ? reinterpret_cast<const volatile float*>(mem + Cfg::KEY_DOWN)[(c - 1) & 3] : 1.f;
 #pragma unroll
           for (int i = 0; i < N; i += 16) {
             uint32_t y[16];
             tmem_ld16(mine + i, y);
             tmem_ld_wait();
 #pragma unroll
-            for (int e = 0; e < 8; ++e) S[i / 2 + e] = fma2(g_hi, S[i / 2 + e], fma2(g_lo, S[i / 2 + e], pk2u(y[2 * e], y[2 * e + 1])));
+            for (int e = 0; e < 8; ++e) {
+              f32x2 delta = pk2u(y[2 * e], y[2 * e + 1]);
+              if (HALF) delta = mul2(delta, pk2(times, times));
+              S[i / 2 + e] = fma2(g_hi, S[i / 2 + e], fma2(g_lo, S[i / 2 + e], delta));
+            }
           }
         }
         if (c < chunks) {  // the next operand (delta of this chunk is behind inter, which has read the last one)

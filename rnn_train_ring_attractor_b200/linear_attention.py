@@ -174,8 +174,8 @@ def linear_attention(q, k, v, log_decay, scale=None, initial_state=None, lengths
 
     Sums and states are fp32.  bfloat16 and float16 of widths up to 128 are multiplied on tensor cores (but for a few sequences
     of up to 32 tokens): products of q and k, and the state where it goes into outputs, are rounded to that type (float16:
-    weighted products of q and k from 65520 on are infinite; the state is scaled by a power of two first), what is added to the
-    state keeps 22 bits or more.  Everything else is multiplied in fp32, products to 2^-21 of themselves or better; an infinity
+    multiplied by a power of two of each 128 tokens first), what is added to the state keeps 22 bits or more (float16: or 2^-38
+    of the largest of 128 tokens).  Everything else is multiplied in fp32, products to 2^-21 of themselves or better; an infinity
     among the inputs may come out as NaN.
     Gradients: q, k, v and initial_state, from those of out and final_state.  Forward-mode derivatives are refused.
     """
