@@ -5,6 +5,8 @@ row draws the same numbers in whatever batch it stands, so data-parallel ranks t
 the whole batch would, and the backward pass recomputes the mask instead of reading it.  The reference's comparison models use
 torch's dropout (train/train_causal_transformer.py), which stores a mask.
 """
+import operator
+
 import torch
 from torch.autograd import Function
 from torch.autograd.function import once_differentiable
@@ -83,11 +85,11 @@ def dropout(x, p, seed, stream=0, first_row=0, residual=None):
         if stream != 0:
             raise ValueError("stream is the second number of a seed tensor")
     else:
-        seed = int(seed)
+        seed = operator.index(seed)
         if not -(1 << 63) <= seed < 1 << 64:
             raise ValueError("seed must fit 64 bits")
         seed &= (1 << 64) - 1
-    stream, first_row = int(stream), int(first_row)
+    stream, first_row = operator.index(stream), operator.index(first_row)
     if not 0 <= stream < 1 << 32 or not 0 <= first_row < 1 << 63:
         raise ValueError("stream must fit 32 bits, first_row 63, and neither may be negative")
     if torch.is_grad_enabled() and (x.requires_grad or (residual is not None and residual.requires_grad)):

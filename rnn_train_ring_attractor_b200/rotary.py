@@ -5,6 +5,7 @@ head turns by a fixed angle each step beside its decay, as the ring network's bu
 (train/train_general_ring_no_gain.py:102-137).  The reference has no counterpart.
 """
 import math
+import operator
 
 import torch
 from torch.autograd import Function
@@ -122,7 +123,12 @@ def rotary(q, k, frequencies, positions=0, interleaved=False, amplitude=1.0):
         if positions.dtype not in (torch.int32, torch.int64) or positions.shape != q.shape[:2] or positions.device != dev:
             raise RuntimeError("positions must be an integer, or int32 / int64 [batch, tokens] on q's device")
     else:
-        first, positions = int(positions), None
+        try:
+            first, positions = operator.index(positions), None
+        except TypeError:
+            raise RuntimeError("positions must be an integer, or int32 / int64 [batch, tokens] on q's device") from None
+        if not -(1 << 63) <= first < 1 << 63:
+            raise ValueError("positions must fit 64 bits")
     if k is not None and k.shape[2] == 0:
         raise RuntimeError("k must have a head (None: q alone)")
     if q.shape[2] == 0:
