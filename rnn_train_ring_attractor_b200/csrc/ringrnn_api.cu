@@ -132,7 +132,12 @@ int host_status_word(volatile int** out) {
   std::lock_guard<std::mutex> lk(g_status_mu);
   if (g_status_direct == nullptr) {
     void* h = nullptr;
-    RINGRNN_CUDA_TRY(cudaHostAlloc(&h, sizeof(int), cudaHostAllocPortable | cudaHostAllocMapped));
+    // (the call that comes first may be one that is captured: this allocation has no part in its graph)
+    cudaStreamCaptureMode mode = cudaStreamCaptureModeRelaxed;
+    RINGRNN_CUDA_TRY(cudaThreadExchangeStreamCaptureMode(&mode));
+    const cudaError_t rc = cudaHostAlloc(&h, sizeof(int), cudaHostAllocPortable | cudaHostAllocMapped);
+    RINGRNN_CUDA_TRY(cudaThreadExchangeStreamCaptureMode(&mode));
+    RINGRNN_CUDA_TRY(rc);
     *static_cast<volatile int*>(h) = 0;
     g_status_direct = static_cast<volatile int*>(h);
   }
