@@ -309,15 +309,15 @@ typedef struct RingRnnStrided {
  *   S_t = g * S_{t-1} + k_t v_t^T        out_t = scale * S_t^T q_t        t = 0 .. length-1, S_{-1} = initial_state (or zero)
  * the linear form of the leaky recurrence above: a state that shrinks by a fixed factor each step, is added to, and read out.
  *   q, k [B,T,H,dk], v [B,T,H,dv] of type `dtype`;  1 <= dk, dv <= 256
- *   log_decay [H] fp32 device, <= 0 (-infinity: nothing is kept)
+ *   log_decay [H] fp32 device, <= 0 (-infinity: nothing is kept; above zero: not checked, not supported)
  *   lengths [B] int32 device, NULL = T each; values are clamped to 0..T.  out beyond a sequence's length is zero, and the
  *     inputs there have no influence, whatever they hold
  *   initial_state, final_state [B,H,dk,dv] fp32 contiguous, NULL = zero / not wanted
- * Sums and states are held in fp32.  bf16 and fp16 tensors of widths up to 128 (but for a few sequences of up to 32 tokens) run
- * on tensor cores: weighted scores q.k, and the state where it goes into outputs, are rounded to their type (fp16: multiplied
- * by a power of two of each 128 tokens first); what is added to a state keeps 22 bits or more (fp16: or 2^-38 of the largest of 128
- * tokens; bf16: sixteen inside a gradient).  All else is multiplied in fp32, products to 2^-21 of themselves or better; an
- * infinity among the inputs may come out as NaN. */
+ * Sums and states are held in fp32.  bf16 and fp16 tensors of widths up to 128 (but for batches of few sequences of up to 32
+ * tokens, which are faster in fp32) run on tensor cores: weighted scores q.k, and the state where it goes into outputs, are
+ * rounded to their type (fp16: multiplied by a power of two of each 128 tokens first); what is added to a state keeps 22 bits or
+ * more (fp16: or 2^-38 of the largest of 128 tokens; bf16: sixteen inside a gradient).  All else is multiplied in fp32, products to
+ * 2^-21 of themselves or better; an infinity among the inputs may come out as NaN. */
 typedef struct RingRnnLinearAttention {
   int B, T, H, dk, dv;
   int dtype; /* RINGRNN_F32 ... */

@@ -592,8 +592,9 @@ Plan make_plan(const RingRnnLinearAttention& p, const RingRnnStrided* d_out) {
   Plan l;
   memset(&l, 0, sizeof(l));
   const bool backward = d_out != nullptr;
-  // A few sequences of one chunk of the fp32 kernel are as fast there (5 x 15 x 20 heads of 95 and 64, forward: 17 us and 28; many are
-  // not: 64 x 32 x 24 heads of 128: 214 and 116), and where an output is a product or two, P's rounding is not averaged away.
+  // A few sequences of one chunk of the fp32 kernel are faster there (5 x 15 x 20 heads of 95 and 64, forward: 17 us and 28; many are
+  // not: 64 x 32 x 24 heads of 128: 214 and 116) and more exact, for P and the state are not rounded.  The rule goes by time alone, so
+  // a short sequence has other last bits, of the types' own size, in a large batch than in a small one.
   const int widest = p.dk > p.dv && backward ? p.dk : p.dv;
   const bool one_round = p.T <= PC && (long long)p.B * p.H * (backward ? 3 : 1) * ((widest + PO - 1) / PO) <= 2 * LA_TC_BLOCKS;
   l.tensor_cores = p.dtype != RINGRNN_F32 && p.dk <= LA_TC_WIDTH && p.dv <= LA_TC_WIDTH && !one_round;

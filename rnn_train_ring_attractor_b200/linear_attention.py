@@ -165,18 +165,20 @@ def linear_attention(q, k, v, log_decay, scale=None, initial_state=None, lengths
     """(out [B,T,H,dv] in q's type, final_state [B,H,dk,dv] fp32) of whole sequences.
 
     ``q``, ``k`` [B,T,H,dk], ``v`` [B,T,H,dv]: float32, bfloat16 or float16, widths up to 256; any strides (heads that share a
-    tensor may be given with ``expand``).  ``log_decay`` [H] fp32, <= 0: the logarithm of the factor by which a head's state
-    shrinks each step (``log(1 - alpha)`` for a leak of alpha); it has no gradient.  ``scale`` defaults to ``dk ** -0.5``.
+    tensor may be given with ``expand``).  ``log_decay`` [H] fp32, <= 0 (what is above is not checked
+    and not supported): the logarithm of the factor by which a head's state shrinks each step (``log(1 - alpha)`` for a leak of
+    alpha); it has no gradient.  ``scale`` defaults to ``dk ** -0.5``.
     ``initial_state`` [B,H,dk,dv] fp32, or None for zero: pass the final state of one call to continue with the next.
     ``lengths`` [B] int32: sequences end after that many tokens (0 to T); outputs beyond are zero, and what q, k and v hold
     there has no influence.  A NaN or an infinity inside a sequence reaches, beside what follows it, up to 127 tokens before it
     (31 where the arithmetic is fp32), and in the gradients of k and v as many behind it; no other sequence or head.
 
-    Sums and states are fp32.  bfloat16 and float16 of widths up to 128 are multiplied on tensor cores (but for a few sequences
-    of up to 32 tokens): products of q and k, and the state where it goes into outputs, are rounded to that type (float16:
-    multiplied by a power of two of each 128 tokens first), what is added to the state keeps 22 bits or more (float16: or 2^-38
-    of the largest of 128 tokens).  Everything else is multiplied in fp32, products to 2^-21 of themselves or better; an infinity
-    among the inputs may come out as NaN.
+    Sums and states are fp32.  bfloat16 and float16 of widths up to 128 are multiplied on tensor cores (but for batches of few
+    sequences of up to 32 tokens, which are faster in fp32; the same sequence may so have other last bits in a larger batch):
+    products of q and k, and the state where it goes into outputs, are rounded to that type (float16: multiplied by a power of
+    two of each 128 tokens first), what is added to the state keeps 22 bits or more (float16: or 2^-38 of the largest of 128
+    tokens).  Everything else is multiplied in fp32, products to 2^-21 of themselves or better; an infinity among the inputs may
+    come out as NaN.
     Gradients: q, k, v and initial_state, from those of out and final_state.  Forward-mode derivatives are refused.
     """
     refuse_tangents("linear_attention", q, k, v, log_decay, initial_state)
