@@ -364,10 +364,10 @@ int scan_launch(const LaLaunch& L, int elems, int reverse, const float* init, fl
 // they are independent of one another, a single head then spreads over dv / 32 SMs, and a row's part is a whole 128-byte line.
 // VEC = 4: a thread owns 4 columns of every THREADS / 8th row; VEC = 1 (odd widths or addresses): 1 column of every THREADS / 32nd.
 // Threads: as many as leave each four rows, all of them under way at once; a block for each 32 x 64 of a small state would be
-// half idle with 256 (256 sequences of 32 heads of 64: 62 us, and 48 with 128, 5.6 TB/s; heads of 128: 176 us, 6.1 TB/s).
+// half idle with 256 (256 sequences of 32 heads of 64: 62 us, and 47 with 128, 5.7 TB/s; heads of 128: 174 us, 6.2 TB/s).
 // WHOLE: a CTA takes all columns, its threads a few rows of them, which lie one behind the other; for widths that are no multiple of
 // 32, whose slices would share sectors and leave the last one half empty, where there are states enough for the GPU (256 sequences
-// of 32 heads of 100: 108 us, in slices 223; of 101: 156 and 249; with the decay as two floats 111 and 174, for one more operation
+// of 32 heads of 100: 109 us, in slices 223; of 101: 158 and 249; with the decay as two floats 109 and 175, for one more operation
 // for each element, which at one element a load is what bounds the kernel).
 constexpr int STEP_COLS = 32, STEP_MAX_DK = 1024;
 template <class E, int VEC, int STEP_THREADS, bool WHOLE>
@@ -378,7 +378,6 @@ __global__ void __launch_bounds__(STEP_THREADS) la_step_kernel(int H, int dk, in
   const int COLS = WHOLE ? dv : STEP_COLS, CG = COLS / VEC, ROWS = STEP_THREADS / CG;
   __shared__ float sq[STEP_MAX_DK], sk[STEP_MAX_DK];
   __shared__ float part[STEP_THREADS * VEC];  // [ROWS][COLS]
-  __shared__ float2 decay;  // as two floats: one float's rounding, the same at every token, would add up over a memory (LaFactor)
   const int tid = threadIdx.x, bh = blockIdx.x, h = bh % H, b = bh / H;
   const int cg = tid % CG, row = tid / CG, col = blockIdx.y * COLS + cg * VEC;
   if (active != nullptr && active[b] == 0) {
@@ -410,10 +409,9 @@ __global__ void __launch_bounds__(STEP_THREADS) la_step_kernel(int H, int dk, in
     sq[i] = up(qp[i]);
     sk[i] = up(kp[i]);
   }
-  if (tid == 0) {
-    const LaFactor f(log_decay[h], 1);
-    decay = make_float2(f.hi, f.lo);
-  }
+  // The decay as two floats: one float's rounding, the same at every token, would add up over a memory (LaFactor).  expm1 is as exact
+  // next to zero as exp is next to one, and hi - 1 has no rounding; below a half no memory is long enough.
+  const float l = log_decay[h], hi = expf(l), lo = hi >= 0.5f && hi <= 2.f ? expm1f(l) - (hi - 1.f) : 0.f;
   float vv[VEC], acc[VEC];
 #pragma unroll
   for (int e = 0; e < VEC; ++e) {
@@ -421,7 +419,6 @@ __global__ void __launch_bounds__(STEP_THREADS) la_step_kernel(int H, int dk, in
     acc[e] = 0.f;
   }
   __syncthreads();
-  const float2 g = decay;
   if (in) {
     for (int i0 = row; i0 < dk; i0 += AHEAD * ROWS) {
 #pragma unroll
@@ -431,7 +428,7 @@ __global__ void __launch_bounds__(STEP_THREADS) la_step_kernel(int H, int dk, in
         const float kk = sk[i], qq = sq[i];
 #pragma unroll
         for (int e = 0; e < VEC; ++e) {
-          s0[a][e] = fmaf(g.x, s0[a][e], fmaf(g.y, s0[a][e], kk * vv[e]));
+          s0[a][e] = fmaf(hi, s0[a][e], fmaf(lo, s0[a][e], kk * vv[e]));
           acc[e] = fmaf(qq, s0[a][e], acc[e]);
         }
         if constexpr (VEC == 4) *reinterpret_cast<float4*>(S + (size_t)i * dv) = make_float4(s0[a][0], s0[a][1], s0[a][2], s0[a][3]);
