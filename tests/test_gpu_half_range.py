@@ -76,11 +76,11 @@ def test_small_gradients(B, T, H, state, size, achieved):
 
 
 @pytest.mark.parametrize("B,H", [(1, 2), (4, 16)])
-@pytest.mark.parametrize("scale", [1e-6, 1.0, 300.0])
+@pytest.mark.parametrize("scale", [1e-6, 1.0, 300.0, -0.25])
 def test_any_scale(B, H, scale):
     """A scale takes part in scores and in gradients' keys; here its place is taken by the values' (and the gradients') size."""
     T, d = 300, 64
-    size = min(1.0, 0.1 / scale)
+    size = min(1.0, 0.1 / abs(scale))
     q, k, v = (_randn(B, T, H, d, seed=s, size=f).requires_grad_() for s, f in ((1, 1.0), (2, 1.0), (3, min(1.0, 10 * size))))
     d_out = _randn(B, T, H, d, seed=4, size=min(1.0, 10 * size))
     l = _decays(H)
@@ -132,3 +132,59 @@ def test_tokens_of_very_different_sizes(B, H, lengths):
     room = f_out * top + small
     assert ref.worst(out, want, room + U * (want.abs() + room) + ref.TINY[FP16]) <= 1.0
     assert ref.worst(final, want_s, f_state * top_s + 2.0 ** -37 * ka.amax() * va.sum(1)[:, :, None, :]) <= 1.0
+
+
+@pytest.mark.parametrize("B,T,H", [(1, 300, 2), (1, 5003, 1), (6, 300, 20)])
+def test_zeros(B, T, H):
+    """Nothing to scale by: a scale of zero, zero keys, zero queries, and a state that goes on beside them."""
+    q, k, v = (_randn(B, T, H, 64, seed=s) for s in (1, 2, 3))
+    s = _randn(B, H, 64, 64, seed=4, to=torch.float32)
+    l = _decays(H)
+    for scale, a, b in ((0.0, q, k), (1.0, q, torch.zeros_like(k)), (1.0, torch.zeros_like(q), k)):
+        leaves = [x.clone().requires_grad_() for x in (a, b, v)]
+        out, final = linear_attention(*leaves, l, scale=scale, initial_state=s)
+        want, want_s = ref.attend(a, b, v, l, scale, s)
+        if bool(want.any()):
+            assert _off(out, want) <= _room(want)
+        else:
+            assert not out.any()
+        # A state that has decayed below 2^-126 is a multiple of 2^-149 (e^-99, in the middle case): each of at most 40 chunks, and of as many
+        # segments, multiplies it by two numbers and rounds to one, by 2^-150 at most each time, and later factors are below one.
+        assert float((final.double() - want_s).norm()) <= STATE_ROOM * float(want_s.norm()) + 160 * 2.0 ** -150 * final.numel() ** 0.5
+        grads = ref.attend_grads(a, b, v, l, scale, s, None, v, None)
+        for x, y in zip(torch.autograd.grad(out, leaves, v), grads):
+            assert _off(x, y) <= _room(y) if bool(y.any()) else not x.any()
+
+
+@pytest.mark.parametrize("B,T,H", [(1, 300, 2), (1, 5003, 1), (6, 300, 20)])
+def test_two_streams_and_a_captured_call(B, T, H):
+    sets = [[_randn(B, T, H, 128, seed=10 * i + s, size=10.0 ** -i) for s in range(4)] for i in range(2)]
+    l = _decays(H)
+
+    def run(q, k, v, d):
+        leaves = [x.detach().requires_grad_() for x in (q, k, v)]
+        out, final = linear_attention(*leaves, l, scale=0.1)
+        return (out.detach(), final.detach(), *torch.autograd.grad(out, leaves, d))
+
+    want = [run(*x) for x in sets]
+    streams = [torch.cuda.Stream() for _ in sets]
+    torch.cuda.synchronize()
+    got = [[], []]
+    for _ in range(5):
+        for i, (x, st) in enumerate(zip(sets, streams)):
+            with torch.cuda.stream(st):
+                got[i].append(run(*x))
+    torch.cuda.synchronize()
+    for g, w in zip(got, want):
+        for one in g:
+            assert all(torch.equal(a, b) for a, b in zip(one, w))
+    held = [x.clone() for x in sets[0]]
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        got = run(*held)
+    for x, w in zip(sets[::-1], want[::-1]):
+        for a, b in zip(held, x):
+            a.copy_(b)
+        graph.replay()
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for a, b in zip(got, w))
