@@ -478,7 +478,7 @@ __device__ __forceinline__ void la_tc_block(const LtParams& A, const int ji, con
         have = n;
       }
       float keys_up = 1.f, keys_top = 0.f, rows_top = 0.f;
-      if constexpr (HALF) {  // each thread has read its row's weight: the weights may be of the chunk before, and are the same then
+      if constexpr (HALF) {
         const float top = row_top(kt, DI, n);
         const float3 all = largest(top * fabsf(key_weights32[r]), top, STATES ? 0.f : row_top(TILES * c + ROWS, DI, n));
         keys_up = below_2_15(all.x, 100);
@@ -494,7 +494,7 @@ __device__ __forceinline__ void la_tc_block(const LtParams& A, const int ji, con
       // in fp32, of bf16 products: z w - hi - lo, rounded
       auto remains = [](uint32_t z, f32x2 w32, E2 hi, E2 lo) { return pack2<E>(add2(fma2(wide(z), w32, wide(bits(__hneg2(hi)))), wide(bits(__hneg2(lo))))); };
       if (q * 32 < DI) {
-        // k w = hi + lo with w = w_hi + w_lo, all of the tensors' type: hi = k w_hi rounded, what that leaves is exact (half of the
+        // bf16: k w = hi + lo with w = w_hi + w_lo, all of the tensors' type: hi = k w_hi rounded, what that leaves is exact (half of the
         // product's bits), lo = k w_lo + that, rounded.  Three instructions for two elements, where the way through fp32 takes eight.
         const int row = half * 64 + (lane >> 4) * 8 + (lane & 7), in = (q & 1) * 32 + ((lane >> 3) & 1) * 8;  // matrices: two of tokens by two of columns
         const uint32_t from = k + (q >> 1) * TILE, to = tm + (STATES ? sum_keys(c) : TM_KEYS) + ((uint32_t)(q * 32) << 16) + half * 32;

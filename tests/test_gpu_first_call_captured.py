@@ -1,10 +1,13 @@
 """The first call a process makes of an operator may be one that is captured."""
+import os
 import subprocess
 import sys
 
 import pytest
 
 pytestmark = pytest.mark.gpu
+
+ROOT = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
 
 PROGRAM = """
 import torch
@@ -41,5 +44,5 @@ print("same")
 
 
 def test_without_a_call_before():
-    got = subprocess.run([sys.executable, "-c", PROGRAM], capture_output=True, text=True, timeout=300)
+    got = subprocess.run([sys.executable, "-c", PROGRAM], capture_output=True, text=True, timeout=300, cwd=ROOT)
     assert got.returncode == 0 and "same" in got.stdout, got.stderr[-2000:]
